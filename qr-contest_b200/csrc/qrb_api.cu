@@ -12,6 +12,7 @@
 // The batch is processed in chunks so that the float32 working set stays bounded.
 #include "../../include/qrb200.h"
 #include "qrb_common.cuh"
+#include "qrb_host.h"
 #include "qrb_gemm_simt.cuh"
 #include "qrb_panel.cuh"
 #include "qrb_panel_reg.cuh"
@@ -42,10 +43,12 @@ static std::atomic<long long> g_launches{0};
 static std::atomic<int> g_gemm_path{0};  // 0 auto, 1 SIMT only, 2 tcgen05 wherever legal
 static thread_local cudaError_t g_last_cuda_error = cudaSuccess;
 
-static inline cudaError_t note(cudaError_t e) {
+cudaError_t note(cudaError_t e) {
   if (e != cudaSuccess) g_last_cuda_error = e;
   return e;
 }
+
+void count_launches(int n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
 // Optional per-launch CUDA-event bracketing (only for the timed entry point).
 struct Prof {

@@ -1,0 +1,519 @@
+// qrb200 -- C ABI of the layer operators: the root-mean-square norm (qrb_norm.cuh) and the matrix
+// product with its epilogue (qrb_linear.cuh).  Every entry point checks its arguments before it
+// touches the GPU, enqueues on the caller's stream and returns a QRB200_* status.
+#include "../../include/qrb200_layer.h"
+#include "qrb_host.h"
+#include "qrb_linear.cuh"
+#include "qrb_norm.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace qrb {
+namespace {
+
+constexpr int kSMs = 148;
+
+bool float_type(int32_t t) { return t == QRB200_F32 || t == QRB200_BF16 || t == QRB200_F16; }
+int esize(int32_t t) { return t == QRB200_F32 ? 4 : (t == QRB200_E4M3 ? 1 : 2); }
+bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Rows of this base and stride (elements) all start on 16 bytes.
+bool rows_on16(const void* p, int64_t ld, int es) { return on16(p) && (ld * es & 15) == 0; }
+
+int launched() {
+  count_launches(1);
+  return note(cudaGetLastError()) == cudaSuccess ? QRB200_OK : QRB200_ERR_CUDA;
+}
+
+// Device memory for one call when the caller gives none; freed in stream order.
+struct Scratch {
+  void* p = nullptr;
+  cudaStream_t st;
+  bool own = false;
+  explicit Scratch(cudaStream_t s) : st(s) {}
+  int get(void* given, size_t given_bytes, size_t need) {
+    if (!need) return QRB200_OK;
+    if (given) {
+      if (given_bytes < need) return QRB200_ERR_WORKSPACE;
+      p = given;
+      return QRB200_OK;
+    }
+    if (note(cudaMallocAsync(&p, need, st)) != cudaSuccess) return QRB200_ERR_CUDA;
+    own = true;
+    return QRB200_OK;
+  }
+  ~Scratch() { if (own) cudaFreeAsync(p, st); }
+};
+
+// ------------------------------------------------------------------ norm
+// Threads of a row and vectors of 8 elements a thread.  Up to 1024 elements a warp takes the row
+// (4 rows a block).  Longer rows: with enough rows to fill the GPU, as many elements a thread as
+// registers allow (32: more bytes in flight, fewer barriers); with few rows, one vector a thread.
+struct Shape { int nt, vpt, rows; };
+Shape norm_shape(int64_t rows, int dim) {
+  const int vecs = (dim + 7) / 8;
+  if (dim <= 1024 && rows > kSMs) return {32, vecs <= 32 ? 1 : (vecs <= 64 ? 2 : 4), 4};
+  int vpt = 1;
+  if (rows > 2 * kSMs) vpt = vecs <= 128 ? 1 : (vecs <= 256 ? 2 : 4);
+  while ((vecs + vpt - 1) / vpt > norm::max_threads(vpt)) vpt *= 2;
+  const int nt = std::max(32, ((vecs + vpt - 1) / vpt + 31) / 32 * 32);
+  return {nt, vpt, 1};
+}
+
+template <typename TX, typename TR, bool Q8, bool NORM>
+int launch_fwd(const norm::FwdArgs& a, bool vec, cudaStream_t st) {
+  if (a.dim > norm::kRegDim) {
+    norm::fwd_long_kernel<TX, TR, Q8, NORM><<<(unsigned)a.rows, norm::kMaxThreads, 0, st>>>(a);
+    return launched();
+  }
+  const Shape s = norm_shape(a.rows, a.dim);
+  const dim3 block(s.nt, s.rows);
+  const unsigned grid = (unsigned)((a.rows + s.rows - 1) / s.rows);
+#define QRB_FWD(V, VEC) norm::fwd_kernel<TX, TR, Q8, NORM, V, VEC><<<grid, block, 0, st>>>(a)
+  if (vec) {
+    if (s.vpt == 1) QRB_FWD(1, true); else if (s.vpt == 2) QRB_FWD(2, true); else QRB_FWD(4, true);
+  } else {
+    if (s.vpt == 1) QRB_FWD(1, false); else if (s.vpt == 2) QRB_FWD(2, false); else QRB_FWD(4, false);
+  }
+#undef QRB_FWD
+  return launched();
+}
+
+template <typename TX, typename TR, bool NORM>
+int launch_fwd_out(const norm::FwdArgs& a, bool q8, bool vec, cudaStream_t st) {
+  return q8 ? launch_fwd<TX, TR, true, NORM>(a, vec, st) : launch_fwd<TX, TR, false, NORM>(a, vec, st);
+}
+
+template <typename TX, typename TR>
+int launch_bwd(const norm::BwdArgs& a, bool vec, int64_t grid, Shape s, cudaStream_t st) {
+  if (a.dim > norm::kRegDim) {
+    norm::bwd_long_kernel<TX, TR><<<(unsigned)grid, norm::kMaxThreads, 0, st>>>(a);
+    return launched();
+  }
+  const dim3 block(s.nt, s.rows);
+#define QRB_BWD(V, VEC) norm::bwd_kernel<TX, TR, V, VEC><<<(unsigned)grid, block, 0, st>>>(a)
+  if (vec) {
+    if (s.vpt == 1) QRB_BWD(1, true); else if (s.vpt == 2) QRB_BWD(2, true); else QRB_BWD(4, true);
+  } else {
+    if (s.vpt == 1) QRB_BWD(1, false); else if (s.vpt == 2) QRB_BWD(2, false); else QRB_BWD(4, false);
+  }
+#undef QRB_BWD
+  return launched();
+}
+
+// Shape and grid of the backward kernel; parts = rows of partial weight gradients it writes.
+// A block walks over its rows, so the grid is what the GPU holds at once.
+struct BwdPlan { Shape s; int64_t grid, parts; };
+BwdPlan bwd_plan(int64_t rows, int dim) {
+  BwdPlan p{};
+  if (dim > norm::kRegDim) {
+    p.s = {norm::kMaxThreads, 0, 1};
+    p.grid = p.parts = std::min<int64_t>(rows, 2 * kSMs);
+    return p;
+  }
+  const int vecs = (dim + 7) / 8;
+  if (dim <= 1024) {
+    p.s = {32, vecs <= 32 ? 1 : (vecs <= 64 ? 2 : 4), 4};
+    p.grid = std::min<int64_t>((rows + 3) / 4, 4 * kSMs);
+  } else {
+    const int vpt = vecs <= 256 ? 2 : 4;
+    const int nt = ((vecs + vpt - 1) / vpt + 31) / 32 * 32;
+    p.s = {nt, vpt, 1};
+    p.grid = std::min<int64_t>(rows, kSMs * std::max(1, 512 / nt));
+  }
+  p.parts = p.grid * p.s.rows;
+  return p;
+}
+
+template <typename T>
+int launch_colsum(const float* part, int64_t parts, int64_t cols, void* out, cudaStream_t st) {
+  norm::colsum_kernel<T><<<(unsigned)((cols + 31) / 32), dim3(32, 32), 0, st>>>(part, parts, cols, static_cast<T*>(out));
+  return launched();
+}
+int colsum(const float* part, int64_t parts, int64_t cols, void* out, int32_t dtype, cudaStream_t st) {
+  if (dtype == QRB200_F32) return launch_colsum<float>(part, parts, cols, out, st);
+  if (dtype == QRB200_BF16) return launch_colsum<__nv_bfloat16>(part, parts, cols, out, st);
+  return launch_colsum<__half>(part, parts, cols, out, st);
+}
+
+// ------------------------------------------------------------------ linear
+// An operand seen as rows x k: k-major (rows contiguous along k) or row-major.
+struct Operand {
+  const void* p;
+  int64_t ld;      // elements between the stored rows
+  bool row_major;
+  int64_t stored_rows(int64_t rows, int64_t k) const { return row_major ? k : rows; }
+  int64_t stored_cols(int64_t rows, int64_t k) const { return row_major ? rows : k; }
+};
+int64_t padded_cols(int64_t cols, int es) { return (cols * es + 15) / 16 * 16 / es; }
+bool addressable(const Operand& o, int es) { return rows_on16(o.p, o.ld, es); }
+size_t aligned_copy_bytes(const Operand& o, int64_t rows, int64_t k, int es) {
+  if (addressable(o, es)) return 0;
+  const size_t b = (size_t)o.stored_rows(rows, k) * padded_cols(o.stored_cols(rows, k), es) * es;
+  return (b + 255) & ~size_t(255);
+}
+// Copies an operand whose rows TMA cannot address to `buf` and points it there.
+int make_addressable(Operand& o, int64_t rows, int64_t k, int es, char*& buf, cudaStream_t st) {
+  const size_t bytes = aligned_copy_bytes(o, rows, k, es);
+  if (!bytes) return QRB200_OK;
+  const int64_t sr = o.stored_rows(rows, k), sc = o.stored_cols(rows, k), ldd = padded_cols(sc, es);
+  const int64_t vecs = sr * ldd * es / 16;
+  const unsigned grid = (unsigned)std::min<int64_t>((vecs + 255) / 256, kSMs * 8);
+  if (es == 2)
+    lin::align_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(o.p), o.ld, sc, reinterpret_cast<uint16_t*>(buf), ldd, sr);
+  else
+    lin::align_rows_kernel<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(o.p), o.ld, sc, reinterpret_cast<uint8_t*>(buf), ldd, sr);
+  o.p = buf;
+  o.ld = ldd;
+  buf += bytes;
+  return launched();
+}
+
+bool encode_operand(CUtensorMap* map, const Operand& o, int64_t rows, int64_t k, int32_t dtype, int box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  const int es = esize(dtype);
+  const CUtensorMapDataType t = dtype == QRB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                              : dtype == QRB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const cuuint64_t dims[2] = {(cuuint64_t)o.stored_cols(rows, k), (cuuint64_t)o.stored_rows(rows, k)};
+  const cuuint64_t strides[1] = {(cuuint64_t)o.ld * es};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)(o.row_major ? 64 : box_rows)};
+  const cuuint32_t one[2] = {1, 1};
+  return fn(map, t, 2, const_cast<void*>(o.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename Out, int ES, int T, bool SLOPE>
+int launch_tile(const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
+  auto kernel = lin::tile_kernel<Out, ES, T, SLOPE>;
+  using C = lin::TileCfg<T>;
+  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit has been raised
+  int dev = 0;
+  if (note(cudaGetDevice(&dev)) != cudaSuccess) return QRB200_ERR_CUDA;
+  if (!(ready.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+    if (note(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess)
+      return QRB200_ERR_CUDA;
+    ready.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
+  }
+  const int64_t tiles = (int64_t)((a.n + 127) / 128) * ((a.m + T - 1) / T);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(tiles * a.splits));
+  cfg.blockDim = dim3(lin::kTileThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)a.splits;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps, a);
+  count_launches(1);
+  if (note(e) != cudaSuccess) {
+    cudaGetLastError();
+    return QRB200_ERR_CUDA;
+  }
+  return QRB200_OK;
+}
+
+template <typename Out, int ES, bool SLOPE>
+int launch_tile_t(int T, const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
+  switch (T) {
+    case 16: return launch_tile<Out, ES, 16, SLOPE>(maps, a, st);
+    case 32: return launch_tile<Out, ES, 32, SLOPE>(maps, a, st);
+    case 64: return launch_tile<Out, ES, 64, SLOPE>(maps, a, st);
+    case 128: return launch_tile<Out, ES, 128, SLOPE>(maps, a, st);
+    default: return launch_tile<Out, ES, 256, SLOPE>(maps, a, st);
+  }
+}
+
+// D = epilogue(P Q^T); P is m x k, Q is n x k, both addressable by TMA.
+int product(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t out_dtype,
+            const lin::Epilogue& e, cudaStream_t st) {
+  lin::Args a{};
+  a.m = (int)m; a.n = (int)n; a.k = (int)k;
+  a.e = e;
+  a.es = esize(dtype);
+  a.p_row = P.row_major; a.q_row = Q.row_major;
+  auto on8 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; };
+  a.vec = on8(e.out) && e.ldo % 4 == 0 && (!e.bias || on8(e.bias)) &&
+          (!e.res || (on8(e.res) && e.ldr % 4 == 0)) && (!e.slope || (on8(e.slope) && n % 4 == 0));
+  // Few rows of P: the narrowest tile that holds them.  Otherwise 128 x 256 tiles where they fill
+  // the GPU, and 128 x 128 ones where only those do.
+  int T;
+  const int64_t tj = (n + 127) / 128;
+  if (m <= 16 && !P.row_major) T = 16;
+  else if (m <= 32 && !P.row_major) T = 32;
+  else if (m <= 64) T = 64;
+  else if (m <= 128 || tj * ((m + 255) / 256) < kSMs) T = 128;
+  else T = 256;
+  // Too few tiles for the GPU: a cluster shares each tile's sum, at least 4 blocks of k a CTA.
+  const int64_t tiles = tj * ((m + T - 1) / T), room = T == 256 ? kSMs : 2 * kSMs;
+  const int nkb = (int)((k * a.es + 127) / 128);
+  a.splits = 1;
+  while (a.splits < 8 && tiles * a.splits * 2 <= room && nkb / (a.splits * 2) >= 4) a.splits *= 2;
+  a.idesc = lin::idesc(dtype == QRB200_BF16 ? 1 : 0, a.q_row, a.p_row, lin::kTileQ, T);
+  lin::Maps maps{};
+  if (k > 0 && !(encode_operand(&maps.p, P, m, k, dtype, T) && encode_operand(&maps.q, Q, n, k, dtype, lin::kTileQ))) {
+    note(cudaErrorInvalidValue);
+    return QRB200_ERR_CUDA;
+  }
+  const bool bf = out_dtype == QRB200_BF16;
+  if (a.es == 1)
+    return bf ? launch_tile_t<__nv_bfloat16, 1, false>(T, maps, a, st) : launch_tile_t<__half, 1, false>(T, maps, a, st);
+  if (e.slope)
+    return bf ? launch_tile_t<__nv_bfloat16, 2, true>(T, maps, a, st) : launch_tile_t<__half, 2, true>(T, maps, a, st);
+  return bf ? launch_tile_t<__nv_bfloat16, 2, false>(T, maps, a, st) : launch_tile_t<__half, 2, false>(T, maps, a, st);
+}
+
+bool sizes_ok(int64_t m, int64_t n, int64_t k) {
+  constexpr int64_t top = (int64_t)1 << 31;
+  return m >= 0 && n >= 0 && k >= 0 && m < top - 256 && n < top - 256 && k < top - 256 &&
+         ((n + 127) / 128) * ((m + 15) / 16) * 8 < top;
+}
+
+// Blocks of dz_kernel along m, each of which leaves one part of the bias' sum: 8 blocks an SM.
+int64_t dz_parts(int64_t m, int64_t n) {
+  const int64_t strips = (n + 255) / 256;
+  return std::max<int64_t>(1, std::min<int64_t>((m + 7) / 8, std::max<int64_t>(1, 8 * kSMs / strips)));
+}
+
+template <typename T>
+int launch_dz(const void* dy, int64_t lddy, const int16_t* slope, void* dz, int64_t lddz, float* part, int64_t m,
+              int64_t n, int64_t parts, cudaStream_t st) {
+  const bool vec = n % 8 == 0 && rows_on16(dy, lddy, 2) && (!slope || on16(slope)) && (!dz || on16(dz));
+  const dim3 grid((unsigned)((n + 255) / 256), (unsigned)parts);
+  if (vec) lin::dz_kernel<T, true><<<grid, 256, 0, st>>>(static_cast<const T*>(dy), lddy, slope, static_cast<T*>(dz), lddz, part, m, n);
+  else lin::dz_kernel<T, false><<<grid, 256, 0, st>>>(static_cast<const T*>(dy), lddy, slope, static_cast<T*>(dz), lddz, part, m, n);
+  return launched();
+}
+
+struct BackwardPlan {
+  size_t dz, part, copies, total;
+  int64_t parts, lddz;
+};
+// Buffers of the backward pass: dz (when it is not dy itself), the bias sum's parts, and copies of
+// the operands TMA cannot address.
+BackwardPlan backward_plan(const void* dy, int64_t lddy, bool slope, const Operand& x, const Operand& w, bool dx,
+                           bool dw, bool db, int64_t m, int64_t n, int64_t k) {
+  BackwardPlan p{};
+  auto up = [](size_t b) { return (b + 255) & ~size_t(255); };
+  const bool products = dx || dw;
+  p.parts = dz_parts(m, n);
+  p.lddz = padded_cols(n, 2);
+  p.dz = slope && products ? up((size_t)m * p.lddz * 2) : 0;
+  p.part = db ? up((size_t)p.parts * n * 4) : 0;
+  if (products && !slope) p.copies += aligned_copy_bytes(Operand{dy, lddy, false}, m, n, 2);
+  if (dx) p.copies += aligned_copy_bytes(Operand{w.p, w.ld, !w.row_major}, k, n, 2);
+  if (dw) p.copies += aligned_copy_bytes(Operand{x.p, x.ld, true}, k, m, 2);
+  p.total = p.dz + p.part + p.copies;
+  return p;
+}
+
+}  // namespace
+}  // namespace qrb
+
+using namespace qrb;
+
+extern "C" {
+
+int qrb200_rms_norm(const void* x, int64_t ldx, const void* weight, int32_t weight_dtype, const void* residual,
+                    int64_t ldr, int32_t stream_dtype, void* y, float* scale, void* h, int64_t rows, int64_t dim,
+                    float eps, int32_t dtype, int32_t out_dtype, void* stream) {
+  const bool q8 = out_dtype == QRB200_E4M3;
+  if (!float_type(dtype) || !(q8 || out_dtype == dtype) || rows < 0 || dim < 0 || !(eps >= 0.f))
+    return QRB200_ERR_INVALID_ARG;
+  if (weight && !(weight_dtype == dtype || weight_dtype == QRB200_F32)) return QRB200_ERR_INVALID_ARG;
+  if (residual && !(stream_dtype == dtype || stream_dtype == QRB200_F32)) return QRB200_ERR_INVALID_ARG;
+  if (rows == 0 || dim == 0) return QRB200_OK;
+  if (!x || !y || (q8 && !scale) || (residual && !h)) return QRB200_ERR_INVALID_ARG;
+  if (rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30) || ldx < 0 || (residual && ldr < 0))
+    return QRB200_ERR_INVALID_ARG;
+  const int es = esize(dtype), rs = residual ? esize(stream_dtype) : es;
+  norm::FwdArgs a{x, ldx, residual, ldr, weight, weight && weight_dtype == QRB200_F32, y, scale, h, rows, (int)dim, eps};
+  const bool vec = dim % 8 == 0 && rows_on16(x, ldx, es) && on16(y) &&
+                   (!residual || (rows_on16(residual, ldr, rs) && on16(h))) && (!weight || on16(weight));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool wide = residual && stream_dtype == QRB200_F32;
+  if (dtype == QRB200_F32) return launch_fwd_out<float, float, true>(a, q8, vec, st);
+  if (dtype == QRB200_BF16)
+    return wide ? launch_fwd_out<__nv_bfloat16, float, true>(a, q8, vec, st)
+                : launch_fwd_out<__nv_bfloat16, __nv_bfloat16, true>(a, q8, vec, st);
+  return wide ? launch_fwd_out<__half, float, true>(a, q8, vec, st)
+              : launch_fwd_out<__half, __half, true>(a, q8, vec, st);
+}
+
+int qrb200_quantize_rows(const void* x, int64_t ldx, void* q, float* scale, int64_t rows, int64_t dim, int32_t dtype,
+                         void* stream) {
+  if (!float_type(dtype) || rows < 0 || dim < 0) return QRB200_ERR_INVALID_ARG;
+  if (rows == 0 || dim == 0) return QRB200_OK;
+  if (!x || !q || !scale || rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30) || ldx < 0)
+    return QRB200_ERR_INVALID_ARG;
+  norm::FwdArgs a{x, ldx, nullptr, 0, nullptr, 0, q, scale, nullptr, rows, (int)dim, 0.f};
+  const bool vec = dim % 8 == 0 && rows_on16(x, ldx, esize(dtype)) && on16(q);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == QRB200_F32) return launch_fwd<float, float, true, false>(a, vec, st);
+  if (dtype == QRB200_BF16) return launch_fwd<__nv_bfloat16, __nv_bfloat16, true, false>(a, vec, st);
+  return launch_fwd<__half, __half, true, false>(a, vec, st);
+}
+
+int qrb200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t dim, size_t* bytes) {
+  if (!bytes || rows < 0 || dim < 0 || rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30))
+    return QRB200_ERR_INVALID_ARG;
+  *bytes = rows && dim ? (size_t)bwd_plan(rows, (int)dim).parts * dim * sizeof(float) : 0;
+  return QRB200_OK;
+}
+
+int qrb200_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* dh, int64_t lddh,
+                             const void* weight, int32_t weight_dtype, void* dx, void* dresidual, void* dweight,
+                             int64_t rows, int64_t dim, float eps, int32_t dtype, int32_t stream_dtype,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  if (!float_type(dtype) || !(stream_dtype == dtype || stream_dtype == QRB200_F32) || rows < 0 || dim < 0 ||
+      !(eps >= 0.f))
+    return QRB200_ERR_INVALID_ARG;
+  if (weight && !(weight_dtype == dtype || weight_dtype == QRB200_F32)) return QRB200_ERR_INVALID_ARG;
+  if (dweight && !weight) return QRB200_ERR_INVALID_ARG;
+  if (dim == 0) return QRB200_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {
+    if (!dweight) return QRB200_OK;
+    return note(cudaMemsetAsync(dweight, 0, (size_t)dim * esize(weight_dtype), st)) == cudaSuccess ? QRB200_OK
+                                                                                                 : QRB200_ERR_CUDA;
+  }
+  if (!dy || !h || rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30) || lddy < 0 || ldh < 0 || (dh && lddh < 0))
+    return QRB200_ERR_INVALID_ARG;
+  const BwdPlan plan = bwd_plan(rows, (int)dim);
+  Scratch ws(st);
+  int rc = ws.get(workspace, workspace_bytes, dweight ? (size_t)plan.parts * dim * sizeof(float) : 0);
+  if (rc != QRB200_OK) return rc;
+  norm::BwdArgs a{dy, lddy, h, ldh, dh, lddh, weight, weight && weight_dtype == QRB200_F32, dx, dresidual,
+                  static_cast<float*>(ws.p), rows, (int)dim, eps};
+  const int es = esize(dtype), rs = esize(stream_dtype);
+  const bool vec = dim % 8 == 0 && rows_on16(dy, lddy, es) && rows_on16(h, ldh, rs) &&
+                   (!dh || rows_on16(dh, lddh, rs)) && (!dx || on16(dx)) && (!dresidual || on16(dresidual)) &&
+                   (!weight || on16(weight)) && (!a.part || on16(a.part));
+  const bool wide = stream_dtype == QRB200_F32 && dtype != QRB200_F32;
+  if (dtype == QRB200_F32) rc = launch_bwd<float, float>(a, vec, plan.grid, plan.s, st);
+  else if (dtype == QRB200_BF16)
+    rc = wide ? launch_bwd<__nv_bfloat16, float>(a, vec, plan.grid, plan.s, st)
+              : launch_bwd<__nv_bfloat16, __nv_bfloat16>(a, vec, plan.grid, plan.s, st);
+  else
+    rc = wide ? launch_bwd<__half, float>(a, vec, plan.grid, plan.s, st)
+              : launch_bwd<__half, __half>(a, vec, plan.grid, plan.s, st);
+  if (rc == QRB200_OK && dweight) rc = colsum(a.part, plan.parts, dim, dweight, weight_dtype, st);
+  return rc;
+}
+
+int qrb200_linear_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t w_transposed,
+                                  int64_t m, int64_t n, int64_t k, int32_t dtype, size_t* bytes) {
+  if (!bytes || !(dtype == QRB200_BF16 || dtype == QRB200_F16 || dtype == QRB200_E4M3) || !sizes_ok(m, n, k) ||
+      (dtype == QRB200_E4M3 && w_transposed))
+    return QRB200_ERR_INVALID_ARG;
+  const int es = esize(dtype);
+  *bytes = m && n && k ? aligned_copy_bytes(Operand{x, ldx, false}, m, k, es) +
+                             aligned_copy_bytes(Operand{w, ldw, w_transposed != 0}, n, k, es)
+                       : 0;
+  return QRB200_OK;
+}
+
+int qrb200_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t w_transposed, const float* x_scale,
+                  const float* w_scale, const void* bias, const void* residual, int64_t ldr, void* y, int64_t ldy,
+                  int16_t* slope, int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t out_dtype,
+                  int32_t activation, void* workspace, size_t workspace_bytes, void* stream) {
+  const bool q8 = dtype == QRB200_E4M3;
+  if (!(dtype == QRB200_BF16 || dtype == QRB200_F16 || q8) || !sizes_ok(m, n, k)) return QRB200_ERR_INVALID_ARG;
+  if (q8 ? !(out_dtype == QRB200_BF16 || out_dtype == QRB200_F16) : out_dtype != dtype) return QRB200_ERR_INVALID_ARG;
+  if (activation < 0 || activation >= lin::ACT_COUNT || (q8 && (w_transposed || slope))) return QRB200_ERR_INVALID_ARG;
+  if (m == 0 || n == 0) return QRB200_OK;
+  if (!y || (k > 0 && (!x || !w))) return QRB200_ERR_INVALID_ARG;
+  if (ldy < n || (residual && ldr < 0) || (k > 0 && (ldx < k || ldw < (w_transposed ? n : k))))
+    return QRB200_ERR_INVALID_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int es = esize(dtype);
+  Operand X{x, ldx, false}, W{w, ldw, w_transposed != 0};
+  Scratch ws(st);
+  int rc = ws.get(workspace, workspace_bytes,
+                  k ? aligned_copy_bytes(X, m, k, es) + aligned_copy_bytes(W, n, k, es) : 0);
+  char* buf = static_cast<char*>(ws.p);
+  if (rc == QRB200_OK && k) rc = make_addressable(X, m, k, es, buf, st);
+  if (rc == QRB200_OK && k) rc = make_addressable(W, n, k, es, buf, st);
+  if (rc != QRB200_OK) return rc;
+  lin::Epilogue e{x_scale, w_scale, bias, residual, ldr, y, ldy, slope, activation};
+  return product(X, W, m, n, k, dtype, out_dtype, e, st);
+}
+
+int qrb200_linear_backward_workspace_bytes(const void* dy, int64_t lddy, int32_t has_slope, const void* x, int64_t ldx,
+                                           const void* w, int64_t ldw, int32_t w_transposed, int32_t want_dx,
+                                           int32_t want_dw, int32_t want_dbias, int64_t m, int64_t n, int64_t k,
+                                           size_t* bytes) {
+  if (!bytes || !sizes_ok(m, n, k) || !sizes_ok(k, m, n)) return QRB200_ERR_INVALID_ARG;
+  *bytes = m && n ? backward_plan(dy, lddy, has_slope != 0, Operand{x, ldx, false}, Operand{w, ldw, w_transposed != 0},
+                                  want_dx && k, want_dw && k, want_dbias, m, n, k)
+                        .total
+                  : 0;
+  return QRB200_OK;
+}
+
+int qrb200_linear_backward(const void* dy, int64_t lddy, const int16_t* slope, const void* x, int64_t ldx,
+                           const void* w, int64_t ldw, int32_t w_transposed, void* dx, void* dw, void* dbias,
+                           int64_t m, int64_t n, int64_t k, int32_t dtype, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  if (!(dtype == QRB200_BF16 || dtype == QRB200_F16) || !sizes_ok(m, n, k) || !sizes_ok(k, m, n))
+    return QRB200_ERR_INVALID_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (m == 0 || n == 0) {  // sums over nothing
+    cudaError_t e = cudaSuccess;
+    if (dx && m * k) e = cudaMemsetAsync(dx, 0, (size_t)m * k * 2, st);
+    if (e == cudaSuccess && dw && n * k) e = cudaMemsetAsync(dw, 0, (size_t)n * k * 2, st);
+    if (e == cudaSuccess && dbias && n) e = cudaMemsetAsync(dbias, 0, (size_t)n * 2, st);
+    return note(e) == cudaSuccess ? QRB200_OK : QRB200_ERR_CUDA;
+  }
+  if (k == 0) dx = dw = nullptr;
+  if (!dx && !dw && !dbias) return QRB200_OK;
+  if (!dy || lddy < n || (dx && (!w || ldw < (w_transposed ? n : k))) || (dw && (!x || ldx < k)))
+    return QRB200_ERR_INVALID_ARG;
+  const Operand X{x, ldx, false}, W{w, ldw, w_transposed != 0};
+  const BackwardPlan p = backward_plan(dy, lddy, slope != nullptr, X, W, dx, dw, dbias, m, n, k);
+  Scratch ws(st);
+  int rc = ws.get(workspace, workspace_bytes, p.total);
+  if (rc != QRB200_OK) return rc;
+  char* buf = static_cast<char*>(ws.p);
+  void* dz = p.dz ? buf : nullptr;
+  buf += p.dz;
+  float* part = p.part ? reinterpret_cast<float*>(buf) : nullptr;
+  buf += p.part;
+  if (dz || part) {
+    rc = dtype == QRB200_BF16 ? launch_dz<__nv_bfloat16>(dy, lddy, slope, dz, p.lddz, part, m, n, p.parts, st)
+                              : launch_dz<__half>(dy, lddy, slope, dz, p.lddz, part, m, n, p.parts, st);
+    if (rc == QRB200_OK && dbias) rc = colsum(part, p.parts, n, dbias, dtype, st);
+    if (rc != QRB200_OK) return rc;
+  }
+  if (!dx && !dw) return QRB200_OK;
+  Operand G = dz ? Operand{dz, p.lddz, false} : Operand{dy, lddy, false};
+  rc = make_addressable(G, m, n, 2, buf, st);
+  if (rc == QRB200_OK && dx) {  // dx_ik = sum_j dz_ij W_jk
+    Operand Wt{w, ldw, !W.row_major};
+    rc = make_addressable(Wt, k, n, 2, buf, st);
+    lin::Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dx, k, nullptr, lin::ACT_NONE};
+    if (rc == QRB200_OK) rc = product(G, Wt, m, k, n, dtype, dtype, e, st);
+  }
+  if (rc == QRB200_OK && dw) {  // dW_jk = sum_i dz_ij x_ik
+    Operand Xt{x, ldx, true};
+    rc = make_addressable(Xt, k, m, 2, buf, st);
+    lin::Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dw, k, nullptr, lin::ACT_NONE};
+    if (rc == QRB200_OK) rc = product(Operand{G.p, G.ld, true}, Xt, n, k, m, dtype, dtype, e, st);
+  }
+  return rc;
+}
+
+int qrb200_layer_status(int32_t* timed_out) {
+  if (!timed_out) return QRB200_ERR_INVALID_ARG;
+  int v = 0, zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, lin::g_timeout, sizeof(v));
+  if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(lin::g_timeout, &zero, sizeof(zero));
+  *timed_out = v;
+  return note(e) == cudaSuccess ? QRB200_OK : QRB200_ERR_CUDA;
+}
+
+}  // extern "C"

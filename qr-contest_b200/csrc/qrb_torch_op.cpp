@@ -1,6 +1,7 @@
-// qrb200 -- PyTorch operator registration: torch.ops.qrb200.geqrf(A) -> (H, tau, info).
+// qrb200 -- PyTorch operator registration: torch.ops.qrb200.geqrf(A) -> (H, tau, info), and the
+// layer operators (rms_norm, quantize_rows, linear and their backward passes).
 //
-// The operator form of the reference entry point custom_kernel(data) -> (H, tau)
+// geqrf is the operator form of the reference entry point custom_kernel(data) -> (H, tau)
 // (reflection_no_reflectors.py:181-196) for callers that dispatch through the torch operator
 // registry (torch.ops, TorchScript, torch.compile graphs).  It is a thin layer over the C ABI of
 // libqrb200.so (include/qrb200.h): no kernel lives here.
@@ -11,12 +12,17 @@
 //   * Enqueued on the current CUDA stream of A's device; the workspace comes from torch's
 //     caching allocator.  A bad argument or a CUDA error raises (TORCH_CHECK).
 // A Meta kernel gives shapes and dtypes without running anything.
+//
+// The layer operators take rows in place where one row stride describes them (any leading shape,
+// slices and expanded tensors included) and copy otherwise; a wrong argument raises ValueError or
+// TypeError before anything is allocated.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
 #include "qrb200.h"
+#include "qrb200_layer.h"
 
 namespace {
 
@@ -80,12 +86,296 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> geqrf_meta(const at::Tensor& data
           at::empty(lead, data.options().dtype(at::kInt))};
 }
 
+// ---------------------------------------------------------------- layer operators
+using OptTensor = c10::optional<at::Tensor>;
+
+int32_t layer_code(at::ScalarType t) {
+  return t == at::kFloat8_e4m3fn ? QRB200_E4M3 : dtype_code(t);
+}
+
+void check_rc(int rc, const char* where) {
+  TORCH_CHECK(rc == QRB200_OK, where, ": ", qrb200_status_string(rc), " (status ", rc, ")",
+              rc == QRB200_ERR_CUDA ? ": " : "", rc == QRB200_ERR_CUDA ? qrb200_last_cuda_error() : "");
+}
+
+void check_device(const at::Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(x.is_cuda() || x.is_meta(), "qrb200: ", name, " must be a CUDA tensor (got one on ", x.device(), ")");
+}
+void check_with(const at::Tensor& t, const at::Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(t.device() == x.device(), "qrb200: ", name, " is on ", t.device(), ", the input on ", x.device());
+}
+void check_type(bool ok, const char* name, at::ScalarType t) {
+  TORCH_CHECK_TYPE(ok, "qrb200: ", name, " cannot be of type ", t);
+}
+
+// A tensor (..., d) as rows of d contiguous elements, `ld` apart: itself where one stride describes
+// it, a contiguous copy otherwise.  apart: rows may not overlap (matrix-product operands).
+struct Rows {
+  at::Tensor t;
+  int64_t rows, d, ld;
+};
+Rows as_rows(const at::Tensor& x, bool apart = false) {
+  Rows r{x, 1, x.size(-1), x.size(-1)};
+  for (int64_t i = 0; i < x.dim() - 1; ++i) r.rows *= x.size(i);
+  if (r.rows == 0 || r.d == 0 || x.is_meta()) return r;
+  bool fits = r.d == 1 || x.stride(-1) == 1;
+  int64_t next = -1;  // the stride the next outer dimension must have
+  for (int64_t i = x.dim() - 2; fits && i >= 0; --i) {
+    if (x.size(i) == 1) continue;
+    if (next < 0) r.ld = x.stride(i);
+    else fits = x.stride(i) == next;
+    next = x.stride(i) * x.size(i);
+  }
+  if (!fits || (apart && r.rows > 1 && r.ld < r.d)) {
+    r.t = x.contiguous();
+    r.ld = r.d;
+  }
+  return r;
+}
+std::vector<int64_t> with_last(const at::Tensor& x, int64_t d) {
+  std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
+  s.back() = d;
+  return s;
+}
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* cur_stream(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+// The norm's weight: (d), contiguous, in x's type or float32.
+at::Tensor norm_weight(const OptTensor& weight, const at::Tensor& x, at::ScalarType xt) {
+  if (!weight) return {};
+  check_with(*weight, x, "weight");
+  TORCH_CHECK_VALUE(weight->dim() == 1 && weight->size(0) == x.size(-1), "qrb200: weight must have shape (", x.size(-1),
+                    "), got ", weight->sizes());
+  check_type(weight->scalar_type() == xt || weight->scalar_type() == at::kFloat, "weight", weight->scalar_type());
+  return weight->contiguous();
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm(const at::Tensor& x, const OptTensor& weight,
+                                                        const OptTensor& residual, double eps,
+                                                        c10::optional<at::ScalarType> out_dtype) {
+  check_device(x, "x");
+  TORCH_CHECK_VALUE(x.dim() >= 1, "qrb200: rms_norm takes a (..., d) tensor");
+  const auto xt = x.scalar_type();
+  check_type(native(xt), "x", xt);
+  const auto ot = out_dtype.value_or(xt);
+  check_type(ot == xt || ot == at::kFloat8_e4m3fn, "the output", ot);
+  TORCH_CHECK_VALUE(eps >= 0, "qrb200: eps must not be negative");
+  const at::Tensor w = norm_weight(weight, x, xt);
+  if (residual) {
+    check_with(*residual, x, "residual");
+    TORCH_CHECK_VALUE(residual->sizes() == x.sizes(), "qrb200: residual must have x's shape ", x.sizes(), ", got ", residual->sizes());
+    check_type(residual->scalar_type() == xt || residual->scalar_type() == at::kFloat, "residual", residual->scalar_type());
+  }
+  const c10::OptionalDeviceGuard guard(x.is_cuda() ? c10::optional<c10::Device>(x.device()) : c10::nullopt);
+  const Rows rx = as_rows(x), rr = residual ? as_rows(*residual) : Rows{{}, 0, 0, 0};
+  at::Tensor y = at::empty(x.sizes(), x.options().dtype(ot)), scale, h;
+  if (ot == at::kFloat8_e4m3fn) scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  if (residual) h = at::empty(x.sizes(), residual->options());
+  if (x.is_meta()) return {y, scale, h};
+  check_rc(qrb200_rms_norm(rx.t.data_ptr(), rx.ld, ptr(w), w.defined() ? layer_code(w.scalar_type()) : 0, ptr(rr.t), rr.ld,
+                           residual ? layer_code(residual->scalar_type()) : 0, y.data_ptr(),
+                           static_cast<float*>(ptr(scale)), ptr(h), rx.rows, rx.d, (float)eps, layer_code(xt),
+                           layer_code(ot), cur_stream(x)),
+           "qrb200_rms_norm");
+  return {y, scale, h};
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x) {
+  check_device(x, "x");
+  TORCH_CHECK_VALUE(x.dim() >= 1, "qrb200: quantize_rows takes a (..., d) tensor");
+  check_type(native(x.scalar_type()), "x", x.scalar_type());
+  const c10::OptionalDeviceGuard guard(x.is_cuda() ? c10::optional<c10::Device>(x.device()) : c10::nullopt);
+  const Rows r = as_rows(x);
+  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  if (x.is_meta()) return {q, scale};
+  check_rc(qrb200_quantize_rows(r.t.data_ptr(), r.ld, q.data_ptr(), scale.data_ptr<float>(), r.rows, r.d,
+                                layer_code(x.scalar_type()), cur_stream(x)),
+           "qrb200_quantize_rows");
+  return {q, scale};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_backward(const at::Tensor& dy, const at::Tensor& h,
+                                                                 const OptTensor& dh, const OptTensor& weight,
+                                                                 double eps, bool want_dx, bool want_dresidual,
+                                                                 bool want_dweight) {
+  check_device(dy, "dy");
+  const auto xt = dy.scalar_type(), ht = h.scalar_type();
+  check_type(native(xt), "dy", xt);
+  check_type(ht == xt || ht == at::kFloat, "h", ht);
+  check_with(h, dy, "h");
+  TORCH_CHECK_VALUE(dy.dim() >= 1 && h.sizes() == dy.sizes(), "qrb200: h must have dy's shape");
+  TORCH_CHECK_VALUE(eps >= 0, "qrb200: eps must not be negative");
+  if (dh) {
+    check_with(*dh, dy, "dh");
+    check_type(dh->scalar_type() == ht, "dh", dh->scalar_type());
+    TORCH_CHECK_VALUE(dh->sizes() == dy.sizes(), "qrb200: dh must have dy's shape");
+  }
+  const at::Tensor w = norm_weight(weight, dy, xt);
+  TORCH_CHECK_VALUE(!want_dweight || w.defined(), "qrb200: a weight's gradient needs the weight");
+  const c10::OptionalDeviceGuard guard(dy.is_cuda() ? c10::optional<c10::Device>(dy.device()) : c10::nullopt);
+  const Rows rg = as_rows(dy), rh = as_rows(h), rd = dh ? as_rows(*dh) : Rows{{}, 0, 0, 0};
+  at::Tensor dx, dres, dw;
+  if (want_dx || (want_dresidual && ht == xt)) dx = at::empty(dy.sizes(), dy.options());
+  if (want_dresidual) dres = ht == xt ? dx : at::empty(dy.sizes(), h.options());
+  if (want_dweight) dw = at::empty(w.sizes(), w.options());
+  if (dy.is_meta()) return {dx, dres, dw};
+  size_t bytes = 0;
+  if (want_dweight) check_rc(qrb200_rms_norm_backward_workspace_bytes(rg.rows, rg.d, &bytes), "qrb200_rms_norm_backward_workspace_bytes");
+  at::Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, dy.options().dtype(at::kByte));
+  check_rc(qrb200_rms_norm_backward(rg.t.data_ptr(), rg.ld, rh.t.data_ptr(), rh.ld, ptr(rd.t), rd.ld, ptr(w),
+                                    w.defined() ? layer_code(w.scalar_type()) : 0, ptr(dx), ht == xt ? nullptr : ptr(dres),
+                                    ptr(dw), rg.rows, rg.d, (float)eps, layer_code(xt), layer_code(ht), ptr(ws), bytes,
+                                    cur_stream(dy)),
+           "qrb200_rms_norm_backward");
+  return {dx, dres, dw};
+}
+
+// The product's weight (n, k): rows in place, or columns (a transposed view) for 16-bit types.
+struct Weight {
+  at::Tensor t;
+  int64_t ld;
+  int32_t transposed;
+};
+Weight as_weight(const at::Tensor& w, bool may_transpose) {
+  if (w.is_meta() || w.numel() == 0) return {w, w.size(1), 0};
+  const int64_t n = w.size(0), k = w.size(1);
+  if ((k == 1 || w.stride(1) == 1) && (n == 1 || w.stride(0) >= k)) return {w, n == 1 ? k : w.stride(0), 0};
+  if (may_transpose && (n == 1 || w.stride(0) == 1) && (k == 1 || w.stride(1) >= n)) return {w, k == 1 ? n : w.stride(1), 1};
+  return {w.contiguous(), k, 0};
+}
+// Scales of the rows of an 8-bit operand: one each, or one for all.
+at::Tensor row_scales(const OptTensor& s, const at::Tensor& x, int64_t rows, const char* name) {
+  if (!s) return {};
+  check_with(*s, x, name);
+  check_type(s->scalar_type() == at::kFloat, name, s->scalar_type());
+  TORCH_CHECK_VALUE(s->numel() == rows || s->numel() == 1, "qrb200: ", name, " must hold one scale or ", rows, ", got ", s->numel());
+  return s->reshape({-1}).expand({rows}).contiguous();
+}
+
+std::tuple<at::Tensor, at::Tensor> linear(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
+                                          const OptTensor& residual, int64_t activation, const OptTensor& x_scale,
+                                          const OptTensor& weight_scale, c10::optional<at::ScalarType> out_dtype,
+                                          bool want_slope) {
+  check_device(x, "x");
+  const auto xt = x.scalar_type();
+  const bool q8 = xt == at::kFloat8_e4m3fn;
+  check_type(xt == at::kBFloat16 || xt == at::kHalf || q8, "x", xt);
+  check_type(weight.scalar_type() == xt, "weight", weight.scalar_type());
+  check_with(weight, x, "weight");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1),
+                    "qrb200: linear takes x (..., k) and weight (n, k), got ", x.sizes(), " and ", weight.sizes());
+  const auto ot = out_dtype.value_or(q8 ? at::kBFloat16 : xt);
+  check_type(q8 ? (ot == at::kBFloat16 || ot == at::kHalf) : ot == xt, "the output", ot);
+  TORCH_CHECK_VALUE(activation >= QRB200_ACT_NONE && activation <= QRB200_ACT_SILU, "qrb200: unknown activation ", activation);
+  TORCH_CHECK_VALUE(q8 || (!x_scale && !weight_scale), "qrb200: scales belong to 8-bit operands");
+  TORCH_CHECK_VALUE(!(q8 && want_slope), "qrb200: the 8-bit product has no gradient");
+  const int64_t n = weight.size(0), k = weight.size(1);
+  const auto shape = with_last(x, n);
+  if (bias) {
+    check_with(*bias, x, "bias");
+    check_type(bias->scalar_type() == ot, "bias", bias->scalar_type());
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == n, "qrb200: bias must have shape (", n, "), got ", bias->sizes());
+  }
+  if (residual) {
+    check_with(*residual, x, "residual");
+    check_type(residual->scalar_type() == ot, "residual", residual->scalar_type());
+    TORCH_CHECK_VALUE(residual->sizes() == at::IntArrayRef(shape), "qrb200: residual must have the output's shape ", at::IntArrayRef(shape), ", got ", residual->sizes());
+  }
+  const c10::OptionalDeviceGuard guard(x.is_cuda() ? c10::optional<c10::Device>(x.device()) : c10::nullopt);
+  const Rows rx = as_rows(x, true), rr = residual ? as_rows(*residual) : Rows{{}, 0, 0, 0};
+  const Weight w = as_weight(weight, !q8);
+  const at::Tensor b = bias ? bias->contiguous() : at::Tensor();
+  const at::Tensor xs = row_scales(x_scale, x, rx.rows, "x_scale"), wsc = row_scales(weight_scale, x, n, "weight_scale");
+  at::Tensor y = at::empty(shape, x.options().dtype(ot)), slope;
+  if (want_slope) slope = at::empty(shape, x.options().dtype(at::kShort));
+  if (x.is_meta()) return {y, slope};
+  size_t bytes = 0;
+  check_rc(qrb200_linear_workspace_bytes(rx.t.data_ptr(), rx.ld, w.t.data_ptr(), w.ld, w.transposed, rx.rows, n, k, layer_code(xt), &bytes),
+           "qrb200_linear_workspace_bytes");
+  at::Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+  check_rc(qrb200_linear(rx.t.data_ptr(), rx.ld, w.t.data_ptr(), w.ld, w.transposed, static_cast<const float*>(ptr(xs)),
+                         static_cast<const float*>(ptr(wsc)), ptr(b), ptr(rr.t), rr.ld, y.data_ptr(), n,
+                         static_cast<int16_t*>(ptr(slope)), rx.rows, n, k, layer_code(xt), layer_code(ot), (int32_t)activation,
+                         ptr(ws), bytes, cur_stream(x)),
+           "qrb200_linear");
+  return {y, slope};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward(const at::Tensor& dy, const OptTensor& slope,
+                                                               const at::Tensor& x, const at::Tensor& weight, bool want_dx,
+                                                               bool want_dweight, bool want_dbias) {
+  check_device(dy, "dy");
+  const auto t = dy.scalar_type();
+  check_type(t == at::kBFloat16 || t == at::kHalf, "dy", t);
+  check_type(x.scalar_type() == t, "x", x.scalar_type());
+  check_type(weight.scalar_type() == t, "weight", weight.scalar_type());
+  check_with(x, dy, "x");
+  check_with(weight, dy, "weight");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1), "qrb200: linear_backward takes x (..., k) and weight (n, k)");
+  const int64_t n = weight.size(0), k = weight.size(1);
+  const auto shape = with_last(x, n);
+  TORCH_CHECK_VALUE(dy.sizes() == at::IntArrayRef(shape), "qrb200: dy must have shape ", at::IntArrayRef(shape), ", got ", dy.sizes());
+  if (slope) {
+    check_with(*slope, dy, "slope");
+    check_type(slope->scalar_type() == at::kShort, "slope", slope->scalar_type());
+    TORCH_CHECK_VALUE(slope->sizes() == dy.sizes() && slope->is_contiguous(), "qrb200: slope must be contiguous, in dy's shape");
+  }
+  const c10::OptionalDeviceGuard guard(dy.is_cuda() ? c10::optional<c10::Device>(dy.device()) : c10::nullopt);
+  const Rows rg = as_rows(dy, true), rx = as_rows(x, true);
+  const Weight w = as_weight(weight, true);
+  at::Tensor dx, dw, db;
+  if (want_dx) dx = at::empty(x.sizes(), x.options());
+  if (want_dweight) dw = at::empty(weight.sizes(), weight.options());
+  if (want_dbias) db = at::empty({n}, dy.options());
+  if (dy.is_meta()) return {dx, dw, db};
+  size_t bytes = 0;
+  check_rc(qrb200_linear_backward_workspace_bytes(rg.t.data_ptr(), rg.ld, slope.has_value(), rx.t.data_ptr(), rx.ld, w.t.data_ptr(),
+                                                  w.ld, w.transposed, want_dx, want_dweight, want_dbias, rg.rows, n, k, &bytes),
+           "qrb200_linear_backward_workspace_bytes");
+  at::Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, dy.options().dtype(at::kByte));
+  check_rc(qrb200_linear_backward(rg.t.data_ptr(), rg.ld, slope ? static_cast<const int16_t*>(slope->data_ptr()) : nullptr,
+                                  rx.t.data_ptr(), rx.ld, w.t.data_ptr(), w.ld, w.transposed, ptr(dx), ptr(dw), ptr(db),
+                                  rg.rows, n, k, layer_code(t), ptr(ws), bytes, cur_stream(dy)),
+           "qrb200_linear_backward");
+  return {dx, dw, db};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(qrb200, m) {
   m.def("geqrf(Tensor A) -> (Tensor H, Tensor tau, Tensor info)");
+  m.def("rms_norm(Tensor x, Tensor? weight, Tensor? residual, float eps, ScalarType? out_dtype) -> (Tensor y, Tensor scale, Tensor h)");
+  m.def("rms_norm_backward(Tensor dy, Tensor h, Tensor? dh, Tensor? weight, float eps, bool want_dx, bool want_dresidual, bool want_dweight) -> (Tensor dx, Tensor dresidual, Tensor dweight)");
+  m.def("quantize_rows(Tensor x) -> (Tensor q, Tensor scale)");
+  m.def("linear(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int activation, Tensor? x_scale, Tensor? weight_scale, ScalarType? out_dtype, bool want_slope) -> (Tensor y, Tensor slope)");
+  m.def("linear_backward(Tensor dy, Tensor? slope, Tensor x, Tensor weight, bool want_dx, bool want_dweight, bool want_dbias) -> (Tensor dx, Tensor dweight, Tensor dbias)");
 }
 
-TORCH_LIBRARY_IMPL(qrb200, CUDA, m) { m.impl("geqrf", geqrf_cuda); }
+namespace {
+// A layer operator's function serves both keys: on meta tensors it returns before it runs anything.
+void layer_impls(torch::Library& m) {
+  m.impl("rms_norm", rms_norm);
+  m.impl("rms_norm_backward", rms_norm_backward);
+  m.impl("quantize_rows", quantize_rows);
+  m.impl("linear", linear);
+  m.impl("linear_backward", linear_backward);
+}
+}  // namespace
 
-TORCH_LIBRARY_IMPL(qrb200, Meta, m) { m.impl("geqrf", geqrf_meta); }
+TORCH_LIBRARY_IMPL(qrb200, CUDA, m) {
+  m.impl("geqrf", geqrf_cuda);
+  layer_impls(m);
+}
+
+TORCH_LIBRARY_IMPL(qrb200, Meta, m) {
+  m.impl("geqrf", geqrf_meta);
+  layer_impls(m);
+}
+
+// Host tensors (and mixes of host and device tensors, which reach this key too) are refused by the
+// functions themselves.
+TORCH_LIBRARY_IMPL(qrb200, CPU, m) { layer_impls(m); }

@@ -1,4 +1,5 @@
-"""ctypes binding of ``libqrb200.so`` (the C ABI declared in ``include/qrb200.h``).
+"""ctypes binding of ``libqrb200.so`` (the C ABI declared in ``include/qrb200.h`` and
+``include/qrb200_layer.h``).
 
 The shared library is built in-tree (``qrb200/build.py``).  Loading it needs no GPU;
 calling the compute entry point does.  There is no fallback: if the library is missing
@@ -25,7 +26,10 @@ NOALLOC_SCRATCH_BYTES = 64 << 20
 NOALLOC_MAX_N_DEFAULT = 1826
 NOALLOC_MAX_N4_DEFAULT = 1792
 
-QRB200_F32, QRB200_BF16, QRB200_F16 = 0, 1, 2
+QRB200_F32, QRB200_BF16, QRB200_F16, QRB200_E4M3 = 0, 1, 2, 3
+
+# activations of qrb200_linear
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = 0, 1, 2, 3, 4
 
 INFO_NONFINITE_INPUT = 1
 INFO_CHOL1_NOT_PD = 2
@@ -43,8 +47,30 @@ OPT_PANEL_LOOP = 6
 OPT_CLOSURE_DUAL_N = 7
 GEMM_AUTO, GEMM_SIMT, GEMM_TC = 0, 1, 2
 
-# every symbol include/qrb200.h declares, with its ctypes signature
+_P, _I64, _I32, _SZ, _F32 = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t,
+                            ctypes.c_float)
+_SZP = ctypes.POINTER(ctypes.c_size_t)
+
+# every symbol include/*.h declares, with its ctypes signature
 SIGNATURES = {
+    # layer operators
+    "qrb200_rms_norm": (ctypes.c_int, [_P, _I64, _P, _I32, _P, _I64, _I32, _P, _P, _P, _I64, _I64,
+                                       _F32, _I32, _I32, _P]),
+    "qrb200_quantize_rows": (ctypes.c_int, [_P, _I64, _P, _P, _I64, _I64, _I32, _P]),
+    "qrb200_rms_norm_backward_workspace_bytes": (ctypes.c_int, [_I64, _I64, _SZP]),
+    "qrb200_rms_norm_backward": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I32, _P, _P, _P,
+                                                _I64, _I64, _F32, _I32, _I32, _P, _SZ, _P]),
+    "qrb200_linear_workspace_bytes": (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _I64, _I64, _I64,
+                                                     _I32, _SZP]),
+    "qrb200_linear": (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _P, _P, _P, _P, _I64, _P, _I64, _P,
+                                     _I64, _I64, _I64, _I32, _I32, _I32, _P, _SZ, _P]),
+    "qrb200_linear_backward_workspace_bytes": (ctypes.c_int, [_P, _I64, _I32, _P, _I64, _P, _I64,
+                                                              _I32, _I32, _I32, _I32, _I64, _I64,
+                                                              _I64, _SZP]),
+    "qrb200_linear_backward": (ctypes.c_int, [_P, _I64, _P, _P, _I64, _P, _I64, _I32, _P, _P, _P,
+                                              _I64, _I64, _I64, _I32, _P, _SZ, _P]),
+    "qrb200_layer_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int32)]),
+    # factorization
     "qrb200_version": (ctypes.c_int, []),
     "qrb200_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "qrb200_max_n": (ctypes.c_int32, []),
@@ -197,3 +223,13 @@ def set_closure_dual_n(n_max: int) -> None:
     rc = lib().qrb200_set_option(OPT_CLOSURE_DUAL_N, int(n_max))
     if rc != 0:
         raise QRB200Error(rc, "qrb200_set_option")
+
+
+def layer_timed_out() -> bool:
+    """Whether a bounded wait of a layer operator has run out on the current device since the last
+    call (its outputs are NaN then).  Synchronises."""
+    v = ctypes.c_int32(0)
+    rc = lib().qrb200_layer_status(ctypes.byref(v))
+    if rc != QRB200_OK:
+        raise QRB200Error(rc, "qrb200_layer_status")
+    return bool(v.value)

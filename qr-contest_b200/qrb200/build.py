@@ -2,7 +2,8 @@
 
     python -m qrb200.build            (from the qr-contest_b200 directory)
 
-The library has no PyTorch dependency: plain ``nvcc -shared`` of ``csrc/qrb_api.cu`` with
+The library has no PyTorch dependency: ``csrc/qrb_api.cu`` (the factorization) and
+``csrc/qrb_layer.cu`` (the layer operators) are compiled to objects side by side and linked with
 the CUDA runtime linked statically.
 """
 from __future__ import annotations
@@ -22,7 +23,7 @@ TESTKIT = PKG / "libqrb200_testkit.so"   # single-stage entry points for the GPU
 CHECKED = PKG / "libqrb200_checked.so"   # the library with the pivot-map bounds checks
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
+FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
          "--expt-relaxed-constexpr", "-Xptxas", "-O3"]
 
 
@@ -33,20 +34,40 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def sources():
-    return (sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.cpp"))
-            + sorted(INCLUDE.glob("*.h")))
-
-
-def up_to_date(target: Path) -> bool:
+def up_to_date(target: Path, inputs) -> bool:
     if not target.exists():
         return False
     t = target.stat().st_mtime
-    return all(p.stat().st_mtime <= t for p in sources())
+    return all(p.exists() and p.stat().st_mtime <= t for p in inputs)
 
 
-def _compile(src: Path, out: Path, verbose: bool, extra) -> None:
-    cmd = [nvcc(), *ARCH, *FLAGS, *extra, "-I", str(INCLUDE), "-o", str(out), str(src)]
+OBJ = ROOT / "build"                   # objects and their dependency files (git-ignored)
+
+
+def _object(src: Path, defs) -> Path:
+    return OBJ / (src.stem + "".join(d.replace("-D", "-") for d in defs) + ".o")
+
+
+def _inputs(obj: Path):
+    """The files an object was compiled from, as nvcc listed them (none: never compiled)."""
+    dep = obj.with_suffix(".d")
+    if not dep.exists():
+        return None
+    files = dep.read_text().replace("\\\n", " ").split(":", 1)[1].split()
+    return [Path(f) for f in files if not f.startswith(("/usr", "/opt"))]
+
+
+def _compile(src: Path, obj: Path, verbose: bool, extra) -> None:
+    OBJ.mkdir(exist_ok=True)
+    cmd = [nvcc(), *ARCH, *FLAGS, *extra, "-I", str(INCLUDE), "-MD", "-MF",
+           str(obj.with_suffix(".d")), "-c", "-o", str(obj), str(src)]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+
+
+def _link(objs, out: Path, verbose: bool) -> None:
+    cmd = [nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", str(out), *map(str, objs)]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
@@ -76,18 +97,31 @@ def _compile_ops(verbose: bool) -> None:
     subprocess.run(cmd, check=True)
 
 
+# what each library is linked from: (source, definitions)
+_CHECK = ["-DQRB_BOUNDS_CHECK"]
+_LINKS = ((LIB, [("qrb_api.cu", []), ("qrb_layer.cu", [])]),
+          (CHECKED, [("qrb_api.cu", _CHECK), ("qrb_layer.cu", [])]),
+          (TESTKIT, [("qrb_testkit.cu", ["-DQRB_PANEL_TIMERS"])]))
+
+
 def build(force: bool = False, verbose: bool = False, extra=()) -> Path:
-    # the three nvcc runs are independent (minutes each): run them side by side
+    # the nvcc runs are independent (minutes each): run them side by side
     from concurrent.futures import ThreadPoolExecutor
-    jobs = [(src, out, defs) for src, out, defs in
-            ((CSRC / "qrb_api.cu", LIB, []),
-             (CSRC / "qrb_api.cu", CHECKED, ["-DQRB_BOUNDS_CHECK"]),
-             (CSRC / "qrb_testkit.cu", TESTKIT, ["-DQRB_PANEL_TIMERS"]))
-            if force or not up_to_date(out)]
+    jobs = {}
+    for _, units in _LINKS:
+        for name, defs in units:
+            obj = _object(CSRC / name, defs)
+            inputs = _inputs(obj)
+            if force or inputs is None or not up_to_date(obj, inputs):
+                jobs[obj] = (CSRC / name, obj, verbose, [*extra, *defs])
     with ThreadPoolExecutor(max_workers=max(1, len(jobs))) as ex:
-        for f in [ex.submit(_compile, src, out, verbose, [*extra, *defs]) for src, out, defs in jobs]:
+        for f in [ex.submit(_compile, *job) for job in jobs.values()]:
             f.result()
-    if force or not up_to_date(OPS) or OPS.stat().st_mtime < (CSRC / "qrb_torch_op.cpp").stat().st_mtime:
+    for out, units in _LINKS:
+        objs = [_object(CSRC / name, defs) for name, defs in units]
+        if force or not up_to_date(out, objs):
+            _link(objs, out, verbose)
+    if force or not up_to_date(OPS, [CSRC / "qrb_torch_op.cpp", *INCLUDE.glob("*.h")]):
         _compile_ops(verbose)
     return LIB
 

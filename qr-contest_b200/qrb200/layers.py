@@ -1,0 +1,147 @@
+"""Layer operators: what is done with an orthogonal factor once it is a weight.
+
+:func:`rms_norm` -- root-mean-square norm of rows with the residual's addition, its output in the
+input's type or in 8 bits (e4m3) with a scale a row; :func:`linear` -- matrix product with bias,
+activation and residual in its epilogue, on 16-bit operands or on 8-bit ones with scales;
+:func:`quantize_rows` -- lays a weight out in 8 bits once.  A root-mean-square norm commutes with an
+orthogonal ``Q`` (:func:`qrb200.geqrf_q`), which is why activations can be rotated before they are
+held in 8 bits.
+
+All take CUDA tensors, run on the current stream without synchronising, and raise ``TypeError`` or
+``ValueError`` on arguments they do not take.  Leading dimensions are free; rows may be slices or
+expanded views (one row stride: read in place, anything else is copied first).  ``rms_norm`` and
+``linear`` are differentiable once in every floating input where all types are 16 bits or more; the
+same inputs give the same bits.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, api
+
+_ACTIVATIONS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
+                "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
+_FP8 = torch.float8_e4m3fn
+
+
+class _Ops:
+    """The operators' handles, looked up once."""
+
+    loaded = False
+
+    @classmethod
+    def load(cls):
+        api.load_torch_ops()
+        ns = torch.ops.qrb200
+        cls.rms_norm = ns.rms_norm.default
+        cls.rms_norm_backward = ns.rms_norm_backward.default
+        cls.quantize_rows = ns.quantize_rows.default
+        cls.linear = ns.linear.default
+        cls.linear_backward = ns.linear_backward.default
+        cls.loaded = True
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        ctx.set_materialize_grads(False)
+        y, _, h = _Ops.rms_norm(x, weight, residual, eps, None)
+        ctx.eps, ctx.dtype = eps, x.dtype
+        ctx.save_for_backward(x if residual is None else h, weight)
+        return y if residual is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight = ctx.saved_tensors
+        want_x, want_w, want_r, _ = ctx.needs_input_grad
+        if dy is None:
+            if dh is None:
+                return None, None, None, None
+            dy = torch.zeros(h.shape, dtype=ctx.dtype, device=h.device)
+        dx, dres, dw = _Ops.rms_norm_backward(dy, h, dh, weight, ctx.eps, want_x, want_r, want_w)
+        return dx if want_x else None, dw, dres, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+             eps: float = 1e-6, out_dtype: torch.dtype | None = None):
+    """``h = x + residual``; ``y = h * (mean(h**2, -1) + eps)**-0.5 * weight``.
+
+    ``x`` is ``(..., d)`` in float32, bfloat16 or float16; ``weight`` ``(d,)`` in x's type or float32;
+    ``residual`` in x's shape, in x's type or float32.  ``h`` is rounded to the residual's type (it is the
+    stream that later layers read) and ``y`` is the norm of that.  Returns ``y``, or ``(y, h)`` with a
+    residual.  With ``out_dtype=torch.float8_e4m3fn`` it returns ``(y, scale)`` or ``(y, scale, h)``:
+    ``scale`` is float32, one a row, ``max(max|y| / 448, 2**-126)``, and ``y * scale[..., None]`` the value.
+    """
+    if not _Ops.loaded:
+        _Ops.load()
+    if _wants_grad(x, weight, residual):
+        if out_dtype is not None and out_dtype != x.dtype:
+            raise ValueError("qrb200: the 8-bit norm has no gradient (use torch.no_grad())")
+        return _RmsNorm.apply(x, weight, residual, eps)
+    y, scale, h = _Ops.rms_norm(x, weight, residual, eps, out_dtype)
+    if scale is None:
+        return y if h is None else (y, h)
+    return (y, scale) if h is None else (y, scale, h)
+
+
+def quantize_rows(x: torch.Tensor):
+    """Rows of ``x`` (``(..., d)``; float32, bfloat16, float16) in e4m3 with a float32 scale each, by
+    :func:`rms_norm`'s rule: returns ``(q, scale)``.  For a weight ``(n, k)`` that is one scale per
+    output feature."""
+    if not _Ops.loaded:
+        _Ops.load()
+    return _Ops.quantize_rows(x)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation, out_dtype):
+        need = any(ctx.needs_input_grad[:3])
+        y, slope = _Ops.linear(x, weight, bias, residual, activation, None, None, out_dtype,
+                               need and activation != _lib.ACT_NONE)
+        if need:
+            ctx.save_for_backward(x, weight, slope)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        want_x, want_w, want_b, want_r, _, _ = ctx.needs_input_grad
+        dx = dw = db = None
+        if want_x or want_w or want_b:
+            x, weight, slope = ctx.saved_tensors
+            dx, dw, db = _Ops.linear_backward(dy, slope, x, weight, want_x, want_w, want_b)
+        return dx, dw, db, dy if want_r else None, None, None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+           activation: str | None = None, residual: torch.Tensor | None = None,
+           x_scale: torch.Tensor | None = None, weight_scale: torch.Tensor | None = None,
+           out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual``.
+
+    ``x`` is ``(..., k)`` and ``weight`` ``(n, k)``, both bfloat16, float16 or float8_e4m3fn (a transposed view is
+    read in place for 16-bit types); ``bias`` ``(n,)`` and ``residual`` ``(..., n)`` are in the output's type, which is
+    x's, or bfloat16 (default) or float16 for 8-bit operands.  ``activation``: None, ``"relu"``, ``"gelu"``,
+    ``"gelu_tanh"``, ``"silu"``.  8-bit operands are multiplied by ``x_scale`` (one float32, or one a row of x) and
+    ``weight_scale`` (one, or one an output feature).  Sums are float32; the result is rounded once.
+    """
+    if not _Ops.loaded:
+        _Ops.load()
+    try:
+        act = _ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise ValueError(f"qrb200: unknown activation {activation!r}") from None
+    if _wants_grad(x, weight, bias, residual):
+        if x.dtype == _FP8:
+            raise ValueError("qrb200: the 8-bit product has no gradient (use torch.no_grad())")
+        if x_scale is not None or weight_scale is not None:
+            raise ValueError("qrb200: scales belong to 8-bit operands")
+        return _Linear.apply(x, weight, bias, residual, act, out_dtype)
+    return _Ops.linear(x, weight, bias, residual, act, x_scale, weight_scale, out_dtype, False)[0]
