@@ -4,6 +4,7 @@
 #include "../../include/qrb200_layer.h"
 #include "qrb_host.h"
 #include "qrb_linear.cuh"
+#include "qrb_linear_pair.cuh"
 #include "qrb_norm.cuh"
 
 #include <algorithm>
@@ -13,6 +14,7 @@ namespace qrb {
 namespace {
 
 constexpr int kSMs = 148;
+constexpr int64_t kPairTiles = 64;
 
 bool float_type(int32_t t) { return t == QRB200_F32 || t == QRB200_BF16 || t == QRB200_F16; }
 int esize(int32_t t) { return t == QRB200_F32 ? 4 : (t == QRB200_E4M3 ? 1 : 2); }
@@ -228,9 +230,76 @@ int launch_tile_t(int T, const lin::Maps& maps, const lin::Args& a, cudaStream_t
   }
 }
 
+// A map over rows of 16-bit results (or a residual), in blocks of 32 rows x 64 columns.
+bool encode_result(CUtensorMap* map, const void* p, int64_t ld, int64_t m, int64_t n) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)n, (cuuint64_t)m};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {64, 32}, one[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(p), dims, strides, box, one,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename Out, int ES, int TN, bool SLOPE>
+int launch_pair(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_t k, int32_t dtype,
+                const lin::Epilogue& e, cudaStream_t st) {
+  auto kernel = lin::pair_kernel<Out, ES, TN, SLOPE>;
+  using C = lin::PairCfg<TN>;
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  if (note(cudaGetDevice(&dev)) != cudaSuccess) return QRB200_ERR_CUDA;
+  if (!(ready.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+    if (note(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess)
+      return QRB200_ERR_CUDA;
+    ready.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
+  }
+  lin::PairMaps maps{};
+  lin::PairArgs a{};
+  a.m = (int)m; a.n = (int)n; a.k = (int)k;
+  a.p_row = P.row_major; a.q_row = Q.row_major;
+  a.idesc = lin::idesc(dtype == QRB200_BF16 ? 1 : 0, a.p_row, a.q_row, lin::kPairM, TN);
+  a.tiles_i = (int)((m + lin::kPairM - 1) / lin::kPairM);
+  a.tiles_j = (int)((n + TN - 1) / TN);
+  a.group = 8;
+  a.e = e;
+  a.tma_out = rows_on16(e.out, e.ldo, 2);
+  a.tma_res = e.res && rows_on16(e.res, e.ldr, 2) && e.ldr > 0;
+  a.tma_slope = e.slope && rows_on16(e.slope, n, 2);
+  bool good = encode_operand(&maps.p, P, m, k, dtype, 128) && encode_operand(&maps.q, Q, n, k, dtype, TN / 2);
+  if (good && a.tma_out) good = encode_result(&maps.out, e.out, e.ldo, m, n);
+  if (good && a.tma_res) good = encode_result(&maps.res, e.res, e.ldr, m, n);
+  if (good && a.tma_slope) good = encode_result(&maps.slope, e.slope, n, m, n);
+  if (!good) {
+    note(cudaErrorInvalidValue);
+    return QRB200_ERR_CUDA;
+  }
+  const int64_t tiles = (int64_t)a.tiles_i * a.tiles_j;
+  const unsigned grid = 2 * (unsigned)std::min<int64_t>(tiles, kSMs / 2);
+  kernel<<<grid, lin::kPairThreads, C::SMEM, st>>>(maps, a);
+  return launched();
+}
+
+template <int TN>
+int product_pair(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t out_dtype,
+                 const lin::Epilogue& e, cudaStream_t st) {
+  const bool bf = out_dtype == QRB200_BF16;
+  if (dtype == QRB200_E4M3)
+    return bf ? launch_pair<__nv_bfloat16, 1, TN, false>(P, Q, m, n, k, dtype, e, st)
+              : launch_pair<__half, 1, TN, false>(P, Q, m, n, k, dtype, e, st);
+  if (e.slope)
+    return bf ? launch_pair<__nv_bfloat16, 2, TN, true>(P, Q, m, n, k, dtype, e, st)
+              : launch_pair<__half, 2, TN, true>(P, Q, m, n, k, dtype, e, st);
+  return bf ? launch_pair<__nv_bfloat16, 2, TN, false>(P, Q, m, n, k, dtype, e, st)
+            : launch_pair<__half, 2, TN, false>(P, Q, m, n, k, dtype, e, st);
+}
+
 // D = epilogue(P Q^T); P is m x k, Q is n x k, both addressable by TMA.
 int product(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t out_dtype,
             const lin::Epilogue& e, cudaStream_t st) {
+  // Enough 256 x 256 tiles for most of the 74 CTA pairs: the persistent kernel.
+  if (k > 0 && ((m + 255) / 256) * ((n + 255) / 256) >= kPairTiles) return product_pair<256>(P, Q, m, n, k, dtype, out_dtype, e, st);
   lin::Args a{};
   a.m = (int)m; a.n = (int)n; a.k = (int)k;
   a.e = e;

@@ -266,6 +266,33 @@ def test_linear(m, n, k, dtype):
     assert torch.equal(q().linear(x, w), plain)
 
 
+# enough 256 x 256 tiles for the persistent kernel; edges inside tiles, rows off 16 bytes
+LARGE = [(2048, 2048, 256), (1793, 2304, 520), (2305, 1793, 77), (16400, 264, 136), (300, 16400, 40), (4000, 2056, 1032)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_linear_large(m, n, k, dtype):
+    x, w = rnd(m, k, dtype=dtype, seed=1), rnd(n, k, dtype=dtype, seed=2, gain=k ** -0.5)
+    b, res = rnd(n, dtype=dtype, seed=3), rnd(m, n, dtype=dtype, seed=4)
+    plain = check_linear(x, w)
+    for i, act in enumerate(ACTS):
+        check_linear(x, w, b if i % 2 else None, act, res if i != 2 else None)
+    assert torch.equal(check_linear(x, w.t().contiguous().t()), plain)
+    assert torch.equal(q().linear(x, w), plain)
+    wide = rnd(m, n + 13, dtype=dtype, seed=6)
+    check_linear(x, w, b, "silu", wide[:, 5:5 + n])
+    check_linear(x, w, b, None, wide[0, :n].expand(m, n))
+
+
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_linear_large_8bit(m, n, k):
+    x8, xs = q().quantize_rows(rnd(m, k, seed=1))
+    w8, ws = q().quantize_rows(rnd(n, k, seed=2, gain=k ** -0.5))
+    check_linear(x8, w8, rnd(n, dtype=BF, seed=3), "gelu", rnd(m, n, dtype=BF, seed=4), xs, ws)
+    check_linear(x8, w8, None, None, None, xs, ws, F16)
+
+
 @pytest.mark.parametrize("out", [None, F16])
 @pytest.mark.parametrize("m,n,k", SIZES)
 def test_linear_8bit(m, n, k, out):
@@ -353,7 +380,7 @@ def test_layers_in_a_graph():
 
 
 GRAD_SIZES = [(1, 1, 1), (3, 5, 7), (16, 128, 64), (70, 130, 200), (64, 512, 1000), (1000, 100, 64), (300, 257, 513),
-              (4100, 64, 128), (256, 512, 512), (700, 1000, 264)]
+              (4100, 64, 128), (256, 512, 512), (700, 1000, 264), (2048, 2048, 2048), (2300, 1993, 2050)]
 
 
 @pytest.mark.parametrize("dtype", [BF, F16])
