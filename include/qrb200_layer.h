@@ -50,7 +50,8 @@ int qrb200_quantize_rows(const void* x, int64_t ldx, void* q, float* scale, int6
  * dx, dresidual and dweight are contiguous and may each be NULL; dresidual equals dx, so it is only
  * needed where stream_dtype differs.  The weight's gradient is added up in a fixed order: the same
  * inputs give the same bits.  `workspace` (NULL: allocated stream-ordered) is needed for dweight. */
-int qrb200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t dim, size_t* bytes);
+int qrb200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t dim, int32_t dtype,
+                                             int32_t stream_dtype, size_t* bytes);
 int qrb200_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh,
                              const void* dh, int64_t lddh, const void* weight,
                              int32_t weight_dtype, void* dx, void* dresidual, void* dweight,

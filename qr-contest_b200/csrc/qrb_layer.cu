@@ -27,6 +27,17 @@ int launched() {
   return note(cudaGetLastError()) == cudaSuccess ? QRB200_OK : QRB200_ERR_CUDA;
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory, once per device (`ready`: the devices done).
+int raise_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  if (note(cudaGetDevice(&dev)) != cudaSuccess) return QRB200_ERR_CUDA;
+  if (ready.load(std::memory_order_relaxed) >> (dev & 63) & 1) return QRB200_OK;
+  if (note(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) != cudaSuccess)
+    return QRB200_ERR_CUDA;
+  if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  return QRB200_OK;
+}
+
 // Device memory for one call when the caller gives none; freed in stream order.
 struct Scratch {
   void* p = nullptr;
@@ -48,83 +59,101 @@ struct Scratch {
 };
 
 // ------------------------------------------------------------------ norm
-// Threads of a row and vectors of 8 elements a thread.  Up to 1024 elements a warp takes the row
-// (4 rows a block).  Longer rows: with enough rows to fill the GPU, as many elements a thread as
-// registers allow (32: more bytes in flight, fewer barriers); with few rows, one vector a thread.
+// Threads of a row, vectors of 8 elements a thread, rows a block.  Up to 1024 elements a warp or a part
+// of one takes the row (128 threads a block).  Longer rows, 16-bit types: with enough rows to fill the
+// GPU, 4 vectors a thread (more bytes in flight, fewer barriers); with few rows, one.  float32
+// vectors take twice the registers: 2 at most.
 struct Shape { int nt, vpt, rows; };
-Shape norm_shape(int64_t rows, int dim) {
+Shape norm_shape(int64_t rows, int dim, bool wide) {
   const int vecs = (dim + 7) / 8;
-  if (dim <= 1024 && rows > kSMs) return {32, vecs <= 32 ? 1 : (vecs <= 64 ? 2 : 4), 4};
+  if (dim <= 1024 && rows > kSMs) {
+    int vpt = vecs <= 32 ? 1 : (vecs <= 64 || wide ? 2 : 4), nt = 4;
+    while (nt * vpt < vecs) nt *= 2;
+    if (nt <= 32) return {nt, vpt, 128 / nt};
+    return {nt, vpt, 1};
+  }
+  const int most = wide ? 2 : 4;
   int vpt = 1;
-  if (rows > 2 * kSMs) vpt = vecs <= 128 ? 1 : (vecs <= 256 ? 2 : 4);
+  if (rows > 2 * kSMs) vpt = vecs <= 128 ? 1 : (vecs <= 256 ? 2 : most);
   while ((vecs + vpt - 1) / vpt > norm::max_threads(vpt)) vpt *= 2;
   const int nt = std::max(32, ((vecs + vpt - 1) / vpt + 31) / 32 * 32);
   return {nt, vpt, 1};
 }
 
-template <typename TX, typename TR, bool Q8, bool NORM>
+template <typename TX, typename TH, bool RES, bool Q8, bool NORM>
 int launch_fwd(const norm::FwdArgs& a, bool vec, cudaStream_t st) {
+  constexpr bool wide = sizeof(TX) == 4 || sizeof(TH) == 4;
   if (a.dim > norm::kRegDim) {
-    norm::fwd_long_kernel<TX, TR, Q8, NORM><<<(unsigned)a.rows, norm::kMaxThreads, 0, st>>>(a);
+    norm::fwd_long_kernel<TX, TH, Q8, NORM><<<(unsigned)a.rows, norm::kMaxThreads, 0, st>>>(a);
     return launched();
   }
-  const Shape s = norm_shape(a.rows, a.dim);
+  const Shape s = norm_shape(a.rows, a.dim, wide);
   const dim3 block(s.nt, s.rows);
   const unsigned grid = (unsigned)((a.rows + s.rows - 1) / s.rows);
-#define QRB_FWD(V, VEC) norm::fwd_kernel<TX, TR, Q8, NORM, V, VEC><<<grid, block, 0, st>>>(a)
-  if (vec) {
-    if (s.vpt == 1) QRB_FWD(1, true); else if (s.vpt == 2) QRB_FWD(2, true); else QRB_FWD(4, true);
-  } else {
-    if (s.vpt == 1) QRB_FWD(1, false); else if (s.vpt == 2) QRB_FWD(2, false); else QRB_FWD(4, false);
-  }
+#define QRB_FWD(V, VEC) norm::fwd_kernel<TX, TH, RES, Q8, NORM, V, VEC><<<grid, block, 0, st>>>(a)
+  if (s.vpt == 1) { if (vec) QRB_FWD(1, true); else QRB_FWD(1, false); }
+  else if (s.vpt == 2) { if (vec) QRB_FWD(2, true); else QRB_FWD(2, false); }
+  else if constexpr (!wide) { if (vec) QRB_FWD(4, true); else QRB_FWD(4, false); }
 #undef QRB_FWD
   return launched();
 }
 
-template <typename TX, typename TR, bool NORM>
-int launch_fwd_out(const norm::FwdArgs& a, bool q8, bool vec, cudaStream_t st) {
-  return q8 ? launch_fwd<TX, TR, true, NORM>(a, vec, st) : launch_fwd<TX, TR, false, NORM>(a, vec, st);
+template <typename TX>
+int launch_norm(const norm::FwdArgs& a, bool q8, bool stream_f32, bool vec, cudaStream_t st) {
+  if (!a.res) return q8 ? launch_fwd<TX, TX, false, true, true>(a, vec, st) : launch_fwd<TX, TX, false, false, true>(a, vec, st);
+  if (stream_f32) return q8 ? launch_fwd<TX, float, true, true, true>(a, vec, st) : launch_fwd<TX, float, true, false, true>(a, vec, st);
+  return q8 ? launch_fwd<TX, TX, true, true, true>(a, vec, st) : launch_fwd<TX, TX, true, false, true>(a, vec, st);
 }
 
-template <typename TX, typename TR>
-int launch_bwd(const norm::BwdArgs& a, bool vec, int64_t grid, Shape s, cudaStream_t st) {
-  if (a.dim > norm::kRegDim) {
-    norm::bwd_long_kernel<TX, TR><<<(unsigned)grid, norm::kMaxThreads, 0, st>>>(a);
-    return launched();
-  }
-  const dim3 block(s.nt, s.rows);
-#define QRB_BWD(V, VEC) norm::bwd_kernel<TX, TR, V, VEC><<<(unsigned)grid, block, 0, st>>>(a)
-  if (vec) {
-    if (s.vpt == 1) QRB_BWD(1, true); else if (s.vpt == 2) QRB_BWD(2, true); else QRB_BWD(4, true);
-  } else {
-    if (s.vpt == 1) QRB_BWD(1, false); else if (s.vpt == 2) QRB_BWD(2, false); else QRB_BWD(4, false);
-  }
-#undef QRB_BWD
-  return launched();
-}
-
-// Shape and grid of the backward kernel; parts = rows of partial weight gradients it writes.
-// A block walks over its rows, so the grid is what the GPU holds at once.
-struct BwdPlan { Shape s; int64_t grid, parts; };
-BwdPlan bwd_plan(int64_t rows, int dim) {
+// Shape, rows of look-ahead and grid of the backward kernel; parts = rows of partial weight gradients
+// it writes.  A block walks over its rows, so the grid is what the GPU holds at once: 128 registers a
+// thread, and shared memory for `depth` rows.
+constexpr int kBwdRing = 220 * 1024;  // shared memory of a block at most
+struct BwdPlan { Shape s; int depth; size_t smem; int64_t grid, parts; };
+BwdPlan bwd_plan(int64_t rows, int dim, int es, int hs) {
   BwdPlan p{};
   if (dim > norm::kRegDim) {
     p.s = {norm::kMaxThreads, 0, 1};
     p.grid = p.parts = std::min<int64_t>(rows, 2 * kSMs);
     return p;
   }
-  const int vecs = (dim + 7) / 8;
+  const int vecs = (dim + 7) / 8, slot = 8 * (es + 2 * hs);
   if (dim <= 1024) {
-    p.s = {32, vecs <= 32 ? 1 : (vecs <= 64 ? 2 : 4), 4};
-    p.grid = std::min<int64_t>((rows + 3) / 4, 4 * kSMs);
+    int vpt = vecs <= 32 ? 1 : (vecs <= 64 ? 2 : 4), nt = 4;
+    while (nt * vpt < vecs) nt *= 2;
+    p.s = {nt, vpt, 128 / nt};
   } else {
     const int vpt = vecs <= 256 ? 2 : 4;
-    const int nt = ((vecs + vpt - 1) / vpt + 31) / 32 * 32;
-    p.s = {nt, vpt, 1};
-    p.grid = std::min<int64_t>(rows, kSMs * std::max(1, 512 / nt));
+    p.s = {((vecs + vpt - 1) / vpt + 31) / 32 * 32, vpt, 1};
   }
+  const int threads = p.s.nt * p.s.rows;
+  const size_t row = (size_t)threads * p.s.vpt * slot;
+  p.depth = 2 * row <= (size_t)kBwdRing ? 2 : 1;
+  p.smem = p.depth * row;
+  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(512 / threads, 225 * 1024 / (int64_t)(p.smem + 1536)));
+  p.grid = std::min<int64_t>((rows + p.s.rows - 1) / p.s.rows, kSMs * per_sm);
   p.parts = p.grid * p.s.rows;
   return p;
+}
+
+template <typename TX, typename TH, int VPT, bool VEC>
+int launch_bwd_as(const norm::BwdArgs& a, const BwdPlan& p, cudaStream_t st) {
+  auto kernel = norm::bwd_kernel<TX, TH, VPT, VEC>;
+  const size_t smem = VEC ? p.smem : 0;
+  static std::atomic<uint64_t> ready{0};
+  if (const int rc = raise_smem(reinterpret_cast<const void*>(kernel), kBwdRing, ready)) return rc;
+  kernel<<<(unsigned)p.grid, dim3(p.s.nt, p.s.rows), smem, st>>>(a, p.depth);
+  return launched();
+}
+template <typename TX, typename TH>
+int launch_bwd(const norm::BwdArgs& a, bool vec, const BwdPlan& p, cudaStream_t st) {
+  if (a.dim > norm::kRegDim) {
+    norm::bwd_long_kernel<TX, TH><<<(unsigned)p.grid, norm::kMaxThreads, 0, st>>>(a);
+    return launched();
+  }
+  if (p.s.vpt == 1) return vec ? launch_bwd_as<TX, TH, 1, true>(a, p, st) : launch_bwd_as<TX, TH, 1, false>(a, p, st);
+  if (p.s.vpt == 2) return vec ? launch_bwd_as<TX, TH, 2, true>(a, p, st) : launch_bwd_as<TX, TH, 2, false>(a, p, st);
+  return vec ? launch_bwd_as<TX, TH, 4, true>(a, p, st) : launch_bwd_as<TX, TH, 4, false>(a, p, st);
 }
 
 template <typename T>
@@ -190,14 +219,8 @@ template <typename Out, int ES, int T, bool SLOPE>
 int launch_tile(const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
   auto kernel = lin::tile_kernel<Out, ES, T, SLOPE>;
   using C = lin::TileCfg<T>;
-  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit has been raised
-  int dev = 0;
-  if (note(cudaGetDevice(&dev)) != cudaSuccess) return QRB200_ERR_CUDA;
-  if (!(ready.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
-    if (note(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess)
-      return QRB200_ERR_CUDA;
-    ready.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
-  }
+  static std::atomic<uint64_t> ready{0};
+  if (const int rc = raise_smem(reinterpret_cast<const void*>(kernel), C::SMEM, ready)) return rc;
   const int64_t tiles = (int64_t)((a.n + 127) / 128) * ((a.m + T - 1) / T);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(tiles * a.splits));
@@ -248,13 +271,7 @@ int launch_pair(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_
   auto kernel = lin::pair_kernel<Out, ES, TN, SLOPE>;
   using C = lin::PairCfg<TN>;
   static std::atomic<uint64_t> ready{0};
-  int dev = 0;
-  if (note(cudaGetDevice(&dev)) != cudaSuccess) return QRB200_ERR_CUDA;
-  if (!(ready.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
-    if (note(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess)
-      return QRB200_ERR_CUDA;
-    ready.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
-  }
+  if (const int rc = raise_smem(reinterpret_cast<const void*>(kernel), C::SMEM, ready)) return rc;
   lin::PairMaps maps{};
   lin::PairArgs a{};
   a.m = (int)m; a.n = (int)n; a.k = (int)k;
@@ -404,13 +421,10 @@ int qrb200_rms_norm(const void* x, int64_t ldx, const void* weight, int32_t weig
   const bool vec = dim % 8 == 0 && rows_on16(x, ldx, es) && on16(y) &&
                    (!residual || (rows_on16(residual, ldr, rs) && on16(h))) && (!weight || on16(weight));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool wide = residual && stream_dtype == QRB200_F32;
-  if (dtype == QRB200_F32) return launch_fwd_out<float, float, true>(a, q8, vec, st);
-  if (dtype == QRB200_BF16)
-    return wide ? launch_fwd_out<__nv_bfloat16, float, true>(a, q8, vec, st)
-                : launch_fwd_out<__nv_bfloat16, __nv_bfloat16, true>(a, q8, vec, st);
-  return wide ? launch_fwd_out<__half, float, true>(a, q8, vec, st)
-              : launch_fwd_out<__half, __half, true>(a, q8, vec, st);
+  const bool wide = residual && stream_dtype == QRB200_F32 && dtype != QRB200_F32;
+  if (dtype == QRB200_F32) return launch_norm<float>(a, q8, wide, vec, st);
+  if (dtype == QRB200_BF16) return launch_norm<__nv_bfloat16>(a, q8, wide, vec, st);
+  return launch_norm<__half>(a, q8, wide, vec, st);
 }
 
 int qrb200_quantize_rows(const void* x, int64_t ldx, void* q, float* scale, int64_t rows, int64_t dim, int32_t dtype,
@@ -422,15 +436,16 @@ int qrb200_quantize_rows(const void* x, int64_t ldx, void* q, float* scale, int6
   norm::FwdArgs a{x, ldx, nullptr, 0, nullptr, 0, q, scale, nullptr, rows, (int)dim, 0.f};
   const bool vec = dim % 8 == 0 && rows_on16(x, ldx, esize(dtype)) && on16(q);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == QRB200_F32) return launch_fwd<float, float, true, false>(a, vec, st);
-  if (dtype == QRB200_BF16) return launch_fwd<__nv_bfloat16, __nv_bfloat16, true, false>(a, vec, st);
-  return launch_fwd<__half, __half, true, false>(a, vec, st);
+  if (dtype == QRB200_F32) return launch_fwd<float, float, false, true, false>(a, vec, st);
+  if (dtype == QRB200_BF16) return launch_fwd<__nv_bfloat16, __nv_bfloat16, false, true, false>(a, vec, st);
+  return launch_fwd<__half, __half, false, true, false>(a, vec, st);
 }
 
-int qrb200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t dim, size_t* bytes) {
-  if (!bytes || rows < 0 || dim < 0 || rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30))
+int qrb200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t dim, int32_t dtype, int32_t stream_dtype,
+                                             size_t* bytes) {
+  if (!bytes || !float_type(dtype) || !(stream_dtype == dtype || stream_dtype == QRB200_F32) || rows < 0 || dim < 0 || rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30))
     return QRB200_ERR_INVALID_ARG;
-  *bytes = rows && dim ? (size_t)bwd_plan(rows, (int)dim).parts * dim * sizeof(float) : 0;
+  *bytes = rows && dim ? (size_t)bwd_plan(rows, (int)dim, esize(dtype), esize(stream_dtype)).parts * dim * sizeof(float) : 0;
   return QRB200_OK;
 }
 
@@ -452,7 +467,7 @@ int qrb200_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_
   }
   if (!dy || !h || rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30) || lddy < 0 || ldh < 0 || (dh && lddh < 0))
     return QRB200_ERR_INVALID_ARG;
-  const BwdPlan plan = bwd_plan(rows, (int)dim);
+  const BwdPlan plan = bwd_plan(rows, (int)dim, esize(dtype), esize(stream_dtype));
   Scratch ws(st);
   int rc = ws.get(workspace, workspace_bytes, dweight ? (size_t)plan.parts * dim * sizeof(float) : 0);
   if (rc != QRB200_OK) return rc;
@@ -463,13 +478,13 @@ int qrb200_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_
                    (!dh || rows_on16(dh, lddh, rs)) && (!dx || on16(dx)) && (!dresidual || on16(dresidual)) &&
                    (!weight || on16(weight)) && (!a.part || on16(a.part));
   const bool wide = stream_dtype == QRB200_F32 && dtype != QRB200_F32;
-  if (dtype == QRB200_F32) rc = launch_bwd<float, float>(a, vec, plan.grid, plan.s, st);
+  if (dtype == QRB200_F32) rc = launch_bwd<float, float>(a, vec, plan, st);
   else if (dtype == QRB200_BF16)
-    rc = wide ? launch_bwd<__nv_bfloat16, float>(a, vec, plan.grid, plan.s, st)
-              : launch_bwd<__nv_bfloat16, __nv_bfloat16>(a, vec, plan.grid, plan.s, st);
+    rc = wide ? launch_bwd<__nv_bfloat16, float>(a, vec, plan, st)
+              : launch_bwd<__nv_bfloat16, __nv_bfloat16>(a, vec, plan, st);
   else
-    rc = wide ? launch_bwd<__half, float>(a, vec, plan.grid, plan.s, st)
-              : launch_bwd<__half, __half>(a, vec, plan.grid, plan.s, st);
+    rc = wide ? launch_bwd<__half, float>(a, vec, plan, st)
+              : launch_bwd<__half, __half>(a, vec, plan, st);
   if (rc == QRB200_OK && dweight) rc = colsum(a.part, plan.parts, dim, dweight, weight_dtype, st);
   return rc;
 }

@@ -10,10 +10,10 @@
 // All sums, r, s and c are float32; every output is rounded once, when it is stored.
 //
 // All of it is bound by memory: about 10 operations an element against 3 to 8 bytes.  So a row is
-// read once and stays in registers between its reductions: VPT 8-element vectors a thread
-// (16 bytes of a 16-bit type each), blockDim.x threads a row.  Rows of up to 1024 elements take a
-// warp each (blockDim.y rows a block, shuffles only); longer ones a block each, up to 16384
-// elements; longer rows still are read again for each pass.  Rows that start off a 16-byte
+// read once and stays in registers, as it is stored, between its reductions: VPT 8-element vectors a
+// thread (16 bytes of a 16-bit type each), blockDim.x threads a row.  Rows of up to 1024 elements take
+// a warp or a part of one (blockDim.y rows a block, shuffles only); longer ones a block each, up to
+// 16384 elements; longer rows still are read again for each pass.  Rows that start off a 16-byte
 // boundary (odd widths, odd strides) use the same kernels with single-element accesses, thread t
 // taking elements t, t + blockDim.x, ... so that a warp's accesses stay adjacent.
 #pragma once
@@ -25,30 +25,35 @@ namespace qrb {
 namespace norm {
 
 constexpr int kMaxThreads = 1024;
-// threads a row: one vector each leaves room for 1024 of them, more vectors for 512
-constexpr int max_threads(int vpt) { return vpt == 1 ? kMaxThreads : 512; }
-constexpr int kRegDim = 512 * 4 * 8;                // longest row that stays in registers
+// Threads a row: 64 registers each, so 1024 of them fill an SM's register file whatever the shape.
+constexpr int max_threads(int vpt) { return vpt == 4 ? 512 : kMaxThreads; }
+constexpr int kRegDim = 16384;                      // longest row that stays in registers
 constexpr float kFp8Max = 448.f;                    // largest e4m3 value
 constexpr float kTiny = 1.17549435e-38f;            // 2^-126
 
-// ---- 8 elements of a row <-> float ----
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// ---- 8 elements of a row, as they are stored: 4 registers for 16-bit types ----
+template <typename T>
+struct Vec8 {
+  static constexpr int Q = sizeof(T) / 2;  // 16-byte parts
+  uint4 q[Q];
+};
+__device__ __forceinline__ void unpack(const Vec8<float>& a, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    v[4 * i] = __uint_as_float(a.q[i].x); v[4 * i + 1] = __uint_as_float(a.q[i].y);
+    v[4 * i + 2] = __uint_as_float(a.q[i].z); v[4 * i + 3] = __uint_as_float(a.q[i].w);
+  }
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void unpack(const Vec8<__nv_bfloat16>& a, float (&v)[8]) {
+  const uint32_t w[4] = {a.q[0].x, a.q[0].y, a.q[0].z, a.q[0].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[2 * i] = __uint_as_float(w[i] << 16);
     v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
   }
 }
-__device__ __forceinline__ void load8(const __half* p, float (&v)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void unpack(const Vec8<__half>& a, float (&v)[8]) {
+  const uint32_t w[4] = {a.q[0].x, a.q[0].y, a.q[0].z, a.q[0].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
@@ -56,22 +61,39 @@ __device__ __forceinline__ void load8(const __half* p, float (&v)[8]) {
     v[2 * i + 1] = f.y;
   }
 }
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
-template <typename T2, typename T>
-__device__ __forceinline__ void store8_16(T* p, const float (&v)[8], T2 (*pack)(float, float)) {
-  T2 w[4];
+__device__ __forceinline__ void pack(Vec8<float>& a, const float (&v)[8]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack(v[2 * i], v[2 * i + 1]);
-  *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(w);
+  for (int i = 0; i < 2; ++i)
+    a.q[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                        __float_as_uint(v[4 * i + 3]));
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
-  store8_16<__nv_bfloat162>(p, v, [](float a, float b) { return __floats2bfloat162_rn(a, b); });
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
-  store8_16<__half2>(p, v, [](float a, float b) { return __floats2half2_rn(a, b); });
+__device__ __forceinline__ uint32_t pack2(__half, float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ void pack(Vec8<T>& a, const float (&v)[8]) {
+  a.q[0] = make_uint4(pack2(T(), v[0], v[1]), pack2(T(), v[2], v[3]), pack2(T(), v[4], v[5]), pack2(T(), v[6], v[7]));
+}
+// Rows are read once: they need not stay in the caches (STREAM); a weight is read for every row.
+template <bool STREAM, typename T>
+__device__ __forceinline__ void load8(const T* p, Vec8<T>& a) {
+#pragma unroll
+  for (int i = 0; i < Vec8<T>::Q; ++i) {
+    const uint4* at = reinterpret_cast<const uint4*>(p) + i;
+    a.q[i] = STREAM ? __ldcs(at) : *at;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  Vec8<T> a;
+  pack(a, v);
+#pragma unroll
+  for (int i = 0; i < Vec8<T>::Q; ++i) reinterpret_cast<uint4*>(p)[i] = a.q[i];
 }
 __device__ __forceinline__ uint8_t to_e4m3(float v) {
   return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
@@ -95,64 +117,51 @@ template <int VPT, bool VEC>
 struct Share {
   int dim, nt, t;
   __device__ Share(int dim_) : dim(dim_), nt(blockDim.x), t(threadIdx.x) {}
-  template <typename T> __device__ __forceinline__ void load(const T* row, float (&v)[VPT][8]) const {
+  // group i of a row, zero beyond its end
+  template <bool STREAM, typename T>
+  __device__ __forceinline__ void load(const T* row, int i, Vec8<T>& a) const {
+    if (VEC) {
+      const int c = 8 * (i * nt + t);
+      if (c < dim) load8<STREAM>(row + c, a);
+      else {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      if (VEC) {
-        const int c = 8 * (i * nt + t);
-        if (c < dim) load8(row + c, v[i]);
-        else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = (8 * i + j) * nt + t;
-          v[i][j] = c < dim ? to_f32(row[c]) : 0.f;
-        }
+        for (int x = 0; x < Vec8<T>::Q; ++x) a.q[x] = make_uint4(0, 0, 0, 0);
       }
+    } else {
+      T e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = (8 * i + j) * nt + t;
+        e[j] = c < dim ? row[c] : from_f32<T>(0.f);
+      }
+      memcpy(&a, e, sizeof(a));
     }
   }
-  template <typename T> __device__ __forceinline__ void store(T* row, const float (&v)[VPT][8]) const {
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, int i, const float (&v)[8]) const {
+    if (VEC) {
+      const int c = 8 * (i * nt + t);
+      if (c < dim) store8(row + c, v);
+    } else {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      if (VEC) {
-        const int c = 8 * (i * nt + t);
-        if (c < dim) store8(row + c, v[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = (8 * i + j) * nt + t;
-          if (c < dim) store1(row + c, v[i][j]);
-        }
+      for (int j = 0; j < 8; ++j) {
+        const int c = (8 * i + j) * nt + t;
+        if (c < dim) store1(row + c, v[j]);
       }
     }
   }
 };
 
 // ---- reductions over the blockDim.x threads of a row ----
-// Warp shuffles; with more than one warp a row (blockDim.y == 1 then) one exchange through
-// `slots` and one barrier.  Every thread gets the result; the order of the additions is fixed.
-__device__ __forceinline__ float row_sum(float v, float* slots) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (blockDim.x == 32) return v;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) slots[warp] = v;
-  __syncthreads();
-  v = lane < (int)(blockDim.x >> 5) ? slots[lane] : 0.f;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
+// Shuffles among the threads of a warp that share the row (a power of two up to 32); with more than
+// one warp a row (blockDim.y == 1 then) one exchange through `slots` and one barrier.  Every thread
+// gets the result; the order of the additions is fixed.
 __device__ __forceinline__ float2 row_sum2(float a, float b, float2* slots) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
+  for (int o = min(blockDim.x, 32u) >> 1; o; o >>= 1) {
     a += __shfl_xor_sync(0xffffffffu, a, o);
     b += __shfl_xor_sync(0xffffffffu, b, o);
   }
-  if (blockDim.x == 32) return make_float2(a, b);
+  if (blockDim.x <= 32) return make_float2(a, b);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (lane == 0) slots[warp] = make_float2(a, b);
   __syncthreads();
@@ -166,9 +175,24 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2* slots) {
   }
   return make_float2(a, b);
 }
+__device__ __forceinline__ float row_sum(float v, float* slots) {
+  for (int o = min(blockDim.x, 32u) >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (blockDim.x <= 32) return v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) slots[warp] = v;
+  __syncthreads();
+  v = lane < (int)(blockDim.x >> 5) ? slots[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 // Largest |v| as bit patterns: without the sign they order like the numbers, with NaN above
 // infinity, so a NaN in the row is the result.
 __device__ __forceinline__ float row_absmax(uint32_t bits, uint32_t* slots) {
+  if (blockDim.x < 32) {
+    for (int o = blockDim.x >> 1; o; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+    return __uint_as_float(bits);
+  }
   bits = __reduce_max_sync(0xffffffffu, bits);
   if (blockDim.x > 32) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -195,63 +219,113 @@ struct FwdArgs {
   float eps;
 };
 
-// v as it is kept in the stream's type.
-template <typename TR> __device__ __forceinline__ float as_kept(float v) { return to_f32(from_f32<TR>(v)); }
+// Group i of the weight as float32.  One in x's type waits in registers; a float32 one is read
+// from the cache where it is used.
+template <typename TX, int VPT, bool VEC>
+struct Weight {
+  Vec8<TX> kept[VPT];
+  __device__ __forceinline__ void load(const Share<VPT, VEC>& mine, const void* w, bool f32) {
+    if (w && !f32) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) mine.template load<false>(static_cast<const TX*>(w), i, kept[i]);
+    }
+  }
+  __device__ __forceinline__ void get(const Share<VPT, VEC>& mine, const void* w, bool f32, int i, float (&v)[8]) const {
+    if (!w) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 1.f;
+    } else if (f32) {
+      Vec8<float> a;
+      mine.template load<false>(static_cast<const float*>(w), i, a);
+      unpack(a, v);
+    } else {
+      unpack(kept[i], v);
+    }
+  }
+};
 
-template <typename TX, typename TR, bool Q8, bool NORM, int VPT, bool VEC>
-__global__ void __launch_bounds__(max_threads(VPT)) fwd_kernel(FwdArgs a) {
+// TH is the type that the norm reads: the stream's with a residual, else x's.
+template <typename TX, typename TH, bool RES, bool Q8, bool NORM, int VPT, bool VEC>
+__global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VPT)) fwd_kernel(FwdArgs a) {
   __shared__ float s_sum[32];
   __shared__ uint32_t s_max[32];
-  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= a.rows) return;  // with several rows a block no barrier follows
+  // rows past the end are computed again from the last row and not stored: no thread leaves early
+  const int64_t at = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  const bool live = at < a.rows;
+  const int64_t row = live ? at : a.rows - 1;
   const Share<VPT, VEC> mine(a.dim);
-  float v[VPT][8];
-  mine.load(static_cast<const TX*>(a.x) + row * a.ldx, v);
-  if (NORM) {
-    if (a.res) {
-      float u[VPT][8];
-      mine.load(static_cast<const TR*>(a.res) + row * a.ldr, u);
+  Vec8<TH> h[VPT];
+  Weight<TX, VPT, VEC> w;
+  if constexpr (RES) {
+    Vec8<TX> x[VPT];
 #pragma unroll
-      for (int i = 0; i < VPT; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = as_kept<TR>(v[i][j] + u[i][j]);
-      mine.store(static_cast<TR*>(a.h) + row * a.dim, v);
+    for (int i = 0; i < VPT; ++i) {
+      mine.template load<true>(static_cast<const TX*>(a.x) + row * a.ldx, i, x[i]);
+      mine.template load<true>(static_cast<const TH*>(a.res) + row * a.ldr, i, h[i]);
     }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float u[8], v[8];
+      unpack(x[i], u);
+      unpack(h[i], v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += u[j];
+      pack(h[i], v);  // rounded as it is kept
+      if (live) mine.store(static_cast<TH*>(a.h) + row * a.dim, i, v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) mine.template load<true>(static_cast<const TH*>(a.x) + row * a.ldx, i, h[i]);
+  }
+  float r = 1.f;
+  if (NORM) {
+    w.load(mine, a.w, a.w_f32);
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
+    for (int i = 0; i < VPT; ++i) {
+      float v[8];
+      unpack(h[i], v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j], v[i][j], ss);
-    float w[VPT][8];
-    if (!a.w) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[i][j] = 1.f;
-    } else if (a.w_f32) mine.load(static_cast<const float*>(a.w), w);
-    else mine.load(static_cast<const TX*>(a.w), w);
-    const float r = rsqrtf(row_sum(ss, s_sum) / a.dim + a.eps);
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * r * w[i][j];
+      for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+    }
+    r = rsqrtf(row_sum(ss, s_sum) / a.dim + a.eps);
   }
+  auto value = [&](int i, float (&v)[8]) {
+    unpack(h[i], v);
+    if (NORM) {
+      float u[8];
+      w.get(mine, a.w, a.w_f32, i, u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = v[j] * r * u[j];
+    }
+  };
   if (Q8) {
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
+    for (int i = 0; i < VPT; ++i) {
+      float v[8];
+      value(i, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
+      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    }
     const float s = scale_of(row_absmax(top, s_max));
     const float inv = 1.f / s;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
+    for (int i = 0; i < VPT; ++i) {
+      float v[8];
+      value(i, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] *= inv;
-    mine.store(static_cast<uint8_t*>(a.y) + row * a.dim, v);
-    if (threadIdx.x == 0) a.scale[row] = s;
+      for (int j = 0; j < 8; ++j) v[j] *= inv;
+      if (live) mine.store(static_cast<uint8_t*>(a.y) + row * a.dim, i, v);
+    }
+    if (live && threadIdx.x == 0) a.scale[row] = s;
   } else {
-    mine.store(static_cast<TX*>(a.y) + row * a.dim, v);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float v[8];
+      value(i, v);
+      if (live) mine.store(static_cast<TX*>(a.y) + row * a.dim, i, v);
+    }
   }
 }
 
@@ -314,59 +388,151 @@ struct BwdArgs {
   float eps;
 };
 
-// One row at a time as in the forward kernel; a block (or, for short rows, a warp) walks over
-// rows a grid apart and keeps its part of the weight's gradient in registers.  The parts are added
-// in a fixed order by colsum_kernel, so the result does not depend on timing.
-template <typename TX, typename TR, int VPT, bool VEC>
-__global__ void __launch_bounds__(max_threads(VPT)) bwd_kernel(BwdArgs a) {
+// 16 bytes from global to shared memory, past the registers.
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Bytes of shared memory a thread needs for one row's h, dy and dh.
+template <typename TX, typename TH, int VPT>
+constexpr int bwd_slot_bytes() { return VPT * 8 * (2 * (int)sizeof(TH) + (int)sizeof(TX)); }
+
+// A block (or, for short rows, part of a warp) walks over rows a grid apart and keeps its part of the
+// weight's gradient in registers; the parts are added in a fixed order by colsum_kernel, so the result
+// does not depend on timing.  VEC: a thread copies its share of the next row(s) to shared memory while
+// it works on this one (`depth` rows in turn; only the thread itself reads it, so that takes no
+// barrier), and reads it there before and after the reduction instead of holding 24 floats a group.
+template <typename TX, typename TH, int VPT, bool VEC>
+__global__ void __launch_bounds__(512, 1) bwd_kernel(BwdArgs a, int depth) {
+  extern __shared__ __align__(16) char ring[];
   __shared__ float2 s_sum[2][32];
   const Share<VPT, VEC> mine(a.dim);
+  const int threads = blockDim.x * blockDim.y, flat = threadIdx.y * blockDim.x + threadIdx.x;
   const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  // part x (16 bytes) of this thread's slot of a row: parts of one number are adjacent over threads
+  constexpr int QH = Vec8<TH>::Q, QX = Vec8<TX>::Q, PARTS = VPT * (2 * QH + QX);
+  char* const slots = ring + 16 * flat;
+  auto part_at = [&](int stage, int x) { return slots + (size_t)16 * threads * (stage * PARTS + x); };
+  auto fetch = [&](int64_t row, int stage) {
+    const TH* h = static_cast<const TH*>(a.h) + row * a.ldh;
+    const TX* dy = static_cast<const TX*>(a.dy) + row * a.lddy;
+    const TH* dh = a.dh ? static_cast<const TH*>(a.dh) + row * a.lddh : nullptr;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = 8 * (i * mine.nt + mine.t);
+      if (c >= a.dim) continue;
+#pragma unroll
+      for (int x = 0; x < QH; ++x) {
+        copy16(smem_at(part_at(stage, i * QH + x)), h + c + 16 / sizeof(TH) * x);
+        if (dh) copy16(smem_at(part_at(stage, VPT * (QH + QX) + i * QH + x)), dh + c + 16 / sizeof(TH) * x);
+      }
+#pragma unroll
+      for (int x = 0; x < QX; ++x) copy16(smem_at(part_at(stage, VPT * QH + i * QX + x)), dy + c + 16 / sizeof(TX) * x);
+    }
+  };
+  Weight<TX, VPT, VEC> w;
+  w.load(mine, a.w, a.w_f32);
   float dw[VPT][8] = {};
-  int turn = 0;
-  for (int64_t row = first; row < a.rows; row += step, turn ^= 1) {
-    float h[VPT][8], g[VPT][8], w[VPT][8];
-    mine.load(static_cast<const TR*>(a.h) + row * a.ldh, h);
-    mine.load(static_cast<const TX*>(a.dy) + row * a.lddy, g);
-    if (!a.w) {
+  // every thread of a warp takes the same number of turns (the shuffles need them all)
+  const int64_t turns = (a.rows + step - 1) / step;
+  if (VEC) {
+    for (int64_t p = 0; p < depth - 1; ++p) {
+      if (first + p * step < a.rows) fetch(first + p * step, (int)p);
+      copy_commit();
+    }
+  }
+  int stage = 0;
+  for (int64_t turn = 0; turn < turns; ++turn) {
+    const int64_t row = first + turn * step;
+    const bool live = row < a.rows;
+    Vec8<TH> hr[VEC ? 1 : VPT], dr[VEC ? 1 : VPT];
+    Vec8<TX> gr[VEC ? 1 : VPT];
+    if (VEC) {
+      const int64_t next = row + (int64_t)(depth - 1) * step;
+      int to = stage + depth - 1;
+      if (to >= depth) to -= depth;
+      if (next < a.rows) fetch(next, to);
+      copy_commit();
+      if (depth == 2) copy_wait<1>();
+      else copy_wait<0>();
+    } else if (live) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i)
+      for (int i = 0; i < VPT; ++i) {
+        mine.template load<true>(static_cast<const TH*>(a.h) + row * a.ldh, i, hr[VEC ? 0 : i]);
+        mine.template load<true>(static_cast<const TX*>(a.dy) + row * a.lddy, i, gr[VEC ? 0 : i]);
+        if (a.dh) mine.template load<true>(static_cast<const TH*>(a.dh) + row * a.lddh, i, dr[VEC ? 0 : i]);
+      }
+    }
+    // group i of the row: h, dy, dh
+    auto group = [&](int i, int which, float (&v)[8]) {
+      bool there = live;
+      if (VEC) there = live && 8 * (i * mine.nt + mine.t) < a.dim;
+      if (which == 2) there = there && a.dh;
+      if (!there) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[i][j] = 1.f;
-    } else if (a.w_f32) mine.load(static_cast<const float*>(a.w), w);
-    else mine.load(static_cast<const TX*>(a.w), w);
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      } else if (which == 1) {
+        Vec8<TX> g;
+        if (VEC) {
+#pragma unroll
+          for (int x = 0; x < QX; ++x) g.q[x] = *reinterpret_cast<const uint4*>(part_at(stage, VPT * QH + i * QX + x));
+        } else g = gr[VEC ? 0 : i];
+        unpack(g, v);
+      } else {
+        Vec8<TH> h;
+        if (VEC) {
+#pragma unroll
+          for (int x = 0; x < QH; ++x)
+            h.q[x] = *reinterpret_cast<const uint4*>(part_at(stage, (which ? VPT * (QH + QX) : 0) + i * QH + x));
+        } else h = which ? dr[VEC ? 0 : i] : hr[VEC ? 0 : i];
+        unpack(h, v);
+      }
+    };
     float hh = 0.f, gh = 0.f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
+    for (int i = 0; i < VPT; ++i) {
+      float h[8], g[8], u[8];
+      group(i, 0, h);
+      group(i, 1, g);
+      w.get(mine, a.w, a.w_f32, i, u);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        hh = fmaf(h[i][j], h[i][j], hh);
-        gh = fmaf(g[i][j] * w[i][j], h[i][j], gh);
+        hh = fmaf(h[j], h[j], hh);
+        gh = fmaf(g[j] * u[j], h[j], gh);
       }
-    // two slot sets in turn: a slow warp may still read the last row's
-    const float2 s = row_sum2(hh, gh, s_sum[turn]);
+    }
+    // two sets of slots in turn: a slow warp may still read the last row's
+    const float2 s = row_sum2(hh, gh, s_sum[turn & 1]);
     const float r = rsqrtf(s.x / a.dim + a.eps);
     const float c = r * r * r * (s.y / a.dim);
-    float d[VPT][8];
-    if (a.dh) mine.load(static_cast<const TR*>(a.dh) + row * a.lddh, d);
-    else {
+    if (live) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i)
+      for (int i = 0; i < VPT; ++i) {
+        float h[8], g[8], u[8], d[8];
+        group(i, 0, h);
+        group(i, 1, g);
+        group(i, 2, d);
+        w.get(mine, a.w, a.w_f32, i, u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[i][j] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        dw[i][j] = fmaf(g[i][j], h[i][j] * r, dw[i][j]);
-        d[i][j] += fmaf(r, g[i][j] * w[i][j], -c * h[i][j]);
+        for (int j = 0; j < 8; ++j) {
+          dw[i][j] = fmaf(g[j], h[j] * r, dw[i][j]);
+          d[j] += fmaf(r, g[j] * u[j], -c * h[j]);
+        }
+        if (a.dx) mine.store(static_cast<TX*>(a.dx) + row * a.dim, i, d);
+        if (a.dres) mine.store(static_cast<TH*>(a.dres) + row * a.dim, i, d);
       }
-    if (a.dx) mine.store(static_cast<TX*>(a.dx) + row * a.dim, d);
-    if (a.dres) mine.store(static_cast<TR*>(a.dres) + row * a.dim, d);
+    }
+    if (++stage == depth) stage = 0;
   }
-  if (a.part) mine.store(a.part + first * a.dim, dw);
+  if (a.part) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) mine.store(a.part + first * a.dim, i, dw[i]);
+  }
 }
 
 // Rows too long for registers; the partial weight gradients are added up in memory.

@@ -221,7 +221,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_backward(const at::Tenso
   if (want_dweight) dw = at::empty(w.sizes(), w.options());
   if (dy.is_meta()) return {dx, dres, dw};
   size_t bytes = 0;
-  if (want_dweight) check_rc(qrb200_rms_norm_backward_workspace_bytes(rg.rows, rg.d, &bytes), "qrb200_rms_norm_backward_workspace_bytes");
+  if (want_dweight) check_rc(qrb200_rms_norm_backward_workspace_bytes(rg.rows, rg.d, layer_code(xt), layer_code(ht), &bytes), "qrb200_rms_norm_backward_workspace_bytes");
   at::Tensor ws;
   if (bytes) ws = at::empty({(int64_t)bytes}, dy.options().dtype(at::kByte));
   check_rc(qrb200_rms_norm_backward(rg.t.data_ptr(), rg.ld, rh.t.data_ptr(), rh.ld, ptr(rd.t), rd.ld, ptr(w),

@@ -57,7 +57,7 @@ SIGNATURES = {
     "qrb200_rms_norm": (ctypes.c_int, [_P, _I64, _P, _I32, _P, _I64, _I32, _P, _P, _P, _I64, _I64,
                                        _F32, _I32, _I32, _P]),
     "qrb200_quantize_rows": (ctypes.c_int, [_P, _I64, _P, _P, _I64, _I64, _I32, _P]),
-    "qrb200_rms_norm_backward_workspace_bytes": (ctypes.c_int, [_I64, _I64, _SZP]),
+    "qrb200_rms_norm_backward_workspace_bytes": (ctypes.c_int, [_I64, _I64, _I32, _I32, _SZP]),
     "qrb200_rms_norm_backward": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I32, _P, _P, _P,
                                                 _I64, _I64, _F32, _I32, _I32, _P, _SZ, _P]),
     "qrb200_linear_workspace_bytes": (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _I64, _I64, _I64,

@@ -99,8 +99,8 @@ def test_norm_abi_checks():
     assert L.qrb200_quantize_rows(16, 8, 16, 16, 2, 8, 3, None) == bad
     assert L.qrb200_quantize_rows(None, 8, None, None, 0, 8, 0, None) == _lib.QRB200_OK
     n = ctypes.c_size_t()
-    assert L.qrb200_rms_norm_backward_workspace_bytes(4, 8, None) == bad
-    assert L.qrb200_rms_norm_backward_workspace_bytes(4, 8, ctypes.byref(n)) == _lib.QRB200_OK and n.value >= 32
+    assert L.qrb200_rms_norm_backward_workspace_bytes(4, 8, 0, 0, None) == bad
+    assert L.qrb200_rms_norm_backward_workspace_bytes(4, 8, 0, 0, ctypes.byref(n)) == _lib.QRB200_OK and n.value >= 32
     back = lambda **k: L.qrb200_rms_norm_backward(  # noqa: E731
         k.get("dy", 16), 8, k.get("h", 16), 8, None, 8, k.get("w", 16), k.get("wt", 0), 16, None, 16, k.get("rows", 2), 8, 1e-6,
         k.get("t", 0), k.get("st", 0), k.get("ws"), k.get("wsb", 0), None)
