@@ -59,13 +59,20 @@ struct Scratch {
 };
 
 // ------------------------------------------------------------------ norm
-// Threads of a row, vectors of 8 elements a thread, rows a block.  Up to 1024 elements a warp or a part
-// of one takes the row (128 threads a block).  Longer rows, 16-bit types: with enough rows to fill the
-// GPU, 4 vectors a thread (more bytes in flight, fewer barriers); with few rows, one.  float32
-// vectors take twice the registers: 2 at most.
+// Threads of a row, groups of 8 elements a thread, rows a block.  Up to 1024 elements a warp or a part
+// of one takes the row (128 threads a block).  Longer rows of 16-bit vectors: with enough rows to fill the
+// GPU, 4 groups a thread (more bytes in flight, fewer barriers); with few rows, one.  float32
+// groups take twice the registers: 2 at most.  Rows of single elements: 32, 256 or 512 threads.
 struct Shape { int nt, vpt, rows; };
-Shape norm_shape(int64_t rows, int dim, bool wide) {
+Shape single_shape(int dim, int most_256) {  // most_256: longest row that 256 threads take
+  const int nt = dim <= 1024 ? 32 : (dim <= most_256 ? 256 : 512);
+  int vpt = 1;
+  while (nt * vpt * 8 < dim) vpt *= 2;
+  return {nt, vpt, nt == 32 ? 4 : 1};
+}
+Shape norm_shape(int64_t rows, int dim, bool wide, bool vec) {
   const int vecs = (dim + 7) / 8;
+  if (!vec) return single_shape(dim, 8192);
   if (dim <= 1024 && rows > kSMs) {
     int vpt = vecs <= 32 ? 1 : (vecs <= 64 || wide ? 2 : 4), nt = 4;
     while (nt * vpt < vecs) nt *= 2;
@@ -87,13 +94,21 @@ int launch_fwd(const norm::FwdArgs& a, bool vec, cudaStream_t st) {
     norm::fwd_long_kernel<TX, TH, Q8, NORM><<<(unsigned)a.rows, norm::kMaxThreads, 0, st>>>(a);
     return launched();
   }
-  const Shape s = norm_shape(a.rows, a.dim, wide);
+  const Shape s = norm_shape(a.rows, a.dim, wide, vec);
   const dim3 block(s.nt, s.rows);
   const unsigned grid = (unsigned)((a.rows + s.rows - 1) / s.rows);
-#define QRB_FWD(V, VEC) norm::fwd_kernel<TX, TH, RES, Q8, NORM, V, VEC><<<grid, block, 0, st>>>(a)
-  if (s.vpt == 1) { if (vec) QRB_FWD(1, true); else QRB_FWD(1, false); }
-  else if (s.vpt == 2) { if (vec) QRB_FWD(2, true); else QRB_FWD(2, false); }
-  else if constexpr (!wide) { if (vec) QRB_FWD(4, true); else QRB_FWD(4, false); }
+#define QRB_FWD(V, NT) norm::fwd_kernel<TX, TH, RES, Q8, NORM, V, NT><<<grid, block, 0, st>>>(a)
+  if (vec) {
+    if (s.vpt == 1) QRB_FWD(1, 0);
+    else if (s.vpt == 2) QRB_FWD(2, 0);
+    else if constexpr (!wide) QRB_FWD(4, 0);
+  } else if (s.nt == 32) {
+    if (s.vpt == 1) QRB_FWD(1, 32); else if (s.vpt == 2) QRB_FWD(2, 32); else QRB_FWD(4, 32);
+  } else if (s.nt == 256) {
+    if (s.vpt == 1) QRB_FWD(1, 256); else if (s.vpt == 2) QRB_FWD(2, 256); else QRB_FWD(4, 256);
+  } else {
+    QRB_FWD(4, 512);
+  }
 #undef QRB_FWD
   return launched();
 }
@@ -106,44 +121,55 @@ int launch_norm(const norm::FwdArgs& a, bool q8, bool stream_f32, bool vec, cuda
 }
 
 // Shape, rows of look-ahead and grid of the backward kernel; parts = rows of partial weight gradients
-// it writes.  A block walks over its rows, so the grid is what the GPU holds at once: 128 registers a
-// thread, and shared memory for `depth` rows.
+// it writes, one a block.  A block walks over its rows, so the grid is what the GPU holds at once: 128
+// registers a thread (64 for rows of single elements up to 4096, which have no look-ahead and need
+// the warps), and shared memory for `depth` rows.  As many groups a thread as registers
+// allow: the two reductions of a row cost the same for few elements as for many.
 constexpr int kBwdRing = 220 * 1024;  // shared memory of a block at most
 struct BwdPlan { Shape s; int depth; size_t smem; int64_t grid, parts; };
-BwdPlan bwd_plan(int64_t rows, int dim, int es, int hs) {
+BwdPlan bwd_plan(int64_t rows, int dim, int es, int hs, bool vec) {
   BwdPlan p{};
   if (dim > norm::kRegDim) {
     p.s = {norm::kMaxThreads, 0, 1};
     p.grid = p.parts = std::min<int64_t>(rows, 2 * kSMs);
     return p;
   }
-  const int vecs = (dim + 7) / 8, slot = 8 * (es + 2 * hs);
-  if (dim <= 1024) {
-    int vpt = vecs <= 32 ? 1 : (vecs <= 64 ? 2 : 4), nt = 4;
-    while (nt * vpt < vecs) nt *= 2;
-    p.s = {nt, vpt, 128 / nt};
+  if (!vec) {
+    p.s = single_shape(dim, 4096);
   } else {
-    const int vpt = vecs <= 256 ? 2 : 4;
-    p.s = {((vecs + vpt - 1) / vpt + 31) / 32 * 32, vpt, 1};
+    const int vecs = (dim + 7) / 8;
+    const int vpt = vecs <= 32 ? 1 : (vecs <= 64 ? 2 : 4);
+    int nt = 4;
+    while (nt < 32 && nt * vpt < vecs) nt *= 2;
+    if (nt * vpt < vecs) nt = ((vecs + vpt - 1) / vpt + 31) / 32 * 32;
+    p.s = {nt, vpt, nt <= 32 ? 128 / nt : 1};
   }
   const int threads = p.s.nt * p.s.rows;
-  const size_t row = (size_t)threads * p.s.vpt * slot;
+  const size_t row = (size_t)threads * p.s.vpt * 8 * (es + 2 * hs);
   p.depth = 2 * row <= (size_t)kBwdRing ? 2 : 1;
-  p.smem = p.depth * row;
-  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(512 / threads, 225 * 1024 / (int64_t)(p.smem + 1536)));
-  p.grid = std::min<int64_t>((rows + p.s.rows - 1) / p.s.rows, kSMs * per_sm);
-  p.parts = p.grid * p.s.rows;
+  // the ring also holds the sums of a block's rows at the end
+  p.smem = std::max(vec ? p.depth * row : 0, p.s.rows > 1 ? (size_t)p.s.rows * dim * 4 : 0);
+  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>((!vec && threads <= 256 ? 1024 : 512) / threads, 225 * 1024 / (int64_t)(p.smem + 1536)));
+  p.grid = p.parts = std::min<int64_t>((rows + p.s.rows - 1) / p.s.rows, kSMs * per_sm);
   return p;
 }
 
-template <typename TX, typename TH, int VPT, bool VEC>
+template <typename TX, typename TH, typename TW, int VPT, int NT>
 int launch_bwd_as(const norm::BwdArgs& a, const BwdPlan& p, cudaStream_t st) {
-  auto kernel = norm::bwd_kernel<TX, TH, VPT, VEC>;
-  const size_t smem = VEC ? p.smem : 0;
+  auto kernel = norm::bwd_kernel<TX, TH, TW, VPT, NT>;
   static std::atomic<uint64_t> ready{0};
   if (const int rc = raise_smem(reinterpret_cast<const void*>(kernel), kBwdRing, ready)) return rc;
-  kernel<<<(unsigned)p.grid, dim3(p.s.nt, p.s.rows), smem, st>>>(a, p.depth);
+  kernel<<<(unsigned)p.grid, dim3(p.s.nt, p.s.rows), p.smem, st>>>(a, p.depth);
   return launched();
+}
+template <typename TX, typename TH, typename TW>
+int launch_bwd_w(const norm::BwdArgs& a, bool vec, const BwdPlan& p, cudaStream_t st) {
+#define QRB_BWD(V, NT) launch_bwd_as<TX, TH, TW, V, NT>(a, p, st)
+  if (vec) return p.s.vpt == 1 ? QRB_BWD(1, 0) : p.s.vpt == 2 ? QRB_BWD(2, 0) : QRB_BWD(4, 0);
+  if (p.s.nt == 32) return p.s.vpt == 1 ? QRB_BWD(1, 32) : p.s.vpt == 2 ? QRB_BWD(2, 32) : QRB_BWD(4, 32);
+  if (p.s.nt == 256) return p.s.vpt == 1 ? QRB_BWD(1, 256) : QRB_BWD(2, 256);
+  return p.s.vpt == 2 ? QRB_BWD(2, 512) : QRB_BWD(4, 512);
+#undef QRB_BWD
 }
 template <typename TX, typename TH>
 int launch_bwd(const norm::BwdArgs& a, bool vec, const BwdPlan& p, cudaStream_t st) {
@@ -151,9 +177,10 @@ int launch_bwd(const norm::BwdArgs& a, bool vec, const BwdPlan& p, cudaStream_t 
     norm::bwd_long_kernel<TX, TH><<<(unsigned)p.grid, norm::kMaxThreads, 0, st>>>(a);
     return launched();
   }
-  if (p.s.vpt == 1) return vec ? launch_bwd_as<TX, TH, 1, true>(a, p, st) : launch_bwd_as<TX, TH, 1, false>(a, p, st);
-  if (p.s.vpt == 2) return vec ? launch_bwd_as<TX, TH, 2, true>(a, p, st) : launch_bwd_as<TX, TH, 2, false>(a, p, st);
-  return vec ? launch_bwd_as<TX, TH, 4, true>(a, p, st) : launch_bwd_as<TX, TH, 4, false>(a, p, st);
+  if constexpr (sizeof(TX) == 2) {
+    if (a.w && a.w_f32) return launch_bwd_w<TX, TH, float>(a, vec, p, st);
+  }
+  return launch_bwd_w<TX, TH, TX>(a, vec, p, st);
 }
 
 template <typename T>
@@ -445,7 +472,10 @@ int qrb200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t dim, int32_t 
                                              size_t* bytes) {
   if (!bytes || !float_type(dtype) || !(stream_dtype == dtype || stream_dtype == QRB200_F32) || rows < 0 || dim < 0 || rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30))
     return QRB200_ERR_INVALID_ARG;
-  *bytes = rows && dim ? (size_t)bwd_plan(rows, (int)dim, esize(dtype), esize(stream_dtype)).parts * dim * sizeof(float) : 0;
+  *bytes = 0;
+  if (rows && dim)  // aligned or not
+    for (const bool vec : {false, true})
+      *bytes = std::max(*bytes, (size_t)bwd_plan(rows, (int)dim, esize(dtype), esize(stream_dtype), vec).parts * dim * sizeof(float));
   return QRB200_OK;
 }
 
@@ -467,16 +497,16 @@ int qrb200_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_
   }
   if (!dy || !h || rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30) || lddy < 0 || ldh < 0 || (dh && lddh < 0))
     return QRB200_ERR_INVALID_ARG;
-  const BwdPlan plan = bwd_plan(rows, (int)dim, esize(dtype), esize(stream_dtype));
+  const int es = esize(dtype), rs = esize(stream_dtype);
+  const bool vec = dim % 8 == 0 && rows_on16(dy, lddy, es) && rows_on16(h, ldh, rs) &&
+                   (!dh || rows_on16(dh, lddh, rs)) && (!dx || on16(dx)) && (!dresidual || on16(dresidual)) &&
+                   (!weight || on16(weight)) && on16(workspace);
+  const BwdPlan plan = bwd_plan(rows, (int)dim, es, rs, vec);
   Scratch ws(st);
   int rc = ws.get(workspace, workspace_bytes, dweight ? (size_t)plan.parts * dim * sizeof(float) : 0);
   if (rc != QRB200_OK) return rc;
   norm::BwdArgs a{dy, lddy, h, ldh, dh, lddh, weight, weight && weight_dtype == QRB200_F32, dx, dresidual,
                   static_cast<float*>(ws.p), rows, (int)dim, eps};
-  const int es = esize(dtype), rs = esize(stream_dtype);
-  const bool vec = dim % 8 == 0 && rows_on16(dy, lddy, es) && rows_on16(h, ldh, rs) &&
-                   (!dh || rows_on16(dh, lddh, rs)) && (!dx || on16(dx)) && (!dresidual || on16(dresidual)) &&
-                   (!weight || on16(weight)) && (!a.part || on16(a.part));
   const bool wide = stream_dtype == QRB200_F32 && dtype != QRB200_F32;
   if (dtype == QRB200_F32) rc = launch_bwd<float, float>(a, vec, plan, st);
   else if (dtype == QRB200_BF16)

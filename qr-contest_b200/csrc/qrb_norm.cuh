@@ -112,11 +112,15 @@ template <typename T> __device__ __forceinline__ void store1(T* p, float v) { *p
 __device__ __forceinline__ void store1(uint8_t* p, float v) { *p = to_e4m3(v); }
 
 // ---- a thread's share of a row: VPT groups of 8 elements ----
-// VEC: group i is the 8 adjacent elements from 8 (i NT + t); otherwise element (8 i + j) NT + t.
-template <int VPT, bool VEC>
+// NT == 0: rows of 16-byte vectors; group i is the 8 adjacent elements from 8 (i nt + t), nt =
+// blockDim.x.  Otherwise single elements, blockDim.x == NT: element (8 i + j) NT + t (a constant
+// distance, so that the accesses of a group need one address).
+template <int VPT, int NT>
 struct Share {
+  static constexpr bool VEC = NT == 0;
   int dim, nt, t;
-  __device__ Share(int dim_) : dim(dim_), nt(blockDim.x), t(threadIdx.x) {}
+  __device__ Share(int dim_) : dim(dim_), nt(VEC ? blockDim.x : NT), t(threadIdx.x) {}
+  __device__ __forceinline__ int column(int i, int j) const { return VEC ? 8 * (i * nt + t) + j : (8 * i + j) * NT + t; }
   // group i of a row, zero beyond its end
   template <bool STREAM, typename T>
   __device__ __forceinline__ void load(const T* row, int i, Vec8<T>& a) const {
@@ -129,10 +133,13 @@ struct Share {
       }
     } else {
       T e[8];
+      const T* p = row + 8 * i * NT + t;
+      if (8 * (i + 1) * NT <= dim) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = (8 * i + j) * nt + t;
-        e[j] = c < dim ? row[c] : from_f32<T>(0.f);
+        for (int j = 0; j < 8; ++j) e[j] = p[j * NT];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = column(i, j) < dim ? p[j * NT] : from_f32<T>(0.f);
       }
       memcpy(&a, e, sizeof(a));
     }
@@ -143,10 +150,14 @@ struct Share {
       const int c = 8 * (i * nt + t);
       if (c < dim) store8(row + c, v);
     } else {
+      T* p = row + 8 * i * NT + t;
+      if (8 * (i + 1) * NT <= dim) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = (8 * i + j) * nt + t;
-        if (c < dim) store1(row + c, v[j]);
+        for (int j = 0; j < 8; ++j) store1(p + j * NT, v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (column(i, j) < dim) store1(p + j * NT, v[j]);
       }
     }
   }
@@ -221,16 +232,16 @@ struct FwdArgs {
 
 // Group i of the weight as float32.  One in x's type waits in registers; a float32 one is read
 // from the cache where it is used.
-template <typename TX, int VPT, bool VEC>
+template <typename TX, int VPT, int NT>
 struct Weight {
   Vec8<TX> kept[VPT];
-  __device__ __forceinline__ void load(const Share<VPT, VEC>& mine, const void* w, bool f32) {
+  __device__ __forceinline__ void load(const Share<VPT, NT>& mine, const void* w, bool f32) {
     if (w && !f32) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) mine.template load<false>(static_cast<const TX*>(w), i, kept[i]);
     }
   }
-  __device__ __forceinline__ void get(const Share<VPT, VEC>& mine, const void* w, bool f32, int i, float (&v)[8]) const {
+  __device__ __forceinline__ void get(const Share<VPT, NT>& mine, const void* w, bool f32, int i, float (&v)[8]) const {
     if (!w) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = 1.f;
@@ -245,7 +256,7 @@ struct Weight {
 };
 
 // TH is the type that the norm reads: the stream's with a residual, else x's.
-template <typename TX, typename TH, bool RES, bool Q8, bool NORM, int VPT, bool VEC>
+template <typename TX, typename TH, bool RES, bool Q8, bool NORM, int VPT, int NT>
 __global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VPT)) fwd_kernel(FwdArgs a) {
   __shared__ float s_sum[32];
   __shared__ uint32_t s_max[32];
@@ -253,9 +264,9 @@ __global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VP
   const int64_t at = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const bool live = at < a.rows;
   const int64_t row = live ? at : a.rows - 1;
-  const Share<VPT, VEC> mine(a.dim);
+  const Share<VPT, NT> mine(a.dim);
   Vec8<TH> h[VPT];
-  Weight<TX, VPT, VEC> w;
+  Weight<TX, VPT, NT> w;
   if constexpr (RES) {
     Vec8<TX> x[VPT];
 #pragma unroll
@@ -382,11 +393,34 @@ struct BwdArgs {
   const void* w; int w_f32;
   void* dx;                      // in x's type
   void* dres;                    // in the stream's type where that is another one, else null
-  float* part;                   // [gridDim.x * blockDim.y][dim] partial weight gradients, or null
+  float* part;                   // [gridDim.x][dim] partial weight gradients, or null
   int64_t rows;
   int dim;
   float eps;
 };
+
+// Two float32 values in a register pair: one instruction does the arithmetic of both.
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ void pairs(const float (&v)[8], F2 (&p)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) p[j] = f2(v[2 * j], v[2 * j + 1]);
+}
 
 // 16 bytes from global to shared memory, past the registers.
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -397,52 +431,64 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Bytes of shared memory a thread needs for one row's h, dy and dh.
-template <typename TX, typename TH, int VPT>
-constexpr int bwd_slot_bytes() { return VPT * 8 * (2 * (int)sizeof(TH) + (int)sizeof(TX)); }
-
 // A block (or, for short rows, part of a warp) walks over rows a grid apart and keeps its part of the
 // weight's gradient in registers; the parts are added in a fixed order by colsum_kernel, so the result
-// does not depend on timing.  VEC: a thread copies its share of the next row(s) to shared memory while
-// it works on this one (`depth` rows in turn; only the thread itself reads it, so that takes no
-// barrier), and reads it there before and after the reduction instead of holding 24 floats a group.
-template <typename TX, typename TH, int VPT, bool VEC>
-__global__ void __launch_bounds__(512, 1) bwd_kernel(BwdArgs a, int depth) {
+// does not depend on timing.  Rows of vectors (NT == 0): a thread copies its share of the next row to
+// shared memory while it works on this one (`depth` rows in turn; only the thread itself reads it, so
+// that takes no barrier), and reads it there before and after the reduction instead of holding 24
+// floats a group.  What lies past a row's end, past the last row, or in an absent dh is zero there, so
+// the arithmetic asks nothing: with questions in it the kernel was bound by its instructions.
+template <typename TX, typename TH, typename TW, int VPT, int NT>
+__global__ void __launch_bounds__(NT == 32 ? 128 : NT == 256 ? 256 : 512, NT == 32 ? 8 : NT == 256 ? 4 : 1)
+    bwd_kernel(BwdArgs a, int depth) {
+  constexpr bool VEC = NT == 0;
   extern __shared__ __align__(16) char ring[];
   __shared__ float2 s_sum[2][32];
-  const Share<VPT, VEC> mine(a.dim);
+  const Share<VPT, NT> mine(a.dim);
   const int threads = blockDim.x * blockDim.y, flat = threadIdx.y * blockDim.x + threadIdx.x;
   const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
-  // part x (16 bytes) of this thread's slot of a row: parts of one number are adjacent over threads
+  // 16-byte part x of this thread's slot of a row (h, dh, dy in this order); the parts of one x are
+  // adjacent over the threads
   constexpr int QH = Vec8<TH>::Q, QX = Vec8<TX>::Q, PARTS = VPT * (2 * QH + QX);
+  const int pitch = 16 * threads;
   char* const slots = ring + 16 * flat;
-  auto part_at = [&](int stage, int x) { return slots + (size_t)16 * threads * (stage * PARTS + x); };
+  auto zero_slot = [&](int stage) {
+    for (int x = 0; x < PARTS; ++x) *reinterpret_cast<uint4*>(slots + (stage * PARTS + x) * pitch) = make_uint4(0, 0, 0, 0);
+  };
   auto fetch = [&](int64_t row, int stage) {
-    const TH* h = static_cast<const TH*>(a.h) + row * a.ldh;
-    const TX* dy = static_cast<const TX*>(a.dy) + row * a.lddy;
-    const TH* dh = a.dh ? static_cast<const TH*>(a.dh) + row * a.lddh : nullptr;
+    const TH* h = static_cast<const TH*>(a.h) + row * a.ldh + 8 * mine.t;
+    const TX* dy = static_cast<const TX*>(a.dy) + row * a.lddy + 8 * mine.t;
+    const TH* dh = static_cast<const TH*>(a.dh) + row * a.lddh + 8 * mine.t;
+    const uint32_t to = smem_at(slots + stage * PARTS * pitch);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = 8 * (i * mine.nt + mine.t);
-      if (c >= a.dim) continue;
+      const int c = 8 * i * mine.nt;
+      if (c + 8 * mine.t >= a.dim) continue;
 #pragma unroll
       for (int x = 0; x < QH; ++x) {
-        copy16(smem_at(part_at(stage, i * QH + x)), h + c + 16 / sizeof(TH) * x);
-        if (dh) copy16(smem_at(part_at(stage, VPT * (QH + QX) + i * QH + x)), dh + c + 16 / sizeof(TH) * x);
+        copy16(to + (i * QH + x) * pitch, h + c + 16 / sizeof(TH) * x);
+        if (a.dh) copy16(to + (VPT * QH + i * QH + x) * pitch, dh + c + 16 / sizeof(TH) * x);
       }
 #pragma unroll
-      for (int x = 0; x < QX; ++x) copy16(smem_at(part_at(stage, VPT * QH + i * QX + x)), dy + c + 16 / sizeof(TX) * x);
+      for (int x = 0; x < QX; ++x) copy16(to + (2 * VPT * QH + i * QX + x) * pitch, dy + c + 16 / sizeof(TX) * x);
     }
   };
-  Weight<TX, VPT, VEC> w;
-  w.load(mine, a.w, a.w_f32);
-  float dw[VPT][8] = {};
+  Vec8<TW> w[VPT];
+  F2 dw[VPT][4];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (a.w) mine.template load<false>(static_cast<const TW*>(a.w), i, w[i]);
+    else pack(w[i], {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f});
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dw[i][j] = f2(0.f, 0.f);
+  }
   // every thread of a warp takes the same number of turns (the shuffles need them all)
   const int64_t turns = (a.rows + step - 1) / step;
   if (VEC) {
-    for (int64_t p = 0; p < depth - 1; ++p) {
-      if (first + p * step < a.rows) fetch(first + p * step, (int)p);
+    for (int p = 0; p < depth; ++p) zero_slot(p);
+    if (depth == 2) {
+      if (first < a.rows) fetch(first, 0);
       copy_commit();
     }
   }
@@ -452,86 +498,123 @@ __global__ void __launch_bounds__(512, 1) bwd_kernel(BwdArgs a, int depth) {
     const bool live = row < a.rows;
     Vec8<TH> hr[VEC ? 1 : VPT], dr[VEC ? 1 : VPT];
     Vec8<TX> gr[VEC ? 1 : VPT];
+    const char* from = slots + stage * PARTS * pitch;
     if (VEC) {
-      const int64_t next = row + (int64_t)(depth - 1) * step;
-      int to = stage + depth - 1;
-      if (to >= depth) to -= depth;
+      const int64_t next = row + (depth - 1) * step;
+      const int to = depth == 2 ? stage ^ 1 : 0;
       if (next < a.rows) fetch(next, to);
+      else zero_slot(to);
       copy_commit();
       if (depth == 2) copy_wait<1>();
       else copy_wait<0>();
-    } else if (live) {
+    } else {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        mine.template load<true>(static_cast<const TH*>(a.h) + row * a.ldh, i, hr[VEC ? 0 : i]);
-        mine.template load<true>(static_cast<const TX*>(a.dy) + row * a.lddy, i, gr[VEC ? 0 : i]);
-        if (a.dh) mine.template load<true>(static_cast<const TH*>(a.dh) + row * a.lddh, i, dr[VEC ? 0 : i]);
+        const int x = VEC ? 0 : i;
+        hr[x] = dr[x] = Vec8<TH>{};
+        gr[x] = Vec8<TX>{};
+        if (live) {
+          mine.template load<true>(static_cast<const TH*>(a.h) + row * a.ldh, i, hr[x]);
+          mine.template load<true>(static_cast<const TX*>(a.dy) + row * a.lddy, i, gr[x]);
+          if (a.dh) mine.template load<true>(static_cast<const TH*>(a.dh) + row * a.lddh, i, dr[x]);
+        }
       }
     }
-    // group i of the row: h, dy, dh
-    auto group = [&](int i, int which, float (&v)[8]) {
-      bool there = live;
-      if (VEC) there = live && 8 * (i * mine.nt + mine.t) < a.dim;
-      if (which == 2) there = there && a.dh;
-      if (!there) {
+    // group i of the row: h (0) or dh (1), and dy
+    auto stream = [&](int i, int which, F2 (&p)[4]) {
+      Vec8<TH> h;
+      if (VEC) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.f;
-      } else if (which == 1) {
-        Vec8<TX> g;
-        if (VEC) {
-#pragma unroll
-          for (int x = 0; x < QX; ++x) g.q[x] = *reinterpret_cast<const uint4*>(part_at(stage, VPT * QH + i * QX + x));
-        } else g = gr[VEC ? 0 : i];
-        unpack(g, v);
-      } else {
-        Vec8<TH> h;
-        if (VEC) {
-#pragma unroll
-          for (int x = 0; x < QH; ++x)
-            h.q[x] = *reinterpret_cast<const uint4*>(part_at(stage, (which ? VPT * (QH + QX) : 0) + i * QH + x));
-        } else h = which ? dr[VEC ? 0 : i] : hr[VEC ? 0 : i];
-        unpack(h, v);
-      }
+        for (int x = 0; x < QH; ++x) h.q[x] = *reinterpret_cast<const uint4*>(from + (which * VPT * QH + i * QH + x) * pitch);
+      } else h = which ? dr[VEC ? 0 : i] : hr[VEC ? 0 : i];
+      float v[8];
+      unpack(h, v);
+      pairs(v, p);
     };
-    float hh = 0.f, gh = 0.f;
+    auto grad = [&](int i, F2 (&p)[4]) {
+      Vec8<TX> g;
+      if (VEC) {
+#pragma unroll
+        for (int x = 0; x < QX; ++x) g.q[x] = *reinterpret_cast<const uint4*>(from + (2 * VPT * QH + i * QX + x) * pitch);
+      } else g = gr[VEC ? 0 : i];
+      float v[8];
+      unpack(g, v);
+      pairs(v, p);
+    };
+    auto weight = [&](int i, F2 (&p)[4]) {
+      float v[8];
+      unpack(w[i], v);
+      pairs(v, p);
+    };
+    F2 hh2 = f2(0.f, 0.f), gh2 = hh2;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      float h[8], g[8], u[8];
-      group(i, 0, h);
-      group(i, 1, g);
-      w.get(mine, a.w, a.w_f32, i, u);
+      F2 h[4], g[4], u[4];
+      stream(i, 0, h);
+      grad(i, g);
+      weight(i, u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        hh = fmaf(h[j], h[j], hh);
-        gh = fmaf(g[j] * u[j], h[j], gh);
+      for (int j = 0; j < 4; ++j) {
+        hh2 = fma(h[j], h[j], hh2);
+        gh2 = fma(mul(g[j], u[j]), h[j], gh2);
       }
     }
+    float hh, gh, hh1, gh1;
+    split(hh2, hh, hh1);
+    split(gh2, gh, gh1);
     // two sets of slots in turn: a slow warp may still read the last row's
-    const float2 s = row_sum2(hh, gh, s_sum[turn & 1]);
+    const float2 s = row_sum2(hh + hh1, gh + gh1, s_sum[turn & 1]);
     const float r = rsqrtf(s.x / a.dim + a.eps);
     const float c = r * r * r * (s.y / a.dim);
-    if (live) {
+    const F2 r2 = f2(r, r), c2 = f2(-c, -c);
+    TX* const dx = live ? static_cast<TX*>(a.dx) + row * a.dim : nullptr;
+    TH* const dres = live ? static_cast<TH*>(a.dres) + row * a.dim : nullptr;
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        float h[8], g[8], u[8], d[8];
-        group(i, 0, h);
-        group(i, 1, g);
-        group(i, 2, d);
-        w.get(mine, a.w, a.w_f32, i, u);
+    for (int i = 0; i < VPT; ++i) {
+      F2 h[4], g[4], u[4], e[4];
+      float d[8];
+      stream(i, 0, h);
+      grad(i, g);
+      stream(i, 1, e);
+      weight(i, u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          dw[i][j] = fmaf(g[j], h[j] * r, dw[i][j]);
-          d[j] += fmaf(r, g[j] * u[j], -c * h[j]);
-        }
-        if (a.dx) mine.store(static_cast<TX*>(a.dx) + row * a.dim, i, d);
-        if (a.dres) mine.store(static_cast<TH*>(a.dres) + row * a.dim, i, d);
+      for (int j = 0; j < 4; ++j) {
+        const F2 gr2 = mul(g[j], r2);
+        if (live) dw[i][j] = fma(gr2, h[j], dw[i][j]);
+        split(fma(gr2, u[j], fma(c2, h[j], e[j])), d[2 * j], d[2 * j + 1]);
       }
+      if (live && a.dx) mine.store(dx, i, d);
+      if (live && a.dres) mine.store(dres, i, d);
     }
-    if (++stage == depth) stage = 0;
+    if (VEC && depth == 2) stage ^= 1;
   }
-  if (a.part) {
+  if (!a.part) return;
+  float sum[VPT][8];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) mine.store(a.part + first * a.dim, i, dw[i]);
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split(dw[i][j], sum[i][2 * j], sum[i][2 * j + 1]);
+  if (blockDim.y == 1) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) mine.store(a.part + (int64_t)blockIdx.x * a.dim, i, sum[i]);
+    return;
+  }
+  // several rows a block: their parts are added through shared memory (the ring, or its size)
+  copy_wait<0>();
+  __syncthreads();
+  float* const sums = reinterpret_cast<float*>(ring);  // [blockDim.y][dim]
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = mine.column(i, j);
+      if (c < a.dim) sums[threadIdx.y * a.dim + c] = sum[i][j];
+    }
+  __syncthreads();
+  for (int c = flat; c < a.dim; c += threads) {
+    float v = 0.f;
+    for (int y = 0; y < (int)blockDim.y; ++y) v += sums[y * a.dim + c];
+    a.part[(int64_t)blockIdx.x * a.dim + c] = v;
   }
 }
 
@@ -574,8 +657,10 @@ __global__ void __launch_bounds__(1024) colsum_kernel(const float* part, int64_t
   __shared__ float s[32][33];
   const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
   float v = 0.f;
-  if (c < cols)
+  if (c < cols) {
+#pragma unroll 8
     for (int64_t p = threadIdx.y; p < parts; p += 32) v += part[p * cols + c];
+  }
   s[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   float t = s[threadIdx.x][threadIdx.y];

@@ -18,7 +18,9 @@
 // TypeError before anything is allocated.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include "qrb200.h"
@@ -137,6 +139,11 @@ std::vector<int64_t> with_last(const at::Tensor& x, int64_t d) {
   s.back() = d;
   return s;
 }
+// A new contiguous tensor beside `like`.
+at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType t) {
+  return like.is_cuda() ? at::detail::empty_cuda(sizes, t, like.device(), c10::nullopt)
+                        : at::empty(sizes, like.options().dtype(t));
+}
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* cur_stream(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
@@ -168,9 +175,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm(const at::Tensor& x, con
   }
   const c10::OptionalDeviceGuard guard(x.is_cuda() ? c10::optional<c10::Device>(x.device()) : c10::nullopt);
   const Rows rx = as_rows(x), rr = residual ? as_rows(*residual) : Rows{{}, 0, 0, 0};
-  at::Tensor y = at::empty(x.sizes(), x.options().dtype(ot)), scale, h;
-  if (ot == at::kFloat8_e4m3fn) scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
-  if (residual) h = at::empty(x.sizes(), residual->options());
+  at::Tensor y = fresh(x.sizes(), x, ot), scale, h;
+  if (ot == at::kFloat8_e4m3fn) scale = fresh(x.sizes().slice(0, x.dim() - 1), x, at::kFloat);
+  if (residual) h = fresh(x.sizes(), x, residual->scalar_type());
   if (x.is_meta()) return {y, scale, h};
   check_rc(qrb200_rms_norm(rx.t.data_ptr(), rx.ld, ptr(w), w.defined() ? layer_code(w.scalar_type()) : 0, ptr(rr.t), rr.ld,
                            residual ? layer_code(residual->scalar_type()) : 0, y.data_ptr(),
@@ -186,8 +193,8 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x) {
   check_type(native(x.scalar_type()), "x", x.scalar_type());
   const c10::OptionalDeviceGuard guard(x.is_cuda() ? c10::optional<c10::Device>(x.device()) : c10::nullopt);
   const Rows r = as_rows(x);
-  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-  at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  at::Tensor q = fresh(x.sizes(), x, at::kFloat8_e4m3fn);
+  at::Tensor scale = fresh(x.sizes().slice(0, x.dim() - 1), x, at::kFloat);
   if (x.is_meta()) return {q, scale};
   check_rc(qrb200_quantize_rows(r.t.data_ptr(), r.ld, q.data_ptr(), scale.data_ptr<float>(), r.rows, r.d,
                                 layer_code(x.scalar_type()), cur_stream(x)),
@@ -216,14 +223,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_backward(const at::Tenso
   const c10::OptionalDeviceGuard guard(dy.is_cuda() ? c10::optional<c10::Device>(dy.device()) : c10::nullopt);
   const Rows rg = as_rows(dy), rh = as_rows(h), rd = dh ? as_rows(*dh) : Rows{{}, 0, 0, 0};
   at::Tensor dx, dres, dw;
-  if (want_dx || (want_dresidual && ht == xt)) dx = at::empty(dy.sizes(), dy.options());
-  if (want_dresidual) dres = ht == xt ? dx : at::empty(dy.sizes(), h.options());
-  if (want_dweight) dw = at::empty(w.sizes(), w.options());
+  if (want_dx || (want_dresidual && ht == xt)) dx = fresh(dy.sizes(), dy, xt);
+  if (want_dresidual) dres = ht == xt ? dx : fresh(dy.sizes(), dy, ht);
+  if (want_dweight) dw = fresh(w.sizes(), dy, w.scalar_type());
   if (dy.is_meta()) return {dx, dres, dw};
   size_t bytes = 0;
   if (want_dweight) check_rc(qrb200_rms_norm_backward_workspace_bytes(rg.rows, rg.d, layer_code(xt), layer_code(ht), &bytes), "qrb200_rms_norm_backward_workspace_bytes");
   at::Tensor ws;
-  if (bytes) ws = at::empty({(int64_t)bytes}, dy.options().dtype(at::kByte));
+  if (bytes) ws = fresh({(int64_t)bytes}, dy, at::kByte);
   check_rc(qrb200_rms_norm_backward(rg.t.data_ptr(), rg.ld, rh.t.data_ptr(), rh.ld, ptr(rd.t), rd.ld, ptr(w),
                                     w.defined() ? layer_code(w.scalar_type()) : 0, ptr(dx), ht == xt ? nullptr : ptr(dres),
                                     ptr(dw), rg.rows, rg.d, (float)eps, layer_code(xt), layer_code(ht), ptr(ws), bytes,
@@ -288,14 +295,14 @@ std::tuple<at::Tensor, at::Tensor> linear(const at::Tensor& x, const at::Tensor&
   const Weight w = as_weight(weight, !q8);
   const at::Tensor b = bias ? bias->contiguous() : at::Tensor();
   const at::Tensor xs = row_scales(x_scale, x, rx.rows, "x_scale"), wsc = row_scales(weight_scale, x, n, "weight_scale");
-  at::Tensor y = at::empty(shape, x.options().dtype(ot)), slope;
-  if (want_slope) slope = at::empty(shape, x.options().dtype(at::kShort));
+  at::Tensor y = fresh(shape, x, ot), slope;
+  if (want_slope) slope = fresh(shape, x, at::kShort);
   if (x.is_meta()) return {y, slope};
   size_t bytes = 0;
   check_rc(qrb200_linear_workspace_bytes(rx.t.data_ptr(), rx.ld, w.t.data_ptr(), w.ld, w.transposed, rx.rows, n, k, layer_code(xt), &bytes),
            "qrb200_linear_workspace_bytes");
   at::Tensor ws;
-  if (bytes) ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+  if (bytes) ws = fresh({(int64_t)bytes}, x, at::kByte);
   check_rc(qrb200_linear(rx.t.data_ptr(), rx.ld, w.t.data_ptr(), w.ld, w.transposed, static_cast<const float*>(ptr(xs)),
                          static_cast<const float*>(ptr(wsc)), ptr(b), ptr(rr.t), rr.ld, y.data_ptr(), n,
                          static_cast<int16_t*>(ptr(slope)), rx.rows, n, k, layer_code(xt), layer_code(ot), (int32_t)activation,
@@ -327,21 +334,125 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward(const at::Tensor&
   const Rows rg = as_rows(dy, true), rx = as_rows(x, true);
   const Weight w = as_weight(weight, true);
   at::Tensor dx, dw, db;
-  if (want_dx) dx = at::empty(x.sizes(), x.options());
-  if (want_dweight) dw = at::empty(weight.sizes(), weight.options());
-  if (want_dbias) db = at::empty({n}, dy.options());
+  if (want_dx) dx = fresh(x.sizes(), x, t);
+  if (want_dweight) dw = fresh(weight.sizes(), x, t);
+  if (want_dbias) db = fresh({n}, dy, t);
   if (dy.is_meta()) return {dx, dw, db};
   size_t bytes = 0;
   check_rc(qrb200_linear_backward_workspace_bytes(rg.t.data_ptr(), rg.ld, slope.has_value(), rx.t.data_ptr(), rx.ld, w.t.data_ptr(),
                                                   w.ld, w.transposed, want_dx, want_dweight, want_dbias, rg.rows, n, k, &bytes),
            "qrb200_linear_backward_workspace_bytes");
   at::Tensor ws;
-  if (bytes) ws = at::empty({(int64_t)bytes}, dy.options().dtype(at::kByte));
+  if (bytes) ws = fresh({(int64_t)bytes}, dy, at::kByte);
   check_rc(qrb200_linear_backward(rg.t.data_ptr(), rg.ld, slope ? static_cast<const int16_t*>(slope->data_ptr()) : nullptr,
                                   rx.t.data_ptr(), rx.ld, w.t.data_ptr(), w.ld, w.transposed, ptr(dx), ptr(dw), ptr(db),
                                   rg.rows, n, k, layer_code(t), ptr(ws), bytes, cur_stream(dy)),
            "qrb200_linear_backward");
   return {dx, dw, db};
+}
+
+// ---- gradients ----
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+OptTensor given(const at::Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
+bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+void check_once() {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), "qrb200: the layer operators are differentiable once (no create_graph)");
+}
+
+struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& weight,
+                               const OptTensor& residual, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->set_materialize_grads(false);
+    auto [y, scale, h] = rms_norm(x, weight, residual, eps, c10::nullopt);
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->saved_data["type"] = x.scalar_type();
+    ctx->save_for_backward({h.defined() ? h : x, weight.value_or(at::Tensor())});
+    return h.defined() ? variable_list{y, h} : variable_list{y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once();
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &h = saved[0], &weight = saved[1];
+    at::Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : at::Tensor();
+    // inputs that were given, in order, have an edge each
+    size_t edge = 0;
+    const bool want_x = ctx->needs_input_grad(edge++);
+    const bool want_w = weight.defined() && ctx->needs_input_grad(edge++);
+    const bool want_r = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(edge++);
+    if (!dy.defined()) {
+      if (!dh.defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+      dy = at::zeros(h.sizes(), h.options().dtype(ctx->saved_data["type"].toScalarType()));
+    }
+    auto [dx, dres, dw] = rms_norm_backward(dy, h, given(dh), given(weight), ctx->saved_data["eps"].toDouble(), want_x, want_r, want_w);
+    return {want_x ? dx : at::Tensor(), dw, dres, at::Tensor()};
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_autograd(const at::Tensor& x, const OptTensor& weight,
+                                                                 const OptTensor& residual, double eps,
+                                                                 c10::optional<at::ScalarType> out_dtype) {
+  const at::Tensor w = weight.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
+  if (!wants_grad({&x, &w, &r})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return rms_norm(x, weight, residual, eps, out_dtype);
+  }
+  TORCH_CHECK_VALUE(!out_dtype || *out_dtype == x.scalar_type(), "qrb200: the 8-bit norm has no gradient (use torch.no_grad())");
+  variable_list out = RmsNormGrad::apply(x, weight, residual, eps);
+  return {out[0], at::Tensor(), out.size() > 1 ? out[1] : at::Tensor()};
+}
+
+struct LinearGrad : torch::autograd::Function<LinearGrad> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
+                               const OptTensor& residual, int64_t activation, c10::optional<at::ScalarType> out_dtype) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->set_materialize_grads(false);
+    const bool sums = x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad());
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    auto [y, slope] = linear(x, weight, bias, residual, activation, c10::nullopt, c10::nullopt, out_dtype,
+                             sums && activation != QRB200_ACT_NONE);
+    if (sums) ctx->save_for_backward({x, weight, slope});
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once();
+    variable_list out(6);
+    const at::Tensor& dy = grads[0];
+    if (!dy.defined()) return out;
+    size_t edge = 0;
+    const bool want_x = ctx->needs_input_grad(edge++), want_w = ctx->needs_input_grad(edge++);
+    const bool want_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(edge++);
+    const bool want_r = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(edge++);
+    if (want_x || want_w || want_b) {
+      const auto saved = ctx->get_saved_variables();
+      std::tie(out[0], out[1], out[2]) = linear_backward(dy, given(saved[2]), saved[0], saved[1], want_x, want_w, want_b);
+    }
+    if (want_r) out[3] = dy;
+    return out;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> linear_autograd(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
+                                                   const OptTensor& residual, int64_t activation, const OptTensor& x_scale,
+                                                   const OptTensor& weight_scale, c10::optional<at::ScalarType> out_dtype,
+                                                   bool want_slope) {
+  const at::Tensor b = bias.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
+  if (!wants_grad({&x, &weight, &b, &r})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return linear(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
+  }
+  TORCH_CHECK_VALUE(x.scalar_type() != at::kFloat8_e4m3fn, "qrb200: the 8-bit product has no gradient (use torch.no_grad())");
+  TORCH_CHECK_VALUE(!x_scale && !weight_scale, "qrb200: scales belong to 8-bit operands");
+  return {LinearGrad::apply(x, weight, bias, residual, activation, out_dtype)[0], at::Tensor()};
 }
 
 }  // namespace
@@ -374,6 +485,11 @@ TORCH_LIBRARY_IMPL(qrb200, CUDA, m) {
 TORCH_LIBRARY_IMPL(qrb200, Meta, m) {
   m.impl("geqrf", geqrf_meta);
   layer_impls(m);
+}
+
+TORCH_LIBRARY_IMPL(qrb200, Autograd, m) {
+  m.impl("rms_norm", rms_norm_autograd);
+  m.impl("linear", linear_autograd);
 }
 
 // Host tensors (and mixes of host and device tensors, which reach this key too) are refused by the

@@ -10,13 +10,12 @@ held in 8 bits.
 All take CUDA tensors, run on the current stream without synchronising, and raise ``TypeError`` or
 ``ValueError`` on arguments they do not take.  Leading dimensions are free; rows may be slices or
 expanded views (one row stride: read in place, anything else is copied first).  ``rms_norm`` and
-``linear`` are differentiable once in every floating input where all types are 16 bits or more; the
-same inputs give the same bits.
+``linear`` are differentiable once in every floating input where all types are 16 bits or more (the
+operators' own autograd formulas, in C++); the same inputs give the same bits.
 """
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, api
 
@@ -42,32 +41,6 @@ class _Ops:
         cls.loaded = True
 
 
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-class _RmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        ctx.set_materialize_grads(False)
-        y, _, h = _Ops.rms_norm(x, weight, residual, eps, None)
-        ctx.eps, ctx.dtype = eps, x.dtype
-        ctx.save_for_backward(x if residual is None else h, weight)
-        return y if residual is None else (y, h)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh=None):
-        h, weight = ctx.saved_tensors
-        want_x, want_w, want_r, _ = ctx.needs_input_grad
-        if dy is None:
-            if dh is None:
-                return None, None, None, None
-            dy = torch.zeros(h.shape, dtype=ctx.dtype, device=h.device)
-        dx, dres, dw = _Ops.rms_norm_backward(dy, h, dh, weight, ctx.eps, want_x, want_r, want_w)
-        return dx if want_x else None, dw, dres, None
-
-
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
              eps: float = 1e-6, out_dtype: torch.dtype | None = None):
     """``h = x + residual``; ``y = h * (mean(h**2, -1) + eps)**-0.5 * weight``.
@@ -80,10 +53,6 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
     """
     if not _Ops.loaded:
         _Ops.load()
-    if _wants_grad(x, weight, residual):
-        if out_dtype is not None and out_dtype != x.dtype:
-            raise ValueError("qrb200: the 8-bit norm has no gradient (use torch.no_grad())")
-        return _RmsNorm.apply(x, weight, residual, eps)
     y, scale, h = _Ops.rms_norm(x, weight, residual, eps, out_dtype)
     if scale is None:
         return y if h is None else (y, h)
@@ -97,27 +66,6 @@ def quantize_rows(x: torch.Tensor):
     if not _Ops.loaded:
         _Ops.load()
     return _Ops.quantize_rows(x)
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation, out_dtype):
-        need = any(ctx.needs_input_grad[:3])
-        y, slope = _Ops.linear(x, weight, bias, residual, activation, None, None, out_dtype,
-                               need and activation != _lib.ACT_NONE)
-        if need:
-            ctx.save_for_backward(x, weight, slope)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        want_x, want_w, want_b, want_r, _, _ = ctx.needs_input_grad
-        dx = dw = db = None
-        if want_x or want_w or want_b:
-            x, weight, slope = ctx.saved_tensors
-            dx, dw, db = _Ops.linear_backward(dy, slope, x, weight, want_x, want_w, want_b)
-        return dx, dw, db, dy if want_r else None, None, None
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -138,10 +86,4 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         act = _ACTIVATIONS[activation]
     except (KeyError, TypeError):
         raise ValueError(f"qrb200: unknown activation {activation!r}") from None
-    if _wants_grad(x, weight, bias, residual):
-        if x.dtype == _FP8:
-            raise ValueError("qrb200: the 8-bit product has no gradient (use torch.no_grad())")
-        if x_scale is not None or weight_scale is not None:
-            raise ValueError("qrb200: scales belong to 8-bit operands")
-        return _Linear.apply(x, weight, bias, residual, act, out_dtype)
     return _Ops.linear(x, weight, bias, residual, act, x_scale, weight_scale, out_dtype, False)[0]
