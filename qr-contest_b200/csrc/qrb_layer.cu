@@ -339,11 +339,30 @@ int product_pair(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64
             : launch_pair<__half, 2, TN, false>(P, Q, m, n, k, dtype, e, st);
 }
 
+// A few tokens, W's features in rows: token_kernel.  SPLIT as there are too few features for the GPU
+// (8 warps an SM at one feature a warp).
+constexpr int64_t kTokens = 4;
+template <typename Out, typename In, int M, bool VEC>
+int launch_token(const lin::TokenArgs& a, cudaStream_t st) {
+  if (a.n >= 2 * 8 * kSMs) lin::token_kernel<Out, In, M, 2, 1, VEC><<<(a.n + 15) / 16, 256, 0, st>>>(a);
+  else if (a.n >= 8 * kSMs || a.k <= 2048) lin::token_kernel<Out, In, M, 1, 1, VEC><<<(a.n + 7) / 8, 256, 0, st>>>(a);
+  else lin::token_kernel<Out, In, M, 1, 8, VEC><<<a.n, 256, 0, st>>>(a);
+  return launched();
+}
+template <typename Out, typename In>
+int product_token(const lin::TokenArgs& a, cudaStream_t st) {
+  const bool vec = a.k % (16 / sizeof(In)) == 0 && rows_on16(a.w, a.n > 1 ? a.ldw : 0, sizeof(In)) &&
+                   rows_on16(a.x, a.m > 1 ? a.ldx : 0, sizeof(In));
+  if (a.m == 1) return vec ? launch_token<Out, In, 1, true>(a, st) : launch_token<Out, In, 1, false>(a, st);
+  if (a.m == 2) return vec ? launch_token<Out, In, 2, true>(a, st) : launch_token<Out, In, 2, false>(a, st);
+  return vec ? launch_token<Out, In, 4, true>(a, st) : launch_token<Out, In, 4, false>(a, st);
+}
+
 // D = epilogue(P Q^T); P is m x k, Q is n x k, both addressable by TMA.
 int product(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t out_dtype,
             const lin::Epilogue& e, cudaStream_t st) {
   // Enough 256 x 256 tiles for most of the 74 CTA pairs: the persistent kernel.
-  if (k > 0 && ((m + 255) / 256) * ((n + 255) / 256) >= kPairTiles) return product_pair<256>(P, Q, m, n, k, dtype, out_dtype, e, st);
+  if (k > 0 && m > 128 && ((m + 255) / 256) * ((n + 255) / 256) >= kPairTiles) return product_pair<256>(P, Q, m, n, k, dtype, out_dtype, e, st);
   lin::Args a{};
   a.m = (int)m; a.n = (int)n; a.k = (int)k;
   a.e = e;
@@ -546,6 +565,12 @@ int qrb200_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int es = esize(dtype);
   Operand X{x, ldx, false}, W{w, ldw, w_transposed != 0};
+  lin::Epilogue e{x_scale, w_scale, bias, residual, ldr, y, ldy, slope, activation};
+  if (m <= kTokens && !w_transposed && !slope && k > 0) {
+    const lin::TokenArgs t{x, ldx, w, ldw, (int)m, (int)n, (int)k, e};
+    if (q8) return out_dtype == QRB200_BF16 ? product_token<__nv_bfloat16, __nv_fp8_e4m3>(t, st) : product_token<__half, __nv_fp8_e4m3>(t, st);
+    return dtype == QRB200_BF16 ? product_token<__nv_bfloat16, __nv_bfloat16>(t, st) : product_token<__half, __half>(t, st);
+  }
   Scratch ws(st);
   int rc = ws.get(workspace, workspace_bytes,
                   k ? aligned_copy_bytes(X, m, k, es) + aligned_copy_bytes(W, n, k, es) : 0);
@@ -553,7 +578,6 @@ int qrb200_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_
   if (rc == QRB200_OK && k) rc = make_addressable(X, m, k, es, buf, st);
   if (rc == QRB200_OK && k) rc = make_addressable(W, n, k, es, buf, st);
   if (rc != QRB200_OK) return rc;
-  lin::Epilogue e{x_scale, w_scale, bias, residual, ldr, y, ldy, slope, activation};
   return product(X, W, m, n, k, dtype, out_dtype, e, st);
 }
 

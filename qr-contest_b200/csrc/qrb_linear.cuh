@@ -15,6 +15,8 @@
 //              1024 between groups of 8 k, 8192 between chunks; the next 16 k start 2048 bytes on.
 // Boxes that reach past an edge are filled with zeros, which add nothing.
 #pragma once
+#include <cuda_fp8.h>
+
 #include "qrb_tc.cuh"
 #include "qrb_tmap.cuh"
 
@@ -63,7 +65,24 @@ __device__ __forceinline__ float slope_from_fixed(int16_t f) {
   return f == -32768 ? __int_as_float(0x7FFFFFFF) : (float)f * (1.f / kSlopeOne);
 }
 
-// act(z); with SLOPE also act'(z).
+// 1 / x and 2^x of the special-function unit, good to about 2^-22 of the result.
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float exp_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+
+// act(z); with SLOPE also act'(z).  The epilogue runs beside the MMAs and shares their power, so
+// each costs two special functions and a dozen multiply-adds: gelu takes the normal integral from
+// Abramowitz and Stegun's approximation 7.1.26 of the error function (off by 1.5e-7 at most),
+//   Phi(-|z|) = exp(-z^2 / 2) (a1 t + ... + a5 t^5) / 2,  t = 1 / (1 + p |z| / sqrt 2),
+// whose exponential is also the one that its slope needs (4096 x 16384 x 4096 with gelu: 431 us with
+// erff, see the table of measurements for the present figure).
 template <bool SLOPE>
 __device__ __forceinline__ float activate(int act, float z, float& slope) {
   switch (act) {
@@ -71,24 +90,48 @@ __device__ __forceinline__ float activate(int act, float z, float& slope) {
       if (SLOPE) slope = z > 0.f ? 1.f : (z != z ? z : 0.f);
       return z < 0.f ? 0.f : z;  // NaN stays
     case ACT_GELU: {
-      const float phi = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-      if (SLOPE) slope = phi + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+      const float x = fabsf(z) * 0.70710678118654752f;
+      const float t = rcp_fast(fmaf(0.3275911f, x, 1.f));
+      const float ex = exp_fast(-x * x);
+      float s = fmaf(1.061405429f, t, -1.453152027f);
+      s = fmaf(s, t, 1.421413741f);
+      s = fmaf(s, t, -0.284496736f);
+      s = fmaf(s, t, 0.254829592f);
+      const float tail = 0.5f * s * t * ex;  // Phi(-|z|)
+      const float phi = z > 0.f ? 1.f - tail : tail;
+      if (SLOPE) slope = fmaf(z * 0.3989422804014327f, ex, phi);
       return z * phi;
     }
     case ACT_GELU_TANH: {  // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
-      const float z2 = z * z;
-      const float p = 1.f / (1.f + __expf(-1.5957691216057308f * z * (1.f + 0.044715f * z2)));
-      if (SLOPE) slope = p + z * p * (1.f - p) * 1.5957691216057308f * (1.f + 0.134145f * z2);
+      const float z2 = fminf(z * z, 1e30f);  // its product with a vanished 1 - p stays 0
+      const float p = rcp_fast(1.f + exp_fast(-1.5957691216057308f * z * fmaf(0.044715f, z2, 1.f)));
+      if (SLOPE) slope = fmaf(z * p * (1.f - p) * 1.5957691216057308f, fmaf(0.134145f, z2, 1.f), p);
       return z * p;
     }
     case ACT_SILU: {
-      const float p = 1.f / (1.f + __expf(-z));
-      if (SLOPE) slope = p * (1.f + z * (1.f - p));
+      const float p = rcp_fast(1.f + exp_fast(-z));
+      if (SLOPE) slope = p * fmaf(z, 1.f - p, 1.f);
       return z * p;
     }
     default:
       if (SLOPE) slope = 1.f;
       return z;
+  }
+}
+template <int ACT, bool SLOPE, int N>
+__device__ __forceinline__ void activate_as(float (&v)[N], float (&sl)[N]) {
+#pragma unroll
+  for (int c = 0; c < N; ++c) v[c] = activate<SLOPE>(ACT, v[c], sl[c]);
+}
+// activate() on N values, with the choice made once.
+template <bool SLOPE, int N>
+__device__ __forceinline__ void activate_all(int act, float (&v)[N], float (&sl)[N]) {
+  switch (act) {
+    case ACT_RELU: activate_as<ACT_RELU, SLOPE>(v, sl); break;
+    case ACT_GELU: activate_as<ACT_GELU, SLOPE>(v, sl); break;
+    case ACT_GELU_TANH: activate_as<ACT_GELU_TANH, SLOPE>(v, sl); break;
+    case ACT_SILU: activate_as<ACT_SILU, SLOPE>(v, sl); break;
+    default: activate_as<ACT_NONE, SLOPE>(v, sl);
   }
 }
 
@@ -148,66 +191,39 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t saddr, uint32_t rank) {
   return v;
 }
 
-// ---- epilogue of 4 adjacent outputs (i, j .. j+3) ----
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {  // 16-bit types, 8 bytes
-  uint2 a = *reinterpret_cast<const uint2*>(p);
-  const T* e = reinterpret_cast<const T*>(&a);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = to_f32(e[i]);
-}
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
-  uint2 a;
-  T* e = reinterpret_cast<T*>(&a);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(v[i]);
-  *reinterpret_cast<uint2*>(p) = a;
+// A role whose wait ran out: raises the flag and gives the loads and MMAs in flight, whose
+// barriers may be another thread's or another CTA's to poll, about 10 ms to end.
+__device__ __forceinline__ void give_up() {
+  atomicExch(&g_timeout, 1);
+  for (int i = 0; i < 1000; ++i) __nanosleep(10000);
 }
 
-template <typename Out, bool SLOPE>
-__device__ __forceinline__ void finish4(const Args& a, int i, int j, const float (&acc)[4]) {
-  const Epilogue& e = a.e;
-  const int left = a.n - j;
-  const bool vec = a.vec && left >= 4;
-  const float rs = e.row_scale ? e.row_scale[i] : 1.f;
-  float b[4] = {}, r[4] = {}, v[4];
-  int16_t sl[4];
-  const Out* bias = static_cast<const Out*>(e.bias);
-  const Out* res = static_cast<const Out*>(e.res) + (e.res ? (int64_t)i * e.ldr : 0);
-  if (vec) {
-    if (bias) load4(bias + j, b);
-    if (e.res) load4(res + j, r);
+// 4 adjacent elements of row i from column j, zero past the edge, as they are stored.
+template <typename T>
+__device__ __forceinline__ uint2 fetch4(const T* p, bool vec, int left) {
+  if (vec && left >= 4) return *reinterpret_cast<const uint2*>(p);
+  uint2 a = make_uint2(0, 0);
+  T* e = reinterpret_cast<T*>(&a);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (c < left) e[c] = p[c];
+  return a;
+}
+template <typename T>
+__device__ __forceinline__ void widen4(uint2 a, float (&v)[4]) {
+  const T* e = reinterpret_cast<const T*>(&a);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) v[c] = to_f32(e[c]);
+}
+// 4 adjacent elements of a row from column j, what lies past the edge left out.
+__device__ __forceinline__ void put4(void* p, uint2 packed, bool vec, int left) {
+  if (vec && left >= 4) {
+    *reinterpret_cast<uint2*>(p) = packed;
   } else {
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(&packed);
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (c < left) {
-        if (bias) b[c] = to_f32(bias[j + c]);
-        if (e.res) r[c] = to_f32(res[j + c]);
-      }
-  }
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    float z = acc[c];
-    if (e.col_scale) z *= rs * (c < left ? e.col_scale[j + c] : 0.f);
-    else if (e.row_scale) z *= rs;
-    z += b[c];
-    float slope;
-    v[c] = activate<SLOPE>(e.act, z, slope) + r[c];
-    if (SLOPE) sl[c] = slope_to_fixed(slope);
-  }
-  Out* out = static_cast<Out*>(e.out) + (int64_t)i * e.ldo + j;
-  int16_t* so = SLOPE ? e.slope + (int64_t)i * a.n + j : nullptr;
-  if (vec) {
-    store4(out, v);
-    if (SLOPE) *reinterpret_cast<short4*>(so) = make_short4(sl[0], sl[1], sl[2], sl[3]);
-  } else {
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c < left) {
-        out[c] = from_f32<Out>(v[c]);
-        if (SLOPE) so[c] = sl[c];
-      }
+      if (c < left) static_cast<uint16_t*>(p)[c] = e[c];
   }
 }
 
@@ -215,8 +231,12 @@ __device__ __forceinline__ void finish4(const Args& a, int i, int j, const float
 // Q's rows are the MMA's 128 rows, P's the T columns, so few tokens cost a narrow MMA and not a
 // padded one; the CTAs of a cluster take equal parts of k, leave their float32 sums in shared
 // memory, and each finishes T / splits of the tile's rows with its peers' sums read over the
-// cluster, added in rank order.
-constexpr int kTileThreads = 256;
+// cluster, added in rank order.  Roles: warps 0-7 epilogue, warp 8 loads, warp 9 MMAs.  The loads
+// start before anything else is set up, and the epilogue warps fetch bias and scales (and the
+// residual, as far as the L2 cache) while the sums are made: these calls are short, and each wait
+// for memory would show.  So would the time to fetch instructions that run once: rows are finished
+// four at a time in a loop that is not unrolled (16 rows unrolled: 16 us for 4096 x 512 x 512, now 1).
+constexpr int kTileThreads = 320;
 constexpr int kTileQ = 128;
 
 template <int T>
@@ -232,14 +252,13 @@ struct TileCfg {
 };
 
 template <typename Out, int ES, int T, bool SLOPE>
-__global__ void __launch_bounds__(kTileThreads)
+__global__ void __launch_bounds__(kTileThreads, T == 256 ? 1 : 2)
     tile_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a) {
   using C = TileCfg<T>;
   extern __shared__ char smraw[];
   char* sm = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[C::STAGES], empty[C::STAGES], done;
   __shared__ uint32_t tslot;
-  __shared__ int s_issued, s_committed, s_drained;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int S = a.splits, rank = blockIdx.x % S;
   const int tile = blockIdx.x / S, tiles_j = (a.n + kTileQ - 1) / kTileQ;
@@ -247,90 +266,104 @@ __global__ void __launch_bounds__(kTileThreads)
   constexpr int BKE = 128 / ES;
   const int nkb = (a.k + BKE - 1) / BKE;
   const int kb = (int)((int64_t)nkb * rank / S), nk = (int)((int64_t)nkb * (rank + 1) / S) - kb;
+  const Epilogue& e = a.e;
 
-  if (warp == 0) {
-    tc::tmem_alloc(&tslot, C::TMEM);
-    tc::tmem_relinquish();
-  }
-  if (tid == 0) {
-    s_issued = s_committed = 0;
-    s_drained = 1;
+  auto load = [&](int t) {  // block t of this CTA's k into its ring slot
+    const int s = t % C::STAGES, k0 = (kb + t) * BKE;
+    const uint32_t pq = tc::smem_u32(sm + s * C::STAGE), pp = pq + C::Q_BYTES;
+    mbar_expect_tx(&full[s], C::STAGE);
+    if (ES == 2 && a.q_row) {
+#pragma unroll
+      for (int c = 0; c < kTileQ / 64; ++c) tma_load_2d(pq + 8192 * c, &maps.q, j0 + 64 * c, k0, &full[s]);
+    } else {
+      tma_load_2d(pq, &maps.q, k0, j0, &full[s]);
+    }
+    if (ES == 2 && T >= 64 && a.p_row) {
+#pragma unroll
+      for (int c = 0; c < T / 64; ++c) tma_load_2d(pp + 8192 * c, &maps.p, i0 + 64 * c, k0, &full[s]);
+    } else {
+      tma_load_2d(pp, &maps.p, k0, i0, &full[s]);
+    }
+  };
+  if (warp == 8 && lane == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
       tc::mbar_init(&full[s], 1);
       tc::mbar_init(&empty[s], 1);
     }
     tc::mbar_init(&done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tc::fence_async_smem();
+    for (int t = 0; t < nk && t < C::STAGES; ++t) load(t);
+  } else if (warp == 9) {
+    tc::tmem_alloc(&tslot, C::TMEM);
+    tc::tmem_relinquish();
   }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tslot;
-  bool ok = true;
 
-  if (warp == 0 && lane == 0) {
-    for (int t = 0; t < nk; ++t) {
-      const int s = t % C::STAGES, k0 = (kb + t) * BKE;
-      if (t >= C::STAGES && !tc::mbar_wait(&empty[s], ((t / C::STAGES) - 1) & 1)) { ok = false; break; }
-      const uint32_t pq = tc::smem_u32(sm + s * C::STAGE), pp = pq + C::Q_BYTES;
-      mbar_expect_tx(&full[s], C::STAGE);
-      if (ES == 2 && a.q_row) {
-#pragma unroll
-        for (int c = 0; c < kTileQ / 64; ++c) tma_load_2d(pq + 8192 * c, &maps.q, j0 + 64 * c, k0, &full[s]);
-      } else {
-        tma_load_2d(pq, &maps.q, k0, j0, &full[s]);
+  // the tile's rows that this CTA finishes, one per warp at a time
+  const int per = T / S, j = j0 + 4 * lane, left = a.n - j;
+  float* acc = reinterpret_cast<float*>(sm);  // [T][128]; the ring is free when the sums are there
+  float bias[4] = {}, cscale[4] = {1.f, 1.f, 1.f, 1.f};
+  if (warp == 8) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int t = C::STAGES; t < nk && ok; ++t) {
+        ok = tc::mbar_wait(&empty[t % C::STAGES], ((t / C::STAGES) - 1) & 1);
+        if (ok) load(t);
       }
-      if (ES == 2 && T >= 64 && a.p_row) {
+      if (!ok) give_up();
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      const uint32_t qstep = (a.q_row ? 2048 : 32) >> 4, pstep = (a.p_row ? 2048 : 32) >> 4;
+      bool ok = true;
+      for (int t = 0; t < nk; ++t) {
+        const int s = t % C::STAGES;
+        ok = tc::mbar_wait(&full[s], (t / C::STAGES) & 1);
+        if (!ok) break;
+        tc::tc_fence_after();
+        const uint32_t pq = tc::smem_u32(sm + s * C::STAGE), pp = pq + C::Q_BYTES;
+        uint64_t dq = operand_desc(pq, a.q_row), dp = operand_desc(pp, a.p_row);
 #pragma unroll
-        for (int c = 0; c < T / 64; ++c) tma_load_2d(pp + 8192 * c, &maps.p, i0 + 64 * c, k0, &full[s]);
-      } else {
-        tma_load_2d(pp, &maps.p, k0, i0, &full[s]);
+        for (int c = 0; c < 4; ++c, dq += qstep, dp += pstep)
+          mma<ES>(tmem, dq, dp, a.idesc, (t | c) ? 1u : 0u);
+        tc::mma_commit(&empty[s]);
       }
-      s_issued = t + 1;
+      if (ok && nk > 0) tc::mma_commit(&done);
+      if (!ok) give_up();
     }
-  } else if (warp == 1 && lane == 0) {
-    const uint32_t qstep = (a.q_row ? 2048 : 32) >> 4, pstep = (a.p_row ? 2048 : 32) >> 4;
-    for (int t = 0; t < nk; ++t) {
-      const int s = t % C::STAGES;
-      if (!tc::mbar_wait(&full[s], (t / C::STAGES) & 1)) { ok = false; break; }
-      tc::tc_fence_after();
-      const uint32_t pq = tc::smem_u32(sm + s * C::STAGE), pp = pq + C::Q_BYTES;
-      uint64_t dq = operand_desc(pq, a.q_row), dp = operand_desc(pp, a.p_row);
+  } else {
+    if (left > 0) {
+      if (e.bias) widen4<Out>(fetch4(static_cast<const Out*>(e.bias) + j, a.vec, left), bias);
+      if (ES == 1 && e.col_scale) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c, dq += qstep, dp += pstep)
-        mma<ES>(tmem, dq, dp, a.idesc, (t | c) ? 1u : 0u);
-      tc::mma_commit(&empty[s]);
-      s_committed = t + 1;
+        for (int c = 0; c < 4; ++c)
+          if (c < left) cscale[c] = e.col_scale[j + c];
+      }
     }
-    if (nk > 0 && ok) {
-      tc::mma_commit(&done);
-      if (!tc::mbar_wait(&done, 0)) ok = false;
+    if (e.res) {  // 256 bytes a row: a lane for each half of the CTA's rows
+      for (int x = 32 * warp + lane; x < 2 * per; x += 256) {
+        const int i = i0 + rank * per + (x >> 1), c = j0 + 64 * (x & 1);
+        if (i < a.m && c < a.n)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const Out*>(e.res) + (int64_t)i * e.ldr + c));
+      }
     }
-  }
-  const bool failed = __syncthreads_or(!ok);
-  if (failed && tid == 0) {
-    // what is in flight ends (each wait again bounded) before the buffers and the TMEM are reused:
-    // commit t completes phase t / STAGES of empty[t % STAGES], load t that of full[t % STAGES]
-    const int nc = s_committed, ni = s_issued;
-    if (nc > 0 && !tc::mbar_wait(&empty[(nc - 1) % C::STAGES], ((nc - 1) / C::STAGES) & 1)) s_drained = 0;
-    for (int u = ni > C::STAGES ? ni - C::STAGES : 0; u < ni; ++u)
-      if (!tc::mbar_wait(&full[u % C::STAGES], (u / C::STAGES) & 1)) s_drained = 0;
-    atomicExch(&g_timeout, 1);
-  }
-  if (failed) __syncthreads();
-  tc::tc_fence_after();
-
-  // float32 sums to shared memory as acc[i][j]: a warp's 32 lanes are 32 adjacent j
-  float* acc = reinterpret_cast<float*>(sm);
-  {
+    bool ok = nk == 0 || tc::mbar_wait(&done, 0);
+    if (!ok) atomicExch(&g_timeout, 1);
+    ok = __all_sync(0xffffffffu, ok);
+    tc::tc_fence_after();
+    // float32 sums to shared memory as acc[i][j]: a warp's 32 lanes are 32 adjacent j
     const int lq = warp & 3;
-    constexpr int HALF = T < 64 ? T : T / 2;  // columns of a warp: all of them, or its half
-    if (T >= 64 || warp < 4) {
+    constexpr int HALF = T < 32 ? T : T / 2;  // columns of a warp: its half, or all 16 of them
+    if (T >= 32 || warp < 4) {
 #pragma unroll
       for (int c = 0; c < HALF; c += 16) {
-        const int col = (T >= 64 ? (warp >> 2) * HALF : 0) + c;
+        const int col = (T >= 32 ? (warp >> 2) * HALF : 0) + c;
         uint32_t r[16];
-        if (nk > 0 && !failed) {
+        if (nk > 0 && ok) {
           asm volatile(
               "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -341,40 +374,234 @@ __global__ void __launch_bounds__(kTileThreads)
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         } else {
 #pragma unroll
-          for (int x = 0; x < 16; ++x) r[x] = 0;
+          for (int x = 0; x < 16; ++x) r[x] = ok ? 0u : 0x7FFFFFFFu;
         }
 #pragma unroll
         for (int x = 0; x < 16; ++x)
-          acc[(col + x) * kTileQ + 32 * lq + lane] =
-              failed ? __int_as_float(0x7FFFFFFF) : __uint_as_float(r[x]);
+          if (i0 + col + x < a.m) acc[(col + x) * kTileQ + 32 * lq + lane] = __uint_as_float(r[x]);
       }
     }
   }
   tc::tc_fence_before();
+  __syncwarp();
   if (S > 1) {
     cluster_arrive();
     cluster_wait();
   } else {
     __syncthreads();
   }
-  if (warp == 0 && s_drained) tc::tmem_dealloc(tmem, C::TMEM);
-  const int per = T / S;
-  for (int x = warp; x < per; x += kTileThreads / 32) {
-    const int il = rank * per + x, i = i0 + il, j = j0 + 4 * lane;
-    if (i >= a.m) break;
-    const uint32_t at = tc::smem_u32(acc + il * kTileQ + 4 * lane);
-    float v[4] = {};
-    for (int s = 0; s < S; ++s) {
-      const float4 u = S > 1 ? ld_cluster(at, s) : *reinterpret_cast<const float4*>(acc + il * kTileQ + 4 * lane);
-      v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w;
+  if (warp == 9) tc::tmem_dealloc(tmem, C::TMEM);
+  if (warp < 8 && left > 0) {
+#pragma unroll 1
+    for (int x0 = warp; x0 < per; x0 += 32) {  // rows x0, x0 + 8, x0 + 16, x0 + 24 of this CTA's
+      uint2 res[4];
+      float v[16], sl[16];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int x = x0 + 8 * y, il = rank * per + x, i = i0 + il;
+        const bool mine = x < per && i < a.m;
+        res[y] = make_uint2(0, 0);
+        float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+        float rs = 1.f;
+        if (mine) {
+          if (e.res) res[y] = fetch4(static_cast<const Out*>(e.res) + (int64_t)i * e.ldr + j, a.vec, left);
+          if (ES == 1 && e.row_scale) rs = e.row_scale[i];
+          const float* at = acc + il * kTileQ + 4 * lane;
+          if (S > 1) {
+            for (int s = 0; s < S; ++s) {
+              const float4 p = ld_cluster(tc::smem_u32(at), s);
+              u.x += p.x; u.y += p.y; u.z += p.z; u.w += p.w;
+            }
+          } else {
+            u = *reinterpret_cast<const float4*>(at);
+          }
+        }
+        const float z[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[4 * y + c] = (ES == 1 ? z[c] * (rs * cscale[c]) : z[c]) + bias[c];
+      }
+      activate_all<SLOPE>(e.act, v, sl);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int x = x0 + 8 * y, i = i0 + rank * per + x;
+        if (x >= per || i >= a.m) continue;
+        float r[4];
+        widen4<Out>(res[y], r);
+        uint2 packed, slopes;
+        Out* o = reinterpret_cast<Out*>(&packed);
+        int16_t* f = reinterpret_cast<int16_t*>(&slopes);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          o[c] = from_f32<Out>(v[4 * y + c] + r[c]);
+          if (SLOPE) f[c] = slope_to_fixed(sl[4 * y + c]);
+        }
+        put4(static_cast<Out*>(e.out) + (int64_t)i * e.ldo + j, packed, a.vec, left);
+        if (SLOPE) put4(e.slope + (int64_t)i * a.n + j, slopes, a.vec, left);
+      }
     }
-    if (j < a.n) finish4<Out, SLOPE>(a, i, j, v);
   }
   __syncwarp();
   if (S > 1) {  // the peers read this CTA's sums until here
     cluster_arrive();
     cluster_wait();
   }
+}
+
+// ---- a few tokens: a warp per R features, W read once, straight into registers ----
+// Bound by W's bytes, and for small W by what a call costs at all: no tensor maps, no shared
+// memory, no set-up.  A warp reads 512 bytes of each of its R rows of W at a time (32 lanes x 16
+// bytes; single elements where rows start off 16 bytes), the same part of the M tokens from the L1
+// cache, and adds the products in float32; SPLIT warps share a feature's k where there are too few
+// features to fill the GPU.  One lane per (token, feature) finishes it.
+template <typename T> struct Chunk;  // 16 bytes of an operand as float
+template <> struct Chunk<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void widen(const uint4& a, float (&v)[8]) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+};
+template <> struct Chunk<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void widen(const uint4& a, float (&v)[8]) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+};
+template <> struct Chunk<__nv_fp8_e4m3> {
+  static constexpr int N = 16;
+  static __device__ __forceinline__ void widen(const uint4& a, float (&v)[16]) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i] >> (16 * h)), __NV_E4M3);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+        v[4 * i + 2 * h] = f.x;
+        v[4 * i + 2 * h + 1] = f.y;
+      }
+  }
+};
+__device__ __forceinline__ float widen1(__nv_bfloat16 x) { return to_f32(x); }
+__device__ __forceinline__ float widen1(__half x) { return to_f32(x); }
+__device__ __forceinline__ float widen1(__nv_fp8_e4m3 x) { return float(x); }
+
+struct TokenArgs {
+  const void* x; int64_t ldx;
+  const void* w; int64_t ldw;
+  int m, n, k;
+  Epilogue e;
+};
+
+template <typename Out, typename In, int M, int R, int SPLIT, bool VEC>
+__global__ void __launch_bounds__(256) token_kernel(TokenArgs a) {
+  __shared__ float s_part[SPLIT == 1 ? 1 : 8][M * R];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = SPLIT == 1 ? 0 : warp;
+  const int j0 = (SPLIT == 1 ? blockIdx.x * 8 + warp : blockIdx.x) * R;
+  if (j0 >= a.n) return;  // SPLIT == 1 only: no barrier follows there
+  const Epilogue& e = a.e;
+  // this lane's output, if it has one: token i, feature j
+  const int i = lane / R, j = j0 + lane % R;
+  const bool mine = lane < M * R && i < a.m && j < a.n && part == 0;
+  float bias = 0.f, res = 0.f, scale = 1.f;
+  if (mine) {
+    if (e.bias) bias = to_f32(static_cast<const Out*>(e.bias)[j]);
+    if (e.res) res = to_f32(static_cast<const Out*>(e.res)[(int64_t)i * e.ldr + j]);
+    if (e.row_scale) scale = e.row_scale[i];
+    if (e.col_scale) scale *= e.col_scale[j];
+  }
+  const In* w[R];
+  const In* x[M];
+#pragma unroll
+  for (int r = 0; r < R; ++r) w[r] = static_cast<const In*>(a.w) + (int64_t)min(j0 + r, a.n - 1) * a.ldw;
+#pragma unroll
+  for (int t = 0; t < M; ++t) x[t] = static_cast<const In*>(a.x) + (int64_t)min(t, a.m - 1) * a.ldx;
+  float acc[M][R] = {};
+  constexpr int N = VEC ? Chunk<In>::N : 1;
+  constexpr int STEP = 32 * N * SPLIT;
+  constexpr int U = VEC ? (R * M >= 8 ? 2 : 4) : 8;  // steps in flight
+  for (int k0 = 32 * N * part + N * lane; k0 < a.k; k0 += STEP * U) {
+    if constexpr (VEC) {
+      uint4 wv[U][R];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int k = k0 + u * STEP;
+          wv[u][r] = k < a.k ? __ldcs(reinterpret_cast<const uint4*>(w[r] + k)) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * STEP;
+        if (k >= a.k) break;
+        float wf[R][N];
+#pragma unroll
+        for (int r = 0; r < R; ++r) Chunk<In>::widen(wv[u][r], wf[r]);
+#pragma unroll
+        for (int t = 0; t < M; ++t) {
+          float xf[N];
+          Chunk<In>::widen(*reinterpret_cast<const uint4*>(x[t] + k), xf);
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int c = 0; c < N; ++c) acc[t][r] = fmaf(xf[c], wf[r][c], acc[t][r]);
+        }
+      }
+    } else {
+      float wf[U][R];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int k = k0 + u * STEP;
+          wf[u][r] = k < a.k ? widen1(w[r][k]) : 0.f;
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * STEP;
+        if (k >= a.k) break;
+#pragma unroll
+        for (int t = 0; t < M; ++t) {
+          const float xf = widen1(x[t][k]);
+#pragma unroll
+          for (int r = 0; r < R; ++r) acc[t][r] = fmaf(xf, wf[u][r], acc[t][r]);
+        }
+      }
+    }
+  }
+  float sum = 0.f;  // of this lane's output
+#pragma unroll
+  for (int t = 0; t < M; ++t)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float v = acc[t][r];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == t * R + r) sum = v;
+    }
+  if (SPLIT > 1) {
+    if (lane < M * R) s_part[warp][lane] = sum;
+    __syncthreads();
+    if (!mine) return;
+    sum = 0.f;
+#pragma unroll
+    for (int p = 0; p < SPLIT; ++p) sum += s_part[p][lane];
+  }
+  if (!mine) return;
+  float slope;
+  const float v = activate<false>(e.act, sum * scale + bias, slope) + res;
+  static_cast<Out*>(e.out)[(int64_t)i * e.ldo + j] = from_f32<Out>(v);
 }
 
 // ---- dz = dy act'(z), and the column sums of dz (the bias' gradient) ----

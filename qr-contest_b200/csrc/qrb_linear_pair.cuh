@@ -120,30 +120,6 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t phase) {
   return false;
 }
 
-// A role whose wait ran out: raises the flag and gives the loads and MMAs in flight, whose
-// barriers may be the other CTA's, about 10 ms to end.
-__device__ __forceinline__ void give_up() {
-  atomicExch(&g_timeout, 1);
-  for (int i = 0; i < 1000; ++i) __nanosleep(10000);
-}
-
-template <int ACT, bool SLOPE>
-__device__ __forceinline__ void activate32_as(float (&v)[32], float (&sl)[32]) {
-#pragma unroll
-  for (int c = 0; c < 32; ++c) v[c] = activate<SLOPE>(ACT, v[c], sl[c]);
-}
-// activate() on 32 values, with the choice made once.
-template <bool SLOPE>
-__device__ __forceinline__ void activate32(int act, float (&v)[32], float (&sl)[32]) {
-  switch (act) {
-    case ACT_RELU: activate32_as<ACT_RELU, SLOPE>(v, sl); break;
-    case ACT_GELU: activate32_as<ACT_GELU, SLOPE>(v, sl); break;
-    case ACT_GELU_TANH: activate32_as<ACT_GELU_TANH, SLOPE>(v, sl); break;
-    case ACT_SILU: activate32_as<ACT_SILU, SLOPE>(v, sl); break;
-    default: activate32_as<ACT_NONE, SLOPE>(v, sl);
-  }
-}
-
 // Address of 16-byte chunk q of row r in a staged block of 32 rows x 128 bytes.
 __device__ __forceinline__ char* staged(char* buf, int r, int q) { return buf + 128 * r + 16 * (q ^ (r & 7)); }
 
@@ -357,7 +333,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
             v[x] += bb.x; v[x + 1] += bb.y; v[x + 2] += bb.z; v[x + 3] += bb.w;
           }
-          activate32<SLOPE>(e.act, v, sl);
+          activate_all<SLOPE>(e.act, v, sl);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint4* at = reinterpret_cast<uint4*>(staged(buf, lane, 4 * h + q));

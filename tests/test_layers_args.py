@@ -123,7 +123,7 @@ def test_linear_abi_checks():
                dict(ldx=7), dict(ldw=7), dict(ldy=3), dict(tr=1, ldw=3), dict(r=16, ldr=-1)):
         assert _linear(**kw) == bad, kw
     # odd rows need an aligned copy, and the caller's workspace has to hold it
-    assert _linear(ldx=9, ws=16, wsb=16) == _lib.QRB200_ERR_WORKSPACE
+    assert _linear(m=40, ldx=9, ws=16, wsb=16) == _lib.QRB200_ERR_WORKSPACE
     assert _linear(m=0, x=None, w=None, y=None) == _lib.QRB200_OK
     assert _linear(n=0, ldy=0, x=None, w=None, y=None) == _lib.QRB200_OK
     L, n = _lib.lib(), ctypes.c_size_t()
