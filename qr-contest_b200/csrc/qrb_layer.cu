@@ -242,15 +242,14 @@ bool encode_operand(CUtensorMap* map, const Operand& o, int64_t rows, int64_t k,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename Out, int ES, int T, bool SLOPE>
-int launch_tile(const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
-  auto kernel = lin::tile_kernel<Out, ES, T, SLOPE>;
-  using C = lin::TileCfg<T>;
+template <typename Out, int ES, int T, bool SLOPE, int RINGS>
+int launch_tile_as(const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
+  auto kernel = lin::tile_kernel<Out, ES, T, SLOPE, RINGS>;
+  using C = lin::TileCfg<T, RINGS>;
   static std::atomic<uint64_t> ready{0};
   if (const int rc = raise_smem(reinterpret_cast<const void*>(kernel), C::SMEM, ready)) return rc;
-  const int64_t tiles = (int64_t)((a.n + 127) / 128) * ((a.m + T - 1) / T);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(tiles * a.splits));
+  cfg.gridDim = dim3((unsigned)a.splits, (unsigned)((a.n + 127) / 128), (unsigned)((a.m + T - 1) / T));
   cfg.blockDim = dim3(lin::kTileThreads);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = st;
@@ -267,6 +266,12 @@ int launch_tile(const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
     return QRB200_ERR_CUDA;
   }
   return QRB200_OK;
+}
+template <typename Out, int ES, int T, bool SLOPE>
+int launch_tile(const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
+  const int64_t ctas = (int64_t)a.splits * ((a.n + 127) / 128) * ((a.m + T - 1) / T);
+  if (T == 256 || ctas <= kSMs) return launch_tile_as<Out, ES, T, SLOPE, 1>(maps, a, st);
+  return launch_tile_as<Out, ES, T, SLOPE, T == 256 ? 1 : 2>(maps, a, st);
 }
 
 template <typename Out, int ES, bool SLOPE>
@@ -339,14 +344,18 @@ int product_pair(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64
             : launch_pair<__half, 2, TN, false>(P, Q, m, n, k, dtype, e, st);
 }
 
-// A few tokens, W's features in rows: token_kernel.  SPLIT as there are too few features for the GPU
-// (8 warps an SM at one feature a warp).
-constexpr int64_t kTokens = 4;
+// A few tokens, W's features in rows: token_kernel.  Up to 2 tokens always; 3 and 4, which make it
+// bound by its instructions, where W is small enough for the call's own cost to matter (4 tokens,
+// 4096 x 4096: 11.8 us against 10.6 with tiles; 1 token 8.8 against 10.5; 512 x 512: 2.4 against 4.4).
+// Features: two a warp from 8192 on (8192 x 8192: 24.0 us against 28.9 with one), one below that
+// (4096 x 4096: 8.8 against 9.3), and one a block, its k shared by 8 warps, where k is long for the
+// number of features (512 x 16384: 5.5 us against 21.9; 4096 x 16384: 23.8 against 25.9).
+bool few_tokens(int64_t m, int64_t n, int64_t k) { return m <= 2 || (m <= 4 && n * k <= 1 << 22); }
 template <typename Out, typename In, int M, bool VEC>
 int launch_token(const lin::TokenArgs& a, cudaStream_t st) {
-  if (a.n >= 2 * 8 * kSMs) lin::token_kernel<Out, In, M, 2, 1, VEC><<<(a.n + 15) / 16, 256, 0, st>>>(a);
-  else if (a.n >= 8 * kSMs || a.k <= 2048) lin::token_kernel<Out, In, M, 1, 1, VEC><<<(a.n + 7) / 8, 256, 0, st>>>(a);
-  else lin::token_kernel<Out, In, M, 1, 8, VEC><<<a.n, 256, 0, st>>>(a);
+  if (a.n >= 8192) lin::token_kernel<Out, In, M, 2, 1, VEC><<<(a.n + 7) / 8, 128, 0, st>>>(a);
+  else if ((int64_t)a.k * sizeof(In) >= 4 * (int64_t)a.n) lin::token_kernel<Out, In, M, 1, 8, VEC><<<a.n, 256, 0, st>>>(a);
+  else lin::token_kernel<Out, In, M, 1, 1, VEC><<<(a.n + 3) / 4, 128, 0, st>>>(a);
   return launched();
 }
 template <typename Out, typename In>
@@ -385,6 +394,7 @@ int product(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_t k,
   const int nkb = (int)((k * a.es + 127) / 128);
   a.splits = 1;
   while (a.splits < 8 && tiles * a.splits * 2 <= room && nkb / (a.splits * 2) >= 4) a.splits *= 2;
+  a.part = (nkb + a.splits - 1) / a.splits;
   a.idesc = lin::idesc(dtype == QRB200_BF16 ? 1 : 0, a.q_row, a.p_row, lin::kTileQ, T);
   lin::Maps maps{};
   if (k > 0 && !(encode_operand(&maps.p, P, m, k, dtype, T) && encode_operand(&maps.q, Q, n, k, dtype, lin::kTileQ))) {
@@ -399,10 +409,11 @@ int product(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_t k,
   return bf ? launch_tile_t<__nv_bfloat16, 2, false>(T, maps, a, st) : launch_tile_t<__half, 2, false>(T, maps, a, st);
 }
 
+constexpr int64_t kMostRows = 128 * 65535;  // of x, and of the weight
 bool sizes_ok(int64_t m, int64_t n, int64_t k) {
   constexpr int64_t top = (int64_t)1 << 31;
-  return m >= 0 && n >= 0 && k >= 0 && m < top - 256 && n < top - 256 && k < top - 256 &&
-         ((n + 127) / 128) * ((m + 15) / 16) * 8 < top;
+  // a grid's y and z have 16 bits, and an index into one operand's rows 31
+  return m >= 0 && n >= 0 && k >= 0 && m <= kMostRows && n <= kMostRows && k < top - 256;
 }
 
 // Blocks of dz_kernel along m, each of which leaves one part of the bias' sum: 8 blocks an SM.
@@ -566,7 +577,7 @@ int qrb200_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_
   const int es = esize(dtype);
   Operand X{x, ldx, false}, W{w, ldw, w_transposed != 0};
   lin::Epilogue e{x_scale, w_scale, bias, residual, ldr, y, ldy, slope, activation};
-  if (m <= kTokens && !w_transposed && !slope && k > 0) {
+  if (few_tokens(m, n, k) && !w_transposed && !slope && k > 0) {
     const lin::TokenArgs t{x, ldx, w, ldw, (int)m, (int)n, (int)k, e};
     if (q8) return out_dtype == QRB200_BF16 ? product_token<__nv_bfloat16, __nv_fp8_e4m3>(t, st) : product_token<__half, __nv_fp8_e4m3>(t, st);
     return dtype == QRB200_BF16 ? product_token<__nv_bfloat16, __nv_bfloat16>(t, st) : product_token<__half, __half>(t, st);

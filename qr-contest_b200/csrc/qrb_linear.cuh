@@ -43,6 +43,7 @@ struct Epilogue {
 struct Args {
   int m, n, k;             // D is m x n
   int splits;              // CTAs of a cluster that share a tile's sum
+  int part;                // 128-byte blocks of k of each of them (the last may have fewer)
   uint32_t idesc;          // element types and operand majors
   int es;                  // bytes of an operand element
   int p_row, q_row;        // operand is row-major (contiguous along its rows)
@@ -174,6 +175,20 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
+// 16 consecutive float32 columns of this thread's tensor-memory lane.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(r[x]);
+}
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
@@ -234,16 +249,16 @@ __device__ __forceinline__ void put4(void* p, uint2 packed, bool vec, int left) 
 // cluster, added in rank order.  Roles: warps 0-7 epilogue, warp 8 loads, warp 9 MMAs.  The loads
 // start before anything else is set up, and the epilogue warps fetch bias and scales (and the
 // residual, as far as the L2 cache) while the sums are made: these calls are short, and each wait
-// for memory would show.  So would the time to fetch instructions that run once: rows are finished
-// four at a time in a loop that is not unrolled (16 rows unrolled: 16 us for 4096 x 512 x 512, now 1).
+// for memory would show.  So would the time to fetch instructions that run once (with 16 rows
+// unrolled, finishing a tile took 16 us): loops stay loops, and there are no divisions.
 constexpr int kTileThreads = 320;
 constexpr int kTileQ = 128;
 
-template <int T>
+// RINGS = 2: half an SM's shared memory, two CTAs an SM; 1: all of it, for grids of one CTA an SM.
+template <int T, int RINGS>
 struct TileCfg {
   static constexpr int P_BYTES = T * 128, Q_BYTES = kTileQ * 128, STAGE = P_BYTES + Q_BYTES;
-  // 2 CTAs per SM up to T = 128; one with four 48 KB stages for T = 256
-  static constexpr int STAGES = T == 256 ? 4 : (T == 128 ? 3 : (T == 64 ? 4 : 5));
+  static constexpr int STAGES = (T >= 128 ? 192 : 180) * 1024 / RINGS / STAGE;
   static constexpr int ACC_BYTES = T * kTileQ * 4;
   static constexpr int RING = STAGES * STAGE;
   static constexpr int DATA = RING > ACC_BYTES ? RING : ACC_BYTES;
@@ -251,21 +266,19 @@ struct TileCfg {
   static constexpr int TMEM = T < 32 ? 32 : T;
 };
 
-template <typename Out, int ES, int T, bool SLOPE>
-__global__ void __launch_bounds__(kTileThreads, T == 256 ? 1 : 2)
+template <typename Out, int ES, int T, bool SLOPE, int RINGS>
+__global__ void __launch_bounds__(kTileThreads, RINGS)
     tile_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a) {
-  using C = TileCfg<T>;
+  using C = TileCfg<T, RINGS>;
   extern __shared__ char smraw[];
   char* sm = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[C::STAGES], empty[C::STAGES], done;
   __shared__ uint32_t tslot;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int S = a.splits, rank = blockIdx.x % S;
-  const int tile = blockIdx.x / S, tiles_j = (a.n + kTileQ - 1) / kTileQ;
-  const int j0 = tile % tiles_j * kTileQ, i0 = tile / tiles_j * T;
+  const int S = a.splits, rank = blockIdx.x;  // the cluster is the grid's x
+  const int j0 = blockIdx.y * kTileQ, i0 = blockIdx.z * T;
   constexpr int BKE = 128 / ES;
-  const int nkb = (a.k + BKE - 1) / BKE;
-  const int kb = (int)((int64_t)nkb * rank / S), nk = (int)((int64_t)nkb * (rank + 1) / S) - kb;
+  const int kb = rank * a.part, nk = max(0, min(a.part, (a.k + BKE - 1) / BKE - kb));
   const Epilogue& e = a.e;
 
   auto load = [&](int t) {  // block t of this CTA's k into its ring slot
@@ -303,7 +316,7 @@ __global__ void __launch_bounds__(kTileThreads, T == 256 ? 1 : 2)
   tc::tc_fence_after();
   const uint32_t tmem = tslot;
 
-  // the tile's rows that this CTA finishes, one per warp at a time
+  // the tile's rows that this CTA finishes, two per warp at a time
   const int per = T / S, j = j0 + 4 * lane, left = a.n - j;
   float* acc = reinterpret_cast<float*>(sm);  // [T][128]; the ring is free when the sums are there
   float bias[4] = {}, cscale[4] = {1.f, 1.f, 1.f, 1.f};
@@ -362,23 +375,16 @@ __global__ void __launch_bounds__(kTileThreads, T == 256 ? 1 : 2)
 #pragma unroll
       for (int c = 0; c < HALF; c += 16) {
         const int col = (T >= 32 ? (warp >> 2) * HALF : 0) + c;
-        uint32_t r[16];
+        float r[16];
         if (nk > 0 && ok) {
-          asm volatile(
-              "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-              "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-              : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-                "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-                "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-              : "r"(tmem + ((uint32_t)(32 * lq) << 16) + col));
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          tmem_ld16(tmem + ((uint32_t)(32 * lq) << 16) + col, r);
         } else {
 #pragma unroll
-          for (int x = 0; x < 16; ++x) r[x] = ok ? 0u : 0x7FFFFFFFu;
+          for (int x = 0; x < 16; ++x) r[x] = ok ? 0.f : __int_as_float(0x7FFFFFFF);
         }
 #pragma unroll
         for (int x = 0; x < 16; ++x)
-          if (i0 + col + x < a.m) acc[(col + x) * kTileQ + 32 * lq + lane] = __uint_as_float(r[x]);
+          if (i0 + col + x < a.m) acc[(col + x) * kTileQ + 32 * lq + lane] = r[x];
       }
     }
   }
@@ -393,11 +399,11 @@ __global__ void __launch_bounds__(kTileThreads, T == 256 ? 1 : 2)
   if (warp == 9) tc::tmem_dealloc(tmem, C::TMEM);
   if (warp < 8 && left > 0) {
 #pragma unroll 1
-    for (int x0 = warp; x0 < per; x0 += 32) {  // rows x0, x0 + 8, x0 + 16, x0 + 24 of this CTA's
-      uint2 res[4];
-      float v[16], sl[16];
+    for (int x0 = warp; x0 < per; x0 += 16) {  // rows x0 and x0 + 8 of this CTA's
+      uint2 res[2];
+      float v[8], sl[8];
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
+      for (int y = 0; y < 2; ++y) {
         const int x = x0 + 8 * y, il = rank * per + x, i = i0 + il;
         const bool mine = x < per && i < a.m;
         res[y] = make_uint2(0, 0);
@@ -408,9 +414,10 @@ __global__ void __launch_bounds__(kTileThreads, T == 256 ? 1 : 2)
           if (ES == 1 && e.row_scale) rs = e.row_scale[i];
           const float* at = acc + il * kTileQ + 4 * lane;
           if (S > 1) {
-            for (int s = 0; s < S; ++s) {
-              const float4 p = ld_cluster(tc::smem_u32(at), s);
-              u.x += p.x; u.y += p.y; u.z += p.z; u.w += p.w;
+#pragma unroll 1
+            for (int s = 0; s < S; s += 2) {  // 2, 4 or 8 parts; two reads in flight, added in rank order
+              const float4 p = ld_cluster(tc::smem_u32(at), s), q = ld_cluster(tc::smem_u32(at), s + 1);
+              u.x = u.x + p.x + q.x; u.y = u.y + p.y + q.y; u.z = u.z + p.z + q.z; u.w = u.w + p.w + q.w;
             }
           } else {
             u = *reinterpret_cast<const float4*>(at);
@@ -422,7 +429,7 @@ __global__ void __launch_bounds__(kTileThreads, T == 256 ? 1 : 2)
       }
       activate_all<SLOPE>(e.act, v, sl);
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
+      for (int y = 0; y < 2; ++y) {
         const int x = x0 + 8 * y, i = i0 + rank * per + x;
         if (x >= per || i >= a.m) continue;
         float r[4];
@@ -508,7 +515,7 @@ __global__ void __launch_bounds__(256) token_kernel(TokenArgs a) {
   __shared__ float s_part[SPLIT == 1 ? 1 : 8][M * R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = SPLIT == 1 ? 0 : warp;
-  const int j0 = (SPLIT == 1 ? blockIdx.x * 8 + warp : blockIdx.x) * R;
+  const int j0 = (SPLIT == 1 ? blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x) * R;
   if (j0 >= a.n) return;  // SPLIT == 1 only: no barrier follows there
   const Epilogue& e = a.e;
   // this lane's output, if it has one: token i, feature j

@@ -305,38 +305,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           res_phase ^= 1;
         }
         ok = __all_sync(0xffffffffu, ok);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float v[32], sl[32];
+        // 16 columns at a time, in a loop: instructions that are fetched to run once cost more than
+        // the loop does
+#pragma unroll 1
+        for (int h = 0; h < 4; ++h) {
+          float v[16], sl[16];
           if (ok) {
-            tc::tmem_ld32(tmem + b * TN + lane_base + c0 + 32 * h, v);
+            tmem_ld16(tmem + b * TN + lane_base + c0 + 16 * h, v);
           } else {
 #pragma unroll
-            for (int x = 0; x < 32; ++x) v[x] = __int_as_float(0x7FFFFFFF);
+            for (int x = 0; x < 16; ++x) v[x] = __int_as_float(0x7FFFFFFF);
           }
-          if (h == 1 && c0 + 64 == (half + 1) * (TN / 2)) {  // the sums are in registers
+          if (h == 3 && c0 + 64 == (half + 1) * (TN / 2)) {  // the sums are in registers
             tc::tc_fence_before();
             __syncwarp();
             if (lane == 0) arrive_at(b ? done_bar1 : done_bar0);
           }
           if (!live) continue;
-          __syncwarp();
-          s_col[warp][0][lane] = bias[h];
-          if (ES == 1) s_col[warp][1][lane] = cscale[h];
-          __syncwarp();
+          if (!(h & 1)) {
+            __syncwarp();
+            s_col[warp][0][lane] = h ? bias[1] : bias[0];
+            if (ES == 1) s_col[warp][1][lane] = h ? cscale[1] : cscale[0];
+            __syncwarp();
+          }
+          const int hc = 16 * (h & 1);
 #pragma unroll
-          for (int x = 0; x < 32; x += 4) {
-            const float4 bb = *reinterpret_cast<const float4*>(&s_col[warp][0][x]);
+          for (int x = 0; x < 16; x += 4) {
+            const float4 bb = *reinterpret_cast<const float4*>(&s_col[warp][0][hc + x]);
             if (ES == 1) {
-              const float4 cs = *reinterpret_cast<const float4*>(&s_col[warp][1][x]);
+              const float4 cs = *reinterpret_cast<const float4*>(&s_col[warp][1][hc + x]);
               v[x] *= rs * cs.x; v[x + 1] *= rs * cs.y; v[x + 2] *= rs * cs.z; v[x + 3] *= rs * cs.w;
             }
             v[x] += bb.x; v[x + 1] += bb.y; v[x + 2] += bb.z; v[x + 3] += bb.w;
           }
           activate_all<SLOPE>(e.act, v, sl);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint4* at = reinterpret_cast<uint4*>(staged(buf, lane, 4 * h + q));
+          for (int q = 0; q < 2; ++q) {
+            uint4* at = reinterpret_cast<uint4*>(staged(buf, lane, 2 * h + q));
             uint4 o;
             Out* w = reinterpret_cast<Out*>(&o);
             if (e.res) {
@@ -352,7 +357,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
               int16_t* g = reinterpret_cast<int16_t*>(&f);
 #pragma unroll
               for (int x = 0; x < 8; ++x) g[x] = slope_to_fixed(sl[8 * q + x]);
-              *reinterpret_cast<uint4*>(staged(bufs + 4096, lane, 4 * h + q)) = f;
+              *reinterpret_cast<uint4*>(staged(bufs + 4096, lane, 2 * h + q)) = f;
             }
           }
         }
