@@ -14,7 +14,6 @@ namespace qrb {
 namespace {
 
 constexpr int kSMs = 148;
-constexpr int64_t kPairTiles = 64;
 
 bool float_type(int32_t t) { return t == QRB200_F32 || t == QRB200_BF16 || t == QRB200_F16; }
 int esize(int32_t t) { return t == QRB200_F32 ? 4 : (t == QRB200_E4M3 ? 1 : 2); }
@@ -270,8 +269,7 @@ int launch_tile_as(const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
 template <typename Out, int ES, int T, bool SLOPE>
 int launch_tile(const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
   const int64_t ctas = (int64_t)a.splits * ((a.n + 127) / 128) * ((a.m + T - 1) / T);
-  if (T == 256 || ctas <= kSMs) return launch_tile_as<Out, ES, T, SLOPE, 1>(maps, a, st);
-  return launch_tile_as<Out, ES, T, SLOPE, T == 256 ? 1 : 2>(maps, a, st);
+  return ctas <= kSMs ? launch_tile_as<Out, ES, T, SLOPE, 1>(maps, a, st) : launch_tile_as<Out, ES, T, SLOPE, 2>(maps, a, st);
 }
 
 template <typename Out, int ES, bool SLOPE>
@@ -280,8 +278,7 @@ int launch_tile_t(int T, const lin::Maps& maps, const lin::Args& a, cudaStream_t
     case 16: return launch_tile<Out, ES, 16, SLOPE>(maps, a, st);
     case 32: return launch_tile<Out, ES, 32, SLOPE>(maps, a, st);
     case 64: return launch_tile<Out, ES, 64, SLOPE>(maps, a, st);
-    case 128: return launch_tile<Out, ES, 128, SLOPE>(maps, a, st);
-    default: return launch_tile<Out, ES, 256, SLOPE>(maps, a, st);
+    default: return launch_tile<Out, ES, 128, SLOPE>(maps, a, st);
   }
 }
 
@@ -367,11 +364,55 @@ int product_token(const lin::TokenArgs& a, cudaStream_t st) {
   return vec ? launch_token<Out, In, 4, true>(a, st) : launch_token<Out, In, 4, false>(a, st);
 }
 
+// Which kernel and tile: the least of their times by a model of them, in microseconds, that fits
+// what a sweep over 18 sizes measured (64 x 4096 x 4096 to 2048^3, each at 5 to 7 choices) and picks
+// the fastest or one within 4% of it on all of them.  Every kernel moves its operands at the rate
+// at which an SM can fetch them, so a CTA's time is its blocks of 128 bytes of k times a cost a block.
+//   pair kernel, 256 x 256: 8 + 0.33 a block and wave over 74 pairs; 256 x 128: 7.3 + 0.31
+//   (2048^3: 18.6, measured 19.2; 512 x 4096 x 4096 in 256 x 128: 27.1, measured 27.3)
+//   tile kernel, 128 x T: 7.3 + T / 128 + 0.21 to 0.28 a block with one CTA an SM, 0.30 to 0.44 with
+//   two, and 0.6 to 3.5 for a cluster's exchange (128 x 4096 x 4096 over clusters of 4: 14.0, measured 13.9)
+struct Choice { bool pair; int tile, splits; };
+Choice choose(int64_t m, int64_t n, int64_t k, int es, bool p_row) {
+  const int64_t nkb = (k * es + 127) / 128, tj = (n + 127) / 128;
+  Choice best{false, 128, 1};
+  double least = 1e30;
+  auto offer = [&](const Choice& c, double t) {
+    if (t < least) {
+      least = t;
+      best = c;
+    }
+  };
+  const struct { int tile; double alone, shared; } kinds[] = {{16, 0.21, 0.30}, {32, 0.21, 0.32}, {64, 0.22, 0.36}, {128, 0.28, 0.44}};
+  const struct { int splits; double exchange; } clusters[] = {{1, 0.0}, {2, 0.6}, {4, 1.2}, {8, 3.5}};
+  for (const auto& kind : kinds) {
+    const int T = kind.tile;
+    // no tile that a narrower one would hold, none that m takes more than two of (128: any number);
+    // operands contiguous along their rows come 64 rows at a time
+    if ((p_row && T < 64) || (T < 128 && m > 2 * T) || (T > (p_row ? 64 : 16) && m <= T / 2)) continue;
+    const int64_t tiles = tj * ((m + T - 1) / T);
+    for (const auto& cl : clusters) {
+      if (cl.splits > 1 && nkb / cl.splits < 2) break;
+      const int64_t ctas = tiles * cl.splits, part = (nkb + cl.splits - 1) / cl.splits, waves = (ctas + 2 * kSMs - 1) / (2 * kSMs);
+      const double body = ctas <= kSMs ? part * kind.alone : waves * part * kind.shared * (waves > 1 ? 1.25 : 1.0);
+      offer({false, T, cl.splits}, 7.3 + T / 128.0 + cl.exchange + body);
+    }
+  }
+  if (m > 128 && k > 0)
+    for (const int tn : {128, 256}) {
+      const int64_t tiles = ((m + 255) / 256) * ((n + tn - 1) / tn), waves = (tiles + kSMs / 2 - 1) / (kSMs / 2);
+      offer({true, tn, 1}, tn == 256 ? 8.0 + waves * nkb * 0.33 : 7.3 + waves * nkb * 0.31);
+    }
+  return best;
+}
+
 // D = epilogue(P Q^T); P is m x k, Q is n x k, both addressable by TMA.
 int product(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t out_dtype,
             const lin::Epilogue& e, cudaStream_t st) {
-  // Enough 256 x 256 tiles for most of the 74 CTA pairs: the persistent kernel.
-  if (k > 0 && m > 128 && ((m + 255) / 256) * ((n + 255) / 256) >= kPairTiles) return product_pair<256>(P, Q, m, n, k, dtype, out_dtype, e, st);
+  const Choice choice = choose(m, n, k, esize(dtype), P.row_major);
+  if (choice.pair)
+    return choice.tile == 256 ? product_pair<256>(P, Q, m, n, k, dtype, out_dtype, e, st)
+                              : product_pair<128>(P, Q, m, n, k, dtype, out_dtype, e, st);
   lin::Args a{};
   a.m = (int)m; a.n = (int)n; a.k = (int)k;
   a.e = e;
@@ -380,20 +421,8 @@ int product(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_t k,
   auto on8 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; };
   a.vec = on8(e.out) && e.ldo % 4 == 0 && (!e.bias || on8(e.bias)) &&
           (!e.res || (on8(e.res) && e.ldr % 4 == 0)) && (!e.slope || (on8(e.slope) && n % 4 == 0));
-  // Few rows of P: the narrowest tile that holds them.  Otherwise 128 x 256 tiles where they fill
-  // the GPU, and 128 x 128 ones where only those do.
-  int T;
-  const int64_t tj = (n + 127) / 128;
-  if (m <= 16 && !P.row_major) T = 16;
-  else if (m <= 32 && !P.row_major) T = 32;
-  else if (m <= 64) T = 64;
-  else if (m <= 128 || tj * ((m + 255) / 256) < kSMs) T = 128;
-  else T = 256;
-  // Too few tiles for the GPU: a cluster shares each tile's sum, at least 4 blocks of k a CTA.
-  const int64_t tiles = tj * ((m + T - 1) / T), room = T == 256 ? kSMs : 2 * kSMs;
-  const int nkb = (int)((k * a.es + 127) / 128);
-  a.splits = 1;
-  while (a.splits < 8 && tiles * a.splits * 2 <= room && nkb / (a.splits * 2) >= 4) a.splits *= 2;
+  const int T = choice.tile, nkb = (int)((k * a.es + 127) / 128);
+  a.splits = choice.splits;
   a.part = (nkb + a.splits - 1) / a.splits;
   a.idesc = lin::idesc(dtype == QRB200_BF16 ? 1 : 0, a.q_row, a.p_row, lin::kTileQ, T);
   lin::Maps maps{};
