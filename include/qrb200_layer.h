@@ -73,16 +73,16 @@ int qrb200_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_
  *   x_scale  [m], w_scale [n], float32, or NULL for ones
  *   bias     [n], residual [m][n], y [m][n]: `out_dtype` (= `dtype`; BF16 or F16 for E4M3);
  *            residual may be y itself (in place)
- *   slope    [m][n] contiguous int16, or NULL: act'(z) for qrb200_linear_backward, in steps of
- *            2^-14 (-32768: NaN); not for E4M3
- * Sums are float32; y is rounded once.  `workspace` (NULL: allocated stream-ordered) holds aligned
+ *   slope    [m][n] contiguous, or NULL: act'(z) for qrb200_linear_backward as
+ *            round(2^15 (act' + 1/4)), 65535 for NaN; not for E4M3
+ * m and n up to 8388480 (128 * 65535).  Sums are float32; y is rounded once.  `workspace` (NULL: allocated stream-ordered) holds aligned
  * copies of operands whose rows do not all start on 16 bytes; none is needed otherwise. */
 int qrb200_linear_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw,
                                   int32_t w_transposed, int64_t m, int64_t n, int64_t k,
                                   int32_t dtype, size_t* bytes);
 int qrb200_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t w_transposed,
                   const float* x_scale, const float* w_scale, const void* bias,
-                  const void* residual, int64_t ldr, void* y, int64_t ldy, int16_t* slope,
+                  const void* residual, int64_t ldr, void* y, int64_t ldy, uint16_t* slope,
                   int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t out_dtype,
                   int32_t activation, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -95,7 +95,7 @@ int qrb200_linear_backward_workspace_bytes(const void* dy, int64_t lddy, int32_t
                                            int64_t ldw, int32_t w_transposed, int32_t want_dx,
                                            int32_t want_dw, int32_t want_dbias, int64_t m,
                                            int64_t n, int64_t k, size_t* bytes);
-int qrb200_linear_backward(const void* dy, int64_t lddy, const int16_t* slope, const void* x,
+int qrb200_linear_backward(const void* dy, int64_t lddy, const uint16_t* slope, const void* x,
                            int64_t ldx, const void* w, int64_t ldw, int32_t w_transposed,
                            void* dx, void* dw, void* dbias, int64_t m, int64_t n, int64_t k,
                            int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);

@@ -452,7 +452,7 @@ int64_t dz_parts(int64_t m, int64_t n) {
 }
 
 template <typename T>
-int launch_dz(const void* dy, int64_t lddy, const int16_t* slope, void* dz, int64_t lddz, float* part, int64_t m,
+int launch_dz(const void* dy, int64_t lddy, const uint16_t* slope, void* dz, int64_t lddz, float* part, int64_t m,
               int64_t n, int64_t parts, cudaStream_t st) {
   const bool vec = n % 8 == 0 && rows_on16(dy, lddy, 2) && (!slope || on16(slope)) && (!dz || on16(dz));
   const dim3 grid((unsigned)((n + 255) / 256), (unsigned)parts);
@@ -592,7 +592,7 @@ int qrb200_linear_workspace_bytes(const void* x, int64_t ldx, const void* w, int
 
 int qrb200_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t w_transposed, const float* x_scale,
                   const float* w_scale, const void* bias, const void* residual, int64_t ldr, void* y, int64_t ldy,
-                  int16_t* slope, int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t out_dtype,
+                  uint16_t* slope, int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t out_dtype,
                   int32_t activation, void* workspace, size_t workspace_bytes, void* stream) {
   const bool q8 = dtype == QRB200_E4M3;
   if (!(dtype == QRB200_BF16 || dtype == QRB200_F16 || q8) || !sizes_ok(m, n, k)) return QRB200_ERR_INVALID_ARG;
@@ -633,7 +633,7 @@ int qrb200_linear_backward_workspace_bytes(const void* dy, int64_t lddy, int32_t
   return QRB200_OK;
 }
 
-int qrb200_linear_backward(const void* dy, int64_t lddy, const int16_t* slope, const void* x, int64_t ldx,
+int qrb200_linear_backward(const void* dy, int64_t lddy, const uint16_t* slope, const void* x, int64_t ldx,
                            const void* w, int64_t ldw, int32_t w_transposed, void* dx, void* dw, void* dbias,
                            int64_t m, int64_t n, int64_t k, int32_t dtype, void* workspace, size_t workspace_bytes,
                            void* stream) {

@@ -17,6 +17,7 @@
 #pragma once
 #include <cuda_fp8.h>
 
+#include "qrb_f2.cuh"
 #include "qrb_tc.cuh"
 #include "qrb_tmap.cuh"
 
@@ -36,7 +37,7 @@ struct Epilogue {
   int64_t ldr;
   void* out;
   int64_t ldo;
-  int16_t* slope;          // act'(z), m x n contiguous, or null (see kSlopeOne)
+  uint16_t* slope;         // act'(z), m x n contiguous, or null (see slope_bits)
   int act;
 };
 
@@ -55,15 +56,19 @@ struct Maps {
   CUtensorMap p, q;
 };
 
-// act' is kept for the backward pass in 16 bits of fixed point: it lies in (-0.13, 1.13) for every
-// activation here, so steps of 2^-14 hold 0 and 1 exactly and the rest to 3e-5, where a bf16 act'
-// or z would be off by up to 2e-3 of its value.  -32768 stands for NaN.
-constexpr float kSlopeOne = 16384.f;
-__device__ __forceinline__ int16_t slope_to_fixed(float s) {
-  return s != s ? (int16_t)-32768 : (int16_t)__float2int_rn(s * kSlopeOne);
+// act' is kept for the backward pass in 16 bits of fixed point, 2^15 (act' + 1/4): it lies in
+// (-0.13, 1.13) for every activation here, so steps of 2^-15 hold 0 and 1 exactly and the rest to
+// 1.6e-5, where a bf16 act' or z would be off by up to 2e-3 of its value.  65535 stands for NaN.
+// Adding 2^23 rounds to an integer and leaves it in the low bits; those of a NaN are all ones.
+__device__ __forceinline__ F2 slope_bits(F2 s) { return fma(s, f2(32768.f), f2(8388608.f + 8192.f)); }
+__device__ __forceinline__ uint32_t pack_slopes(F2 s) {  // two of them
+  float a, b;
+  split(slope_bits(s), a, b);
+  return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x5410);
 }
-__device__ __forceinline__ float slope_from_fixed(int16_t f) {
-  return f == -32768 ? __int_as_float(0x7FFFFFFF) : (float)f * (1.f / kSlopeOne);
+__device__ __forceinline__ float slope_value(uint32_t bits) {
+  const float v = fmaf(__uint_as_float(0x4B000000u | bits), 1.f / 32768.f, -256.25f);
+  return bits == 0xFFFFu ? __int_as_float(0x7FFFFFFF) : v;
 }
 
 // 1 / x and 2^x of the special-function unit, good to about 2^-22 of the result.
@@ -72,61 +77,80 @@ __device__ __forceinline__ float rcp_fast(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ float exp_fast(float x) {
+__device__ __forceinline__ float exp2_fast(float x) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ F2 rcp(F2 x) {
+  float a, b;
+  split(x, a, b);
+  return f2(rcp_fast(a), rcp_fast(b));
+}
+__device__ __forceinline__ F2 exp2_(F2 x) {
+  float a, b;
+  split(x, a, b);
+  return f2(exp2_fast(a), exp2_fast(b));
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN stays
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
-// act(z); with SLOPE also act'(z).  The epilogue runs beside the MMAs and shares their power, so
-// each costs two special functions and a dozen multiply-adds: gelu takes the normal integral from
-// Abramowitz and Stegun's approximation 7.1.26 of the error function (off by 1.5e-7 at most),
+// act(z) of two values; with SLOPE also act'(z).  The epilogue runs beside the MMAs and shares their
+// power, so every instruction shows: two special functions and about seven others a value.  gelu
+// takes the normal integral from Abramowitz and Stegun's approximation 7.1.26 of the error function
+// (off by 1.5e-7 at most),
 //   Phi(-|z|) = exp(-z^2 / 2) (a1 t + ... + a5 t^5) / 2,  t = 1 / (1 + p |z| / sqrt 2),
-// whose exponential is also the one that its slope needs (4096 x 16384 x 4096 with gelu: 431 us with
-// erff, see the table of measurements for the present figure).
-template <bool SLOPE>
-__device__ __forceinline__ float activate(int act, float z, float& slope) {
-  switch (act) {
-    case ACT_RELU:
-      if (SLOPE) slope = z > 0.f ? 1.f : (z != z ? z : 0.f);
-      return z < 0.f ? 0.f : z;  // NaN stays
-    case ACT_GELU: {
-      const float x = fabsf(z) * 0.70710678118654752f;
-      const float t = rcp_fast(fmaf(0.3275911f, x, 1.f));
-      const float ex = exp_fast(-x * x);
-      float s = fmaf(1.061405429f, t, -1.453152027f);
-      s = fmaf(s, t, 1.421413741f);
-      s = fmaf(s, t, -0.284496736f);
-      s = fmaf(s, t, 0.254829592f);
-      const float tail = 0.5f * s * t * ex;  // Phi(-|z|)
-      const float phi = z > 0.f ? 1.f - tail : tail;
-      if (SLOPE) slope = fmaf(z * 0.3989422804014327f, ex, phi);
-      return z * phi;
+// as z Phi(z) = max(z, 0) - |z| Phi(-|z|); its slope needs the same exponential.
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ F2 activate(F2 z, F2& slope) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  float a, b;
+  split(z, a, b);
+  if constexpr (ACT == ACT_RELU) {
+    if (SLOPE) slope = f2(a > 0.f ? 1.f : (a != a ? a : 0.f), b > 0.f ? 1.f : (b != b ? b : 0.f));
+    return f2(max_nan(a, 0.f), max_nan(b, 0.f));
+  } else if constexpr (ACT == ACT_GELU) {
+    const float ma = fminf(fabsf(a), 1e18f), mb = fminf(fabsf(b), 1e18f);  // finite: times a tail of 0
+    const F2 m = f2(ma, mb);
+    const F2 t = rcp(fma(m, f2(0.3275911f * 0.70710678118654752f), f2(1.f)));
+    const F2 ex = exp2_(mul(mul(z, z), f2(-0.5f * kLog2e)));
+    F2 s = fma(t, f2(0.5f * 1.061405429f), f2(0.5f * -1.453152027f));
+    s = fma(s, t, f2(0.5f * 1.421413741f));
+    s = fma(s, t, f2(0.5f * -0.284496736f));
+    s = fma(s, t, f2(0.5f * 0.254829592f));
+    const F2 tail = mul(mul(s, t), ex);  // Phi(-|z|)
+    if (SLOPE) {
+      float ta, tb;
+      split(tail, ta, tb);
+      slope = fma(mul(z, ex), f2(0.3989422804014327f), f2(a > 0.f ? 1.f - ta : ta, b > 0.f ? 1.f - tb : tb));
     }
-    case ACT_GELU_TANH: {  // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
-      const float z2 = fminf(z * z, 1e30f);  // its product with a vanished 1 - p stays 0
-      const float p = rcp_fast(1.f + exp_fast(-1.5957691216057308f * z * fmaf(0.044715f, z2, 1.f)));
-      if (SLOPE) slope = fmaf(z * p * (1.f - p) * 1.5957691216057308f, fmaf(0.134145f, z2, 1.f), p);
-      return z * p;
-    }
-    case ACT_SILU: {
-      const float p = rcp_fast(1.f + exp_fast(-z));
-      if (SLOPE) slope = p * fmaf(z, 1.f - p, 1.f);
-      return z * p;
-    }
-    default:
-      if (SLOPE) slope = 1.f;
-      return z;
+    return fma(f2(-ma, -mb), tail, f2(max_nan(a, 0.f), max_nan(b, 0.f)));
+  } else if constexpr (ACT == ACT_GELU_TANH) {  // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
+    const F2 z2 = f2(fminf(a * a, 1e30f), fminf(b * b, 1e30f));  // its product with a vanished 1 - p stays 0
+    const F2 p = rcp(add(exp2_(mul(mul(z, f2(-1.5957691216057308f * kLog2e)), fma(z2, f2(0.044715f), f2(1.f)))), f2(1.f)));
+    const F2 y = mul(z, p);
+    if (SLOPE) slope = fma(mul(mul(y, fma(p, f2(-1.f), f2(1.f))), f2(1.5957691216057308f)), fma(z2, f2(0.134145f), f2(1.f)), p);
+    return y;
+  } else if constexpr (ACT == ACT_SILU) {
+    const F2 p = rcp(add(exp2_(mul(z, f2(-kLog2e))), f2(1.f)));
+    if (SLOPE) slope = mul(p, fma(z, fma(p, f2(-1.f), f2(1.f)), f2(1.f)));
+    return mul(z, p);
+  } else {
+    if (SLOPE) slope = f2(1.f);
+    return z;
   }
 }
 template <int ACT, bool SLOPE, int N>
-__device__ __forceinline__ void activate_as(float (&v)[N], float (&sl)[N]) {
+__device__ __forceinline__ void activate_as(F2 (&v)[N], F2 (&sl)[N]) {
 #pragma unroll
-  for (int c = 0; c < N; ++c) v[c] = activate<SLOPE>(ACT, v[c], sl[c]);
+  for (int c = 0; c < N; ++c) v[c] = activate<ACT, SLOPE>(v[c], sl[c]);
 }
-// activate() on N values, with the choice made once.
+// act() of 2N values, with the choice made once.
 template <bool SLOPE, int N>
-__device__ __forceinline__ void activate_all(int act, float (&v)[N], float (&sl)[N]) {
+__device__ __forceinline__ void activate_all(int act, F2 (&v)[N], F2 (&sl)[N]) {
   switch (act) {
     case ACT_RELU: activate_as<ACT_RELU, SLOPE>(v, sl); break;
     case ACT_GELU: activate_as<ACT_GELU, SLOPE>(v, sl); break;
@@ -134,6 +158,25 @@ __device__ __forceinline__ void activate_all(int act, float (&v)[N], float (&sl)
     case ACT_SILU: activate_as<ACT_SILU, SLOPE>(v, sl); break;
     default: activate_as<ACT_NONE, SLOPE>(v, sl);
   }
+}
+
+// Two 16-bit values <-> float32 pair.
+__device__ __forceinline__ F2 widen2(uint32_t w, __nv_bfloat16) { return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ F2 widen2(uint32_t w, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return f2(f.x, f.y);
+}
+__device__ __forceinline__ uint32_t narrow2(F2 x, __nv_bfloat16) {
+  float a, b;
+  split(x, a, b);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t narrow2(F2 x, __half) {
+  float a, b;
+  split(x, a, b);
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // ---- small PTX helpers on top of qrb_tc.cuh ----
@@ -401,7 +444,7 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
 #pragma unroll 1
     for (int x0 = warp; x0 < per; x0 += 16) {  // rows x0 and x0 + 8 of this CTA's
       uint2 res[2];
-      float v[8], sl[8];
+      F2 v[4], sl[4];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         const int x = x0 + 8 * y, il = rank * per + x, i = i0 + il;
@@ -423,27 +466,24 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
             u = *reinterpret_cast<const float4*>(at);
           }
         }
-        const float z[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[4 * y + c] = (ES == 1 ? z[c] * (rs * cscale[c]) : z[c]) + bias[c];
+        F2 lo = f2(u.x, u.y), hi = f2(u.z, u.w);
+        if (ES == 1) {
+          lo = mul(lo, mul(f2(rs), f2(cscale[0], cscale[1])));
+          hi = mul(hi, mul(f2(rs), f2(cscale[2], cscale[3])));
+        }
+        v[2 * y] = add(lo, f2(bias[0], bias[1]));
+        v[2 * y + 1] = add(hi, f2(bias[2], bias[3]));
       }
       activate_all<SLOPE>(e.act, v, sl);
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         const int x = x0 + 8 * y, i = i0 + rank * per + x;
         if (x >= per || i >= a.m) continue;
-        float r[4];
-        widen4<Out>(res[y], r);
-        uint2 packed, slopes;
-        Out* o = reinterpret_cast<Out*>(&packed);
-        int16_t* f = reinterpret_cast<int16_t*>(&slopes);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          o[c] = from_f32<Out>(v[4 * y + c] + r[c]);
-          if (SLOPE) f[c] = slope_to_fixed(sl[4 * y + c]);
-        }
+        const uint2 packed = make_uint2(narrow2(add(v[2 * y], widen2(res[y].x, Out())), Out()),
+                                        narrow2(add(v[2 * y + 1], widen2(res[y].y, Out())), Out()));
         put4(static_cast<Out*>(e.out) + (int64_t)i * e.ldo + j, packed, a.vec, left);
-        if (SLOPE) put4(e.slope + (int64_t)i * a.n + j, slopes, a.vec, left);
+        if (SLOPE)
+          put4(e.slope + (int64_t)i * a.n + j, make_uint2(pack_slopes(sl[2 * y]), pack_slopes(sl[2 * y + 1])), a.vec, left);
       }
     }
   }
@@ -606,9 +646,11 @@ __global__ void __launch_bounds__(256) token_kernel(TokenArgs a) {
     for (int p = 0; p < SPLIT; ++p) sum += s_part[p][lane];
   }
   if (!mine) return;
-  float slope;
-  const float v = activate<false>(e.act, sum * scale + bias, slope) + res;
-  static_cast<Out*>(e.out)[(int64_t)i * e.ldo + j] = from_f32<Out>(v);
+  F2 v[1] = {f2(sum * scale + bias)}, slope[1];
+  activate_all<false>(e.act, v, slope);
+  float y, same;
+  split(v[0], y, same);
+  static_cast<Out*>(e.out)[(int64_t)i * e.ldo + j] = from_f32<Out>(y + res);
 }
 
 // ---- dz = dy act'(z), and the column sums of dz (the bias' gradient) ----
@@ -617,7 +659,7 @@ __global__ void __launch_bounds__(256) token_kernel(TokenArgs a) {
 // before dz is rounded to the operands' type for the two products.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-    dz_kernel(const T* dy, int64_t lddy, const int16_t* slope, T* dz, int64_t lddz, float* part,
+    dz_kernel(const T* dy, int64_t lddy, const uint16_t* slope, T* dz, int64_t lddz, float* part,
               int64_t m, int64_t n) {
   __shared__ float s[8][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -625,7 +667,7 @@ __global__ void __launch_bounds__(256)
   float sum[8] = {};
   for (int64_t i = (int64_t)blockIdx.y * 8 + warp; i < m; i += (int64_t)gridDim.y * 8) {
     const T* src = dy + i * lddy;
-    const int16_t* sl = slope ? slope + i * n : nullptr;
+    const uint16_t* sl = slope ? slope + i * n : nullptr;
     T* dst = dz ? dz + i * lddz : nullptr;
     if (VEC) {
       const int64_t j = j0 + 8 * lane;
@@ -637,9 +679,9 @@ __global__ void __launch_bounds__(256)
       for (int c = 0; c < 8; ++c) v[c] = to_f32(e[c]);
       if (sl) {
         const uint4 f = *reinterpret_cast<const uint4*>(sl + j);
-        const int16_t* g = reinterpret_cast<const int16_t*>(&f);
+        const uint16_t* g = reinterpret_cast<const uint16_t*>(&f);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] *= slope_from_fixed(g[c]);
+        for (int c = 0; c < 8; ++c) v[c] *= slope_value(g[c]);
       }
 #pragma unroll
       for (int c = 0; c < 8; ++c) sum[c] += v[c];
@@ -656,7 +698,7 @@ __global__ void __launch_bounds__(256)
         const int64_t j = j0 + 32 * c + lane;
         if (j >= n) continue;
         float v = to_f32(src[j]);
-        if (sl) v *= slope_from_fixed(sl[j]);
+        if (sl) v *= slope_value(sl[j]);
         sum[c] += v;
         if (dst) dst[j] = from_f32<T>(v);
       }

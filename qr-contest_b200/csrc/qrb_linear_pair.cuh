@@ -309,12 +309,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         // the loop does
 #pragma unroll 1
         for (int h = 0; h < 4; ++h) {
-          float v[16], sl[16];
+          float raw[16];
           if (ok) {
-            tmem_ld16(tmem + b * TN + lane_base + c0 + 16 * h, v);
+            tmem_ld16(tmem + b * TN + lane_base + c0 + 16 * h, raw);
           } else {
 #pragma unroll
-            for (int x = 0; x < 16; ++x) v[x] = __int_as_float(0x7FFFFFFF);
+            for (int x = 0; x < 16; ++x) raw[x] = __int_as_float(0x7FFFFFFF);
           }
           if (h == 3 && c0 + 64 == (half + 1) * (TN / 2)) {  // the sums are in registers
             tc::tc_fence_before();
@@ -329,36 +329,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             __syncwarp();
           }
           const int hc = 16 * (h & 1);
+          F2 v[8], sl[8];
 #pragma unroll
-          for (int x = 0; x < 16; x += 4) {
-            const float4 bb = *reinterpret_cast<const float4*>(&s_col[warp][0][hc + x]);
+          for (int x = 0; x < 8; x += 2) {
+            const float4 bb = *reinterpret_cast<const float4*>(&s_col[warp][0][hc + 2 * x]);
+            F2 lo = f2(raw[2 * x], raw[2 * x + 1]), hi = f2(raw[2 * x + 2], raw[2 * x + 3]);
             if (ES == 1) {
-              const float4 cs = *reinterpret_cast<const float4*>(&s_col[warp][1][hc + x]);
-              v[x] *= rs * cs.x; v[x + 1] *= rs * cs.y; v[x + 2] *= rs * cs.z; v[x + 3] *= rs * cs.w;
+              const float4 cs = *reinterpret_cast<const float4*>(&s_col[warp][1][hc + 2 * x]);
+              lo = mul(lo, mul(f2(rs), f2(cs.x, cs.y)));
+              hi = mul(hi, mul(f2(rs), f2(cs.z, cs.w)));
             }
-            v[x] += bb.x; v[x + 1] += bb.y; v[x + 2] += bb.z; v[x + 3] += bb.w;
+            v[x] = add(lo, f2(bb.x, bb.y));
+            v[x + 1] = add(hi, f2(bb.z, bb.w));
           }
           activate_all<SLOPE>(e.act, v, sl);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             uint4* at = reinterpret_cast<uint4*>(staged(buf, lane, 2 * h + q));
-            uint4 o;
-            Out* w = reinterpret_cast<Out*>(&o);
+            F2* w = v + 4 * q;
             if (e.res) {
-              o = *at;
-#pragma unroll
-              for (int x = 0; x < 8; ++x) v[8 * q + x] += to_f32(w[x]);
+              const uint4 r = *at;
+              w[0] = add(w[0], widen2(r.x, Out())); w[1] = add(w[1], widen2(r.y, Out()));
+              w[2] = add(w[2], widen2(r.z, Out())); w[3] = add(w[3], widen2(r.w, Out()));
             }
-#pragma unroll
-            for (int x = 0; x < 8; ++x) w[x] = from_f32<Out>(v[8 * q + x]);
-            *at = o;
-            if (SLOPE) {
-              uint4 f;
-              int16_t* g = reinterpret_cast<int16_t*>(&f);
-#pragma unroll
-              for (int x = 0; x < 8; ++x) g[x] = slope_to_fixed(sl[8 * q + x]);
-              *reinterpret_cast<uint4*>(staged(bufs + 4096, lane, 2 * h + q)) = f;
-            }
+            *at = make_uint4(narrow2(w[0], Out()), narrow2(w[1], Out()), narrow2(w[2], Out()), narrow2(w[3], Out()));
+            if (SLOPE)
+              *reinterpret_cast<uint4*>(staged(bufs + 4096, lane, 2 * h + q)) =
+                  make_uint4(pack_slopes(sl[4 * q]), pack_slopes(sl[4 * q + 1]), pack_slopes(sl[4 * q + 2]), pack_slopes(sl[4 * q + 3]));
           }
         }
         if (live) {

@@ -20,6 +20,7 @@
 #include <cuda_fp8.h>
 
 #include "qrb_common.cuh"
+#include "qrb_f2.cuh"
 
 namespace qrb {
 namespace norm {
@@ -399,24 +400,6 @@ struct BwdArgs {
   float eps;
 };
 
-// Two float32 values in a register pair: one instruction does the arithmetic of both.
-struct F2 { unsigned long long v; };
-__device__ __forceinline__ F2 f2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void split(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
-__device__ __forceinline__ F2 mul(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
 __device__ __forceinline__ void pairs(const float (&v)[8], F2 (&p)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) p[j] = f2(v[2 * j], v[2 * j + 1]);

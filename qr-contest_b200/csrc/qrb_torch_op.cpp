@@ -305,7 +305,7 @@ std::tuple<at::Tensor, at::Tensor> linear(const at::Tensor& x, const at::Tensor&
   if (bytes) ws = fresh({(int64_t)bytes}, x, at::kByte);
   check_rc(qrb200_linear(rx.t.data_ptr(), rx.ld, w.t.data_ptr(), w.ld, w.transposed, static_cast<const float*>(ptr(xs)),
                          static_cast<const float*>(ptr(wsc)), ptr(b), ptr(rr.t), rr.ld, y.data_ptr(), n,
-                         static_cast<int16_t*>(ptr(slope)), rx.rows, n, k, layer_code(xt), layer_code(ot), (int32_t)activation,
+                         static_cast<uint16_t*>(ptr(slope)), rx.rows, n, k, layer_code(xt), layer_code(ot), (int32_t)activation,
                          ptr(ws), bytes, cur_stream(x)),
            "qrb200_linear");
   return {y, slope};
@@ -344,7 +344,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward(const at::Tensor&
            "qrb200_linear_backward_workspace_bytes");
   at::Tensor ws;
   if (bytes) ws = fresh({(int64_t)bytes}, dy, at::kByte);
-  check_rc(qrb200_linear_backward(rg.t.data_ptr(), rg.ld, slope ? static_cast<const int16_t*>(slope->data_ptr()) : nullptr,
+  check_rc(qrb200_linear_backward(rg.t.data_ptr(), rg.ld, slope ? static_cast<const uint16_t*>(slope->data_ptr()) : nullptr,
                                   rx.t.data_ptr(), rx.ld, w.t.data_ptr(), w.ld, w.transposed, ptr(dx), ptr(dw), ptr(db),
                                   rg.rows, n, k, layer_code(t), ptr(ws), bytes, cur_stream(dy)),
            "qrb200_linear_backward");
