@@ -209,22 +209,30 @@ size_t aligned_copy_bytes(const Operand& o, int64_t rows, int64_t k, int es) {
   const size_t b = (size_t)o.stored_rows(rows, k) * padded_cols(o.stored_cols(rows, k), es) * es;
   return (b + 255) & ~size_t(255);
 }
-// Copies an operand whose rows TMA cannot address to `buf` and points it there.
-int make_addressable(Operand& o, int64_t rows, int64_t k, int es, char*& buf, cudaStream_t st) {
-  const size_t bytes = aligned_copy_bytes(o, rows, k, es);
-  if (!bytes) return QRB200_OK;
-  const int64_t sr = o.stored_rows(rows, k), sc = o.stored_cols(rows, k), ldd = padded_cols(sc, es);
-  const int64_t vecs = sr * ldd * es / 16;
-  const unsigned grid = (unsigned)std::min<int64_t>((vecs + 255) / 256, kSMs * 8);
-  if (es == 2)
-    lin::align_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(o.p), o.ld, sc, reinterpret_cast<uint16_t*>(buf), ldd, sr);
-  else
-    lin::align_rows_kernel<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(o.p), o.ld, sc, reinterpret_cast<uint8_t*>(buf), ldd, sr);
-  o.p = buf;
-  o.ld = ldd;
-  buf += bytes;
-  return launched();
-}
+// Points operands whose rows TMA cannot address to copies in `buf`, all made by one launch.
+struct Aligner {
+  lin::AlignJobs jobs{};
+  int count = 0, es;
+  int64_t most = 0;  // 16-byte pieces of the largest
+  char* buf;
+  void want(Operand& o, int64_t rows, int64_t k) {
+    const size_t bytes = aligned_copy_bytes(o, rows, k, es);
+    if (!bytes) return;
+    const int64_t sr = o.stored_rows(rows, k), sc = o.stored_cols(rows, k), ldd = padded_cols(sc, es);
+    jobs.job[count++] = {o.p, o.ld, sc, sr, buf, ldd};
+    most = std::max(most, sr * ldd * es / 16);
+    o.p = buf;
+    o.ld = ldd;
+    buf += bytes;
+  }
+  int run(cudaStream_t st) const {
+    if (!count) return QRB200_OK;
+    const dim3 grid((unsigned)std::min<int64_t>((most + 255) / 256, kSMs * 8), (unsigned)count);
+    if (es == 2) lin::align_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(jobs);
+    else lin::align_rows_kernel<uint8_t><<<grid, 256, 0, st>>>(jobs);
+    return launched();
+  }
+};
 
 bool encode_operand(CUtensorMap* map, const Operand& o, int64_t rows, int64_t k, int32_t dtype, int box_rows) {
   EncodeTiledFn fn = encode_tiled_fn();
@@ -614,9 +622,12 @@ int qrb200_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_
   Scratch ws(st);
   int rc = ws.get(workspace, workspace_bytes,
                   k ? aligned_copy_bytes(X, m, k, es) + aligned_copy_bytes(W, n, k, es) : 0);
-  char* buf = static_cast<char*>(ws.p);
-  if (rc == QRB200_OK && k) rc = make_addressable(X, m, k, es, buf, st);
-  if (rc == QRB200_OK && k) rc = make_addressable(W, n, k, es, buf, st);
+  if (rc == QRB200_OK && k) {
+    Aligner align{{}, 0, es, 0, static_cast<char*>(ws.p)};
+    align.want(X, m, k);
+    align.want(W, n, k);
+    rc = align.run(st);
+  }
   if (rc != QRB200_OK) return rc;
   return product(X, W, m, n, k, dtype, out_dtype, e, st);
 }
@@ -669,18 +680,19 @@ int qrb200_linear_backward(const void* dy, int64_t lddy, const uint16_t* slope, 
   }
   if (!dx && !dw) return QRB200_OK;
   Operand G = dz ? Operand{dz, p.lddz, false} : Operand{dy, lddy, false};
-  rc = make_addressable(G, m, n, 2, buf, st);
+  Operand Wt{w, ldw, !W.row_major}, Xt{x, ldx, true};
+  Aligner align{{}, 0, 2, 0, buf};
+  align.want(G, m, n);
+  if (dx) align.want(Wt, k, n);
+  if (dw) align.want(Xt, k, m);
+  rc = align.run(st);
   if (rc == QRB200_OK && dx) {  // dx_ik = sum_j dz_ij W_jk
-    Operand Wt{w, ldw, !W.row_major};
-    rc = make_addressable(Wt, k, n, 2, buf, st);
     lin::Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dx, k, nullptr, lin::ACT_NONE};
-    if (rc == QRB200_OK) rc = product(G, Wt, m, k, n, dtype, dtype, e, st);
+    rc = product(G, Wt, m, k, n, dtype, dtype, e, st);
   }
   if (rc == QRB200_OK && dw) {  // dW_jk = sum_i dz_ij x_ik
-    Operand Xt{x, ldx, true};
-    rc = make_addressable(Xt, k, m, 2, buf, st);
     lin::Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dw, k, nullptr, lin::ACT_NONE};
-    if (rc == QRB200_OK) rc = product(Operand{G.p, G.ld, true}, Xt, n, k, m, dtype, dtype, e, st);
+    rc = product(Operand{G.p, G.ld, true}, Xt, n, k, m, dtype, dtype, e, st);
   }
   return rc;
 }

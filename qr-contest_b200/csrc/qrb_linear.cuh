@@ -715,18 +715,23 @@ __global__ void __launch_bounds__(256)
   if (j < n) part[blockIdx.y * n + j] = t;
 }
 
-// ---- rows of an operand that TMA cannot address (a base or a stride off 16 bytes), copied into
-// rows 16 bytes apart; bound by memory, 16 bytes written a thread ----
+// ---- rows of operands that TMA cannot address (a base or a stride off 16 bytes), copied into rows
+// 16 bytes apart; bound by memory, 16 bytes written a thread; blockIdx.y is the operand ----
+struct AlignJobs {
+  struct { const void* src; int64_t ld, cols, rows; void* dst; int64_t ldd; } job[3];
+};
 template <typename T>
-__global__ void __launch_bounds__(256) align_rows_kernel(const T* src, int64_t ld, int64_t cols, T* dst, int64_t ldd, int64_t rows) {
+__global__ void __launch_bounds__(256) align_rows_kernel(AlignJobs jobs) {
   constexpr int V = 16 / sizeof(T);
-  const int64_t per = ldd / V, total = rows * per;
+  const auto& o = jobs.job[blockIdx.y];
+  const T* src = static_cast<const T*>(o.src);
+  const int64_t per = o.ldd / V, total = o.rows * per;
   for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < total; x += (int64_t)gridDim.x * 256) {
     const int64_t r = x / per, c = x % per * V;
     T v[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = c + e < cols ? src[r * ld + c + e] : T(0);
-    *reinterpret_cast<uint4*>(dst + r * ldd + c) = *reinterpret_cast<const uint4*>(v);
+    for (int e = 0; e < V; ++e) v[e] = c + e < o.cols ? src[r * o.ld + c + e] : T(0);
+    *reinterpret_cast<uint4*>(static_cast<T*>(o.dst) + r * o.ldd + c) = *reinterpret_cast<const uint4*>(v);
   }
 }
 

@@ -25,6 +25,7 @@
 
 #include "qrb200.h"
 #include "qrb200_layer.h"
+#include "qrb_torch_layers.h"
 
 namespace {
 
@@ -89,7 +90,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> geqrf_meta(const at::Tensor& data
 }
 
 // ---------------------------------------------------------------- layer operators
-using OptTensor = c10::optional<at::Tensor>;
+using qrb200::OptTensor;
 
 int32_t layer_code(at::ScalarType t) {
   return t == at::kFloat8_e4m3fn ? QRB200_E4M3 : dtype_code(t);
@@ -397,18 +398,23 @@ struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
   }
 };
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_autograd(const at::Tensor& x, const OptTensor& weight,
-                                                                 const OptTensor& residual, double eps,
-                                                                 c10::optional<at::ScalarType> out_dtype) {
+}  // namespace
+
+// Below autograd with nothing to differentiate; otherwise with a node that can.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> qrb200::rms_norm(const at::Tensor& x, const OptTensor& weight,
+                                                                const OptTensor& residual, double eps,
+                                                                c10::optional<at::ScalarType> out_dtype) {
   const at::Tensor w = weight.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
   if (!wants_grad({&x, &w, &r})) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return rms_norm(x, weight, residual, eps, out_dtype);
+    return ::rms_norm(x, weight, residual, eps, out_dtype);
   }
   TORCH_CHECK_VALUE(!out_dtype || *out_dtype == x.scalar_type(), "qrb200: the 8-bit norm has no gradient (use torch.no_grad())");
   variable_list out = RmsNormGrad::apply(x, weight, residual, eps);
   return {out[0], at::Tensor(), out.size() > 1 ? out[1] : at::Tensor()};
 }
+
+namespace {
 
 struct LinearGrad : torch::autograd::Function<LinearGrad> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
@@ -441,21 +447,21 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
   }
 };
 
-std::tuple<at::Tensor, at::Tensor> linear_autograd(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
-                                                   const OptTensor& residual, int64_t activation, const OptTensor& x_scale,
-                                                   const OptTensor& weight_scale, c10::optional<at::ScalarType> out_dtype,
-                                                   bool want_slope) {
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> qrb200::linear(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
+                                                  const OptTensor& residual, int64_t activation, const OptTensor& x_scale,
+                                                  const OptTensor& weight_scale, c10::optional<at::ScalarType> out_dtype,
+                                                  bool want_slope) {
   const at::Tensor b = bias.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
   if (!wants_grad({&x, &weight, &b, &r})) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return linear(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
+    return ::linear(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
   }
   TORCH_CHECK_VALUE(x.scalar_type() != at::kFloat8_e4m3fn, "qrb200: the 8-bit product has no gradient (use torch.no_grad())");
   TORCH_CHECK_VALUE(!x_scale && !weight_scale, "qrb200: scales belong to 8-bit operands");
   return {LinearGrad::apply(x, weight, bias, residual, activation, out_dtype)[0], at::Tensor()};
 }
-
-}  // namespace
 
 TORCH_LIBRARY(qrb200, m) {
   m.def("geqrf(Tensor A) -> (Tensor H, Tensor tau, Tensor info)");
@@ -488,8 +494,8 @@ TORCH_LIBRARY_IMPL(qrb200, Meta, m) {
 }
 
 TORCH_LIBRARY_IMPL(qrb200, Autograd, m) {
-  m.impl("rms_norm", rms_norm_autograd);
-  m.impl("linear", linear_autograd);
+  m.impl("rms_norm", qrb200::rms_norm);
+  m.impl("linear", qrb200::linear);
 }
 
 // Host tensors (and mixes of host and device tensors, which reach this key too) are refused by the

@@ -73,28 +73,40 @@ def _link(objs, out: Path, verbose: bool) -> None:
     subprocess.run(cmd, check=True)
 
 
-OPS = PKG / "libqrb200_torch_ops.so"  # torch.ops.qrb200.geqrf (links libqrb200.so)
+OPS = PKG / "libqrb200_torch_ops.so"  # torch.ops.qrb200.* (links libqrb200.so)
+PY = PKG / "_layers.so"               # the layer operators' Python functions (links OPS)
 
 
-def _compile_ops(verbose: bool) -> None:
-    """The TORCH_LIBRARY operator library: g++ against torch's headers and libraries, linked
-    to libqrb200.so next to it (rpath $ORIGIN).  No CUDA code is compiled here."""
+def _compile_host(src: Path, out: Path, verbose: bool, include, link) -> None:
+    """A library against torch's headers and libraries, next to the ones it is linked to (rpath
+    $ORIGIN).  No CUDA code is compiled here."""
     import torch
     from torch.utils import cpp_extension as ce
     cuda_home = Path(ce.CUDA_HOME or "/usr/local/cuda")
     abi = int(torch.compiled_with_cxx11_abi())
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-I", str(INCLUDE), "-I", str(cuda_home / "include")]
+           "-I", str(INCLUDE), "-I", str(cuda_home / "include"), *include]
     for d in ce.include_paths():
         cmd += ["-I", d]
-    cmd += ["-o", str(OPS), str(CSRC / "qrb_torch_op.cpp"), "-L", str(PKG), "-l:libqrb200.so",
-            "-Wl,-rpath,$ORIGIN"]
+    cmd += ["-o", str(out), str(src), "-L", str(PKG), "-Wl,-rpath,$ORIGIN"]
     for d in ce.library_paths():
         cmd += ["-L", d, f"-Wl,-rpath,{d}"]
-    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch"]
+    cmd += [*link, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
+
+
+def _compile_ops(verbose: bool) -> None:
+    """The TORCH_LIBRARY operator library, linked to libqrb200.so."""
+    _compile_host(CSRC / "qrb_torch_op.cpp", OPS, verbose, [], ["-l:libqrb200.so"])
+
+
+def _compile_py(verbose: bool) -> None:
+    """The Python module of the layer operators, linked to the operator library."""
+    import sysconfig
+    _compile_host(CSRC / "qrb_py_layers.cpp", PY, verbose, ["-I", sysconfig.get_paths()["include"]],
+                  ["-l:libqrb200_torch_ops.so", "-ltorch_python"])
 
 
 # what each library is linked from: (source, definitions)
@@ -121,8 +133,10 @@ def build(force: bool = False, verbose: bool = False, extra=()) -> Path:
         objs = [_object(CSRC / name, defs) for name, defs in units]
         if force or not up_to_date(out, objs):
             _link(objs, out, verbose)
-    if force or not up_to_date(OPS, [CSRC / "qrb_torch_op.cpp", *INCLUDE.glob("*.h")]):
+    if force or not up_to_date(OPS, [CSRC / "qrb_torch_op.cpp", CSRC / "qrb_torch_layers.h", *INCLUDE.glob("*.h")]):
         _compile_ops(verbose)
+    if force or not up_to_date(PY, [CSRC / "qrb_py_layers.cpp", CSRC / "qrb_torch_layers.h", OPS]):
+        _compile_py(verbose)
     return LIB
 
 

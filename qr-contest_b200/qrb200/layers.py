@@ -25,7 +25,8 @@ _FP8 = torch.float8_e4m3fn
 
 
 class _Ops:
-    """The operators' handles, looked up once."""
+    """The operators' handles, looked up once; ``fast_*`` take plain CUDA tensors without the operator
+    registry and return NotImplemented for anything else."""
 
     loaded = False
 
@@ -38,6 +39,9 @@ class _Ops:
         cls.quantize_rows = ns.quantize_rows.default
         cls.linear = ns.linear.default
         cls.linear_backward = ns.linear_backward.default
+        from . import _layers
+        cls.fast_rms_norm = staticmethod(_layers.rms_norm)
+        cls.fast_linear = staticmethod(_layers.linear)
         cls.loaded = True
 
 
@@ -53,6 +57,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
     """
     if not _Ops.loaded:
         _Ops.load()
+    if not torch.compiler.is_compiling():
+        got = _Ops.fast_rms_norm(x, weight, residual, eps, out_dtype)
+        if got is not NotImplemented:
+            return got
     y, scale, h = _Ops.rms_norm(x, weight, residual, eps, out_dtype)
     if scale is None:
         return y if h is None else (y, h)
@@ -86,4 +94,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         act = _ACTIVATIONS[activation]
     except (KeyError, TypeError):
         raise ValueError(f"qrb200: unknown activation {activation!r}") from None
+    if not torch.compiler.is_compiling():
+        got = _Ops.fast_linear(x, weight, bias, residual, act, x_scale, weight_scale, out_dtype)
+        if got is not NotImplemented:
+            return got
     return _Ops.linear(x, weight, bias, residual, act, x_scale, weight_scale, out_dtype, False)[0]

@@ -477,3 +477,44 @@ def test_linear_gradient_special():
 def test_no_wait_ran_out():
     from qrb200 import _lib
     assert not _lib.layer_timed_out()
+
+
+def test_both_ways_in():
+    """The short way from Python and torch.ops are the same operator; what the short way does not take goes the other."""
+    from qrb200 import layers
+    x, w, r = rnd(7, 96, dtype=BF, seed=1), rnd(96, dtype=BF, seed=2), rnd(7, 96, dtype=BF, seed=3)
+    W = rnd(40, 96, dtype=BF, seed=4)
+    layers._Ops.loaded or layers._Ops.load()
+    y, _, h = torch.ops.qrb200.rms_norm(x, w, r, 1e-6, None)
+    a, b = q().rms_norm(x, w, residual=r)
+    assert torch.equal(a, y) and torch.equal(b, h)
+    assert torch.equal(q().linear(x, W, activation="silu"), torch.ops.qrb200.linear(x, W, None, None, 4, None, None, None, False)[0])
+    # eps as an int, a tensor subclass, a function mode, a transform: not the short way, the same result
+    one = q().rms_norm(x, w, eps=1.0)
+    assert torch.equal(q().rms_norm(x, w, eps=1), one)
+
+    class Sub(torch.Tensor):
+        pass
+    assert torch.equal(q().rms_norm(x.as_subclass(Sub), w, eps=1.0).as_subclass(torch.Tensor), one)
+
+    class Mode(torch.overrides.TorchFunctionMode):
+        seen = 0
+
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            Mode.seen += 1
+            return func(*args, **(kwargs or {}))
+    with Mode():
+        assert torch.equal(q().rms_norm(x, w, eps=1.0), one)
+    assert Mode.seen
+    with torch.inference_mode():
+        assert torch.equal(q().rms_norm(x, w, eps=1.0), one)
+    with torch.no_grad():
+        assert not q().linear(x.clone().requires_grad_(), W).requires_grad
+    for bad in (lambda: q().rms_norm(x.double()), lambda: q().linear(x, W, out_dtype=F32), lambda: q().rms_norm(x, r)):
+        with pytest.raises((TypeError, ValueError)):
+            bad()
+    p = torch.nn.Parameter(W)
+    y = q().linear(x, p)
+    assert y.requires_grad and torch.autograd.grad(y.sum(), p)[0].shape == W.shape
+    with pytest.raises(NotImplementedError):
+        torch.autograd.grad(q().linear(x, p).square().sum(), p, create_graph=True)
