@@ -214,6 +214,27 @@ __device__ __forceinline__ float row_absmax(uint32_t bits, uint32_t* slots) {
   }
   return __uint_as_float(bits);
 }
+// Sum and largest |v| of a row with one exchange.
+struct SumMax { float sum, absmax; };
+__device__ __forceinline__ SumMax row_sum_max(float v, uint32_t bits, uint2* slots) {
+  for (int o = min(blockDim.x, 32u) >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (blockDim.x < 32) {
+    for (int o = blockDim.x >> 1; o; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+  } else {
+    bits = __reduce_max_sync(0xffffffffu, bits);
+  }
+  if (blockDim.x > 32) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) slots[warp] = make_uint2(__float_as_uint(v), bits);
+    __syncthreads();
+    const uint2 s = lane < (int)(blockDim.x >> 5) ? slots[lane] : make_uint2(0, 0);
+    v = __uint_as_float(s.x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    bits = __reduce_max_sync(0xffffffffu, s.y);
+  }
+  return {v, __uint_as_float(bits)};
+}
 // The row's scale; a NaN stays (fmaxf would drop it).
 __device__ __forceinline__ float scale_of(float absmax) {
   const float s = absmax / kFp8Max;
@@ -260,7 +281,7 @@ struct Weight {
 template <typename TX, typename TH, bool RES, bool Q8, bool NORM, int VPT, int NT>
 __global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VPT)) fwd_kernel(FwdArgs a) {
   __shared__ float s_sum[32];
-  __shared__ uint32_t s_max[32];
+  __shared__ uint2 s_both[32];
   // rows past the end are computed again from the last row and not stored: no thread leaves early
   const int64_t at = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const bool live = at < a.rows;
@@ -290,17 +311,34 @@ __global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VP
     for (int i = 0; i < VPT; ++i) mine.template load<true>(static_cast<const TH*>(a.x) + row * a.ldx, i, h[i]);
   }
   float r = 1.f;
-  if (NORM) {
-    w.load(mine, a.w, a.w_f32);
+  if (NORM) w.load(mine, a.w, a.w_f32);
+  float absmax = 0.f;
+  if (NORM || Q8) {
+    // max |y| = r max |h w|, so the scale takes no reduction of its own after r is known
     float ss = 0.f;
+    uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      float v[8];
+      float v[8], u[8];
       unpack(h[i], v);
+      if (Q8 && NORM) w.get(mine, a.w, a.w_f32, i, u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+      for (int j = 0; j < 8; ++j) {
+        if (NORM) ss = fmaf(v[j], v[j], ss);
+        if (Q8) top = max(top, __float_as_uint(NORM ? v[j] * u[j] : v[j]) & 0x7FFFFFFFu);
+      }
     }
-    r = rsqrtf(row_sum(ss, s_sum) / a.dim + a.eps);
+    if (Q8) {
+      const SumMax s = row_sum_max(ss, top, s_both);
+      ss = s.sum;
+      absmax = s.absmax;
+    } else {
+      ss = row_sum(ss, s_sum);
+    }
+    if (NORM) {
+      r = rsqrtf(ss / a.dim + a.eps);
+      absmax *= r;
+    }
   }
   auto value = [&](int i, float (&v)[8]) {
     unpack(h[i], v);
@@ -312,15 +350,7 @@ __global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VP
     }
   };
   if (Q8) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      float v[8];
-      value(i, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-    }
-    const float s = scale_of(row_absmax(top, s_max));
+    const float s = scale_of(absmax);
     const float inv = 1.f / s;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
