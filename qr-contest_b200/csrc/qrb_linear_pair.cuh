@@ -6,7 +6,7 @@
 // CTAs' shared memory, so a byte of Q is fetched once per 256 rows instead of once per 128 and shared
 // memory holds twice the k.  Each CTA's tensor memory holds its 128 rows x TN float32 sums twice:
 // while 8 warps finish one tile (bias, activation, residual, rounding), the MMAs of the next run.
-// Roles: warps 0-7 epilogue, warp 8 loads, warp 9 (first CTA) MMAs.  Hand-offs are mbarriers:
+// Roles: warps 0-7 epilogue, warp 8 loads P, warp 10 loads Q, warp 9 (first CTA) MMAs.  Hand-offs are mbarriers:
 //   full[s]       loads of both CTAs -> MMA        (in the first CTA; bytes of both)
 //   empty[s]      MMA -> loads of both CTAs        (commit to both)
 //   acc_full[a]   MMA -> epilogues of both CTAs    (commit to both)
@@ -23,7 +23,7 @@
 namespace qrb {
 namespace lin {
 
-constexpr int kPairThreads = 320;
+constexpr int kPairThreads = 352;
 constexpr int kPairM = 256;  // tile rows of a pair
 
 struct PairMaps {
@@ -104,22 +104,6 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// A wait for what the other CTA of the pair may have written or signalled.
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t phase) {
-  for (unsigned i = 0; i < tc::kSpinLimit; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(tc::smem_u32(bar)), "r"(phase)
-        : "memory");
-    if (ok) return true;
-  }
-  return false;
-}
-
 // Address of 16-byte chunk q of row r in a staged block of 32 rows x 128 bytes.
 __device__ __forceinline__ char* staged(char* buf, int r, int q) { return buf + 128 * r + 16 * (q ^ (r & 7)); }
 
@@ -197,31 +181,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   };
 
   bool ok = true;
-  if (warp == 8) {
+  if (warp == 8 || warp == 10) {  // P's rows, Q's rows: a thread each, which has little time a block
     if (lane == 0) {
-      const int i_off = 128 * rank, j_off = TN / 2 * rank;
-      int it = 0;
+      const bool is_p = warp == 8, by_rows = ES == 2 && (is_p ? a.p_row : a.q_row);
+      const CUtensorMap* map = is_p ? &maps.p : &maps.q;
+      const uint32_t base = tc::smem_u32(sm) + (is_p ? 0 : C::P_BYTES), full0 = in_rank(tc::smem_u32(full), 0);
+      const int chunks = is_p ? 2 : TN / 128;
+      int s = 0, first = 1;
+      uint32_t phase = 0;  // of the wait for a slot's last use
       for (int t = pair; t < tiles && ok; t += pairs) {
         int ti, tj;
         place(t, ti, tj);
-        const int i0 = ti * kPairM + i_off, j0 = tj * TN + j_off;
-        for (int kb = 0; kb < nk; ++kb, ++it) {
-          const int s = it % C::STAGES, k0 = kb * BKE;
-          if (it >= C::STAGES && !wait_cluster(&empty[s], ((it / C::STAGES) - 1) & 1)) { ok = false; break; }
-          const uint32_t sp = tc::smem_u32(sm + s * C::STAGE), sq = sp + C::P_BYTES;
-          const uint32_t bar = in_rank(tc::smem_u32(&full[s]), 0);
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
-          if (ES == 2 && a.p_row) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) tma_load_2d_pair(sp + 8192 * c, &maps.p, i0 + 64 * c, k0, bar);
+        const int r0 = is_p ? ti * kPairM + 128 * (int)rank : tj * TN + TN / 2 * (int)rank;
+        for (int kb = 0, k0 = 0; kb < nk; ++kb, k0 += BKE) {
+          if (!first && !tc::mbar_wait(&empty[s], phase)) { ok = false; break; }
+          if (is_p && rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
+          const uint32_t to = base + s * C::STAGE, bar = full0 + 8 * s;
+          if (by_rows) {
+            for (int c = 0; c < chunks; ++c) tma_load_2d_pair(to + 8192 * c, map, r0 + 64 * c, k0, bar);
           } else {
-            tma_load_2d_pair(sp, &maps.p, k0, i0, bar);
+            tma_load_2d_pair(to, map, k0, r0, bar);
           }
-          if (ES == 2 && a.q_row) {
-#pragma unroll
-            for (int c = 0; c < TN / 128; ++c) tma_load_2d_pair(sq + 8192 * c, &maps.q, j0 + 64 * c, k0, bar);
-          } else {
-            tma_load_2d_pair(sq, &maps.q, k0, j0, bar);
+          if (++s == C::STAGES) {
+            s = 0;
+            if (first) first = 0;
+            else phase ^= 1;
           }
         }
       }
@@ -231,21 +215,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   } else if (warp == 9) {
     if (lane == 0 && rank == 0) {
       const uint32_t pstep = (a.p_row ? 2048 : 32) >> 4, qstep = (a.q_row ? 2048 : 32) >> 4;
-      int it = 0, turn = 0;
+      const uint64_t p0 = operand_desc(tc::smem_u32(sm), a.p_row), q0 = operand_desc(tc::smem_u32(sm) + C::P_BYTES, a.q_row);
+      int s = 0, turn = 0;
+      uint32_t phase = 0;
       for (int t = pair; t < tiles && ok; t += pairs, ++turn) {
         const int b = turn & 1;
-        if (turn >= 2 && !wait_cluster(&acc_empty[b], ((turn >> 1) - 1) & 1)) { ok = false; break; }
+        if (turn >= 2 && !tc::mbar_wait(&acc_empty[b], ((turn >> 1) - 1) & 1)) { ok = false; break; }
         tc::tc_fence_after();
-        for (int kb = 0; kb < nk; ++kb, ++it) {
-          const int s = it % C::STAGES;
-          if (!wait_cluster(&full[s], (it / C::STAGES) & 1)) { ok = false; break; }
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!tc::mbar_wait(&full[s], phase)) { ok = false; break; }
           tc::tc_fence_after();
-          const uint32_t sp = tc::smem_u32(sm + s * C::STAGE), sq = sp + C::P_BYTES;
-          uint64_t dp = operand_desc(sp, a.p_row), dq = operand_desc(sq, a.q_row);
+          uint64_t dp = p0 + (uint64_t)(s * (C::STAGE >> 4)), dq = q0 + (uint64_t)(s * (C::STAGE >> 4));
 #pragma unroll
           for (int c = 0; c < 4; ++c, dp += pstep, dq += qstep)
             mma_pair<ES>(tmem + b * TN, dp, dq, a.idesc, (kb | c) ? 1u : 0u);
           commit_pair(&empty[s]);
+          if (++s == C::STAGES) {
+            s = 0;
+            phase ^= 1;
+          }
         }
         if (ok) commit_pair(&acc_full[b]);
       }
@@ -296,7 +284,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           cscale[h] = ES == 1 && e.col_scale && j < a.n ? e.col_scale[j] : 1.f;
         }
         if (!waited) {
-          if (ok && !wait_cluster(&acc_full[b], (turn >> 1) & 1)) ok = false;
+          if (ok && !tc::mbar_wait(&acc_full[b], (turn >> 1) & 1)) ok = false;
           tc::tc_fence_after();
           waited = true;
         }
