@@ -286,7 +286,8 @@ int launch_tile_t(int T, const lin::Maps& maps, const lin::Args& a, cudaStream_t
     case 16: return launch_tile<Out, ES, 16, SLOPE>(maps, a, st);
     case 32: return launch_tile<Out, ES, 32, SLOPE>(maps, a, st);
     case 64: return launch_tile<Out, ES, 64, SLOPE>(maps, a, st);
-    default: return launch_tile<Out, ES, 128, SLOPE>(maps, a, st);
+    case 128: return launch_tile<Out, ES, 128, SLOPE>(maps, a, st);
+    default: return QRB200_ERR_INVALID_ARG;  // the maps' boxes are made for T
   }
 }
 

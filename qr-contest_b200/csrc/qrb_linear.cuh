@@ -289,12 +289,12 @@ __device__ __forceinline__ void put4(void* p, uint2 packed, bool vec, int left) 
 // Q's rows are the MMA's 128 rows, P's the T columns, so few tokens cost a narrow MMA and not a
 // padded one; the CTAs of a cluster take equal parts of k, leave their float32 sums in shared
 // memory, and each finishes T / splits of the tile's rows with its peers' sums read over the
-// cluster, added in rank order.  Roles: warps 0-7 epilogue, warp 8 loads, warp 9 MMAs.  The loads
+// cluster, added in rank order.  Roles: warps 0-7 epilogue, warps 8 and 10 loads, warp 9 MMAs.  The loads
 // start before anything else is set up, and the epilogue warps fetch bias and scales (and the
 // residual, as far as the L2 cache) while the sums are made: these calls are short, and each wait
 // for memory would show.  So would the time to fetch instructions that run once (with 16 rows
 // unrolled, finishing a tile took 16 us): loops stay loops, and there are no divisions.
-constexpr int kTileThreads = 320;
+constexpr int kTileThreads = 352;
 constexpr int kTileQ = 128;
 
 // RINGS = 2: half an SM's shared memory, two CTAs an SM; 1: all of it, for grids of one CTA an SM.
@@ -324,21 +324,26 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
   const int kb = rank * a.part, nk = max(0, min(a.part, (a.k + BKE - 1) / BKE - kb));
   const Epilogue& e = a.e;
 
-  auto load = [&](int t) {  // block t of this CTA's k into its ring slot
-    const int s = t % C::STAGES, k0 = (kb + t) * BKE;
-    const uint32_t pq = tc::smem_u32(sm + s * C::STAGE), pp = pq + C::Q_BYTES;
+  // block t of this CTA's k into ring slot s: Q's rows (which also announces the bytes of both), P's
+  auto load_q = [&](int t, int s) {
+    const uint32_t to = tc::smem_u32(sm + s * C::STAGE);
+    const int k0 = (kb + t) * BKE;
     mbar_expect_tx(&full[s], C::STAGE);
     if (ES == 2 && a.q_row) {
 #pragma unroll
-      for (int c = 0; c < kTileQ / 64; ++c) tma_load_2d(pq + 8192 * c, &maps.q, j0 + 64 * c, k0, &full[s]);
+      for (int c = 0; c < kTileQ / 64; ++c) tma_load_2d(to + 8192 * c, &maps.q, j0 + 64 * c, k0, &full[s]);
     } else {
-      tma_load_2d(pq, &maps.q, k0, j0, &full[s]);
+      tma_load_2d(to, &maps.q, k0, j0, &full[s]);
     }
+  };
+  auto load_p = [&](int t, int s) {
+    const uint32_t to = tc::smem_u32(sm + s * C::STAGE) + C::Q_BYTES;
+    const int k0 = (kb + t) * BKE;
     if (ES == 2 && T >= 64 && a.p_row) {
 #pragma unroll
-      for (int c = 0; c < T / 64; ++c) tma_load_2d(pp + 8192 * c, &maps.p, i0 + 64 * c, k0, &full[s]);
+      for (int c = 0; c < T / 64; ++c) tma_load_2d(to + 8192 * c, &maps.p, i0 + 64 * c, k0, &full[s]);
     } else {
-      tma_load_2d(pp, &maps.p, k0, i0, &full[s]);
+      tma_load_2d(to, &maps.p, k0, i0, &full[s]);
     }
   };
   if (warp == 8 && lane == 0) {
@@ -349,7 +354,10 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
     tc::mbar_init(&done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tc::fence_async_smem();
-    for (int t = 0; t < nk && t < C::STAGES; ++t) load(t);
+    for (int t = 0; t < nk && t < C::STAGES; ++t) {
+      load_q(t, t);
+      load_p(t, t);
+    }
   } else if (warp == 9) {
     tc::tmem_alloc(&tslot, C::TMEM);
     tc::tmem_relinquish();
@@ -363,30 +371,44 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
   const int per = T / S, j = j0 + 4 * lane, left = a.n - j;
   float* acc = reinterpret_cast<float*>(sm);  // [T][128]; the ring is free when the sums are there
   float bias[4] = {}, cscale[4] = {1.f, 1.f, 1.f, 1.f};
-  if (warp == 8) {
+  if (warp == 8 || warp == 10) {
     if (lane == 0) {
       bool ok = true;
+      int s = 0;
+      uint32_t phase = 0;  // of the wait for the slot's last use
       for (int t = C::STAGES; t < nk && ok; ++t) {
-        ok = tc::mbar_wait(&empty[t % C::STAGES], ((t / C::STAGES) - 1) & 1);
-        if (ok) load(t);
+        ok = tc::mbar_wait(&empty[s], phase);
+        if (ok) {
+          if (warp == 8) load_q(t, s);
+          else load_p(t, s);
+        }
+        if (++s == C::STAGES) {
+          s = 0;
+          phase ^= 1;
+        }
       }
       if (!ok) give_up();
     }
   } else if (warp == 9) {
     if (lane == 0) {
       const uint32_t qstep = (a.q_row ? 2048 : 32) >> 4, pstep = (a.p_row ? 2048 : 32) >> 4;
+      const uint64_t q0 = operand_desc(tc::smem_u32(sm), a.q_row), p0 = operand_desc(tc::smem_u32(sm) + C::Q_BYTES, a.p_row);
       bool ok = true;
+      int s = 0;
+      uint32_t phase = 0;
       for (int t = 0; t < nk; ++t) {
-        const int s = t % C::STAGES;
-        ok = tc::mbar_wait(&full[s], (t / C::STAGES) & 1);
+        ok = tc::mbar_wait(&full[s], phase);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint32_t pq = tc::smem_u32(sm + s * C::STAGE), pp = pq + C::Q_BYTES;
-        uint64_t dq = operand_desc(pq, a.q_row), dp = operand_desc(pp, a.p_row);
+        uint64_t dq = q0 + (uint64_t)(s * (C::STAGE >> 4)), dp = p0 + (uint64_t)(s * (C::STAGE >> 4));
 #pragma unroll
         for (int c = 0; c < 4; ++c, dq += qstep, dp += pstep)
           mma<ES>(tmem, dq, dp, a.idesc, (t | c) ? 1u : 0u);
         tc::mma_commit(&empty[s]);
+        if (++s == C::STAGES) {
+          s = 0;
+          phase ^= 1;
+        }
       }
       if (ok && nk > 0) tc::mma_commit(&done);
       if (!ok) give_up();
