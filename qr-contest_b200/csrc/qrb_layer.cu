@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <utility>
 
 namespace qrb {
 namespace {
@@ -21,9 +22,18 @@ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // Rows of this base and stride (elements) all start on 16 bytes.
 bool rows_on16(const void* p, int64_t ld, int es) { return on16(p) && (ld * es & 15) == 0; }
 
-int launched() {
+// Launches one kernel (see qrb_pdl.cuh) and counts it.
+template <typename... P, typename... A>
+int launch_cluster(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, unsigned cluster, A&&... args) {
+  const cudaError_t e = launch_overlapped(kernel, grid, block, smem, st, cluster, std::forward<A>(args)...);
   count_launches(1);
-  return note(cudaGetLastError()) == cudaSuccess ? QRB200_OK : QRB200_ERR_CUDA;
+  if (note(e) == cudaSuccess) return QRB200_OK;
+  cudaGetLastError();  // not left for a later call to find
+  return QRB200_ERR_CUDA;
+}
+template <typename... P, typename... A>
+int launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
+  return launch_cluster(kernel, grid, block, smem, st, 0, std::forward<A>(args)...);
 }
 
 // Lets a kernel use `bytes` of dynamic shared memory, once per device (`ready`: the devices done).
@@ -90,26 +100,21 @@ template <typename TX, typename TH, bool RES, bool Q8, bool NORM>
 int launch_fwd(const norm::FwdArgs& a, bool vec, cudaStream_t st) {
   constexpr bool wide = sizeof(TX) == 4 || sizeof(TH) == 4;
   if (a.dim > norm::kRegDim) {
-    norm::fwd_long_kernel<TX, TH, Q8, NORM><<<(unsigned)a.rows, norm::kMaxThreads, 0, st>>>(a);
-    return launched();
+    return launch(norm::fwd_long_kernel<TX, TH, Q8, NORM>, (unsigned)a.rows, norm::kMaxThreads, 0, st, a);
   }
   const Shape s = norm_shape(a.rows, a.dim, wide, vec);
   const dim3 block(s.nt, s.rows);
   const unsigned grid = (unsigned)((a.rows + s.rows - 1) / s.rows);
-#define QRB_FWD(V, NT) norm::fwd_kernel<TX, TH, RES, Q8, NORM, V, NT><<<grid, block, 0, st>>>(a)
+#define QRB_FWD(V, NT) launch(norm::fwd_kernel<TX, TH, RES, Q8, NORM, V, NT>, grid, block, 0, st, a)
   if (vec) {
-    if (s.vpt == 1) QRB_FWD(1, 0);
-    else if (s.vpt == 2) QRB_FWD(2, 0);
-    else if constexpr (!wide) QRB_FWD(4, 0);
-  } else if (s.nt == 32) {
-    if (s.vpt == 1) QRB_FWD(1, 32); else if (s.vpt == 2) QRB_FWD(2, 32); else QRB_FWD(4, 32);
-  } else if (s.nt == 256) {
-    if (s.vpt == 1) QRB_FWD(1, 256); else if (s.vpt == 2) QRB_FWD(2, 256); else QRB_FWD(4, 256);
-  } else {
-    QRB_FWD(4, 512);
+    if (s.vpt == 1) return QRB_FWD(1, 0);
+    if (s.vpt == 2 || wide) return QRB_FWD(2, 0);
+    if constexpr (!wide) return QRB_FWD(4, 0);
   }
+  if (s.nt == 32) return s.vpt == 1 ? QRB_FWD(1, 32) : s.vpt == 2 ? QRB_FWD(2, 32) : QRB_FWD(4, 32);
+  if (s.nt == 256) return s.vpt == 1 ? QRB_FWD(1, 256) : s.vpt == 2 ? QRB_FWD(2, 256) : QRB_FWD(4, 256);
+  return QRB_FWD(4, 512);
 #undef QRB_FWD
-  return launched();
 }
 
 template <typename TX>
@@ -158,8 +163,7 @@ int launch_bwd_as(const norm::BwdArgs& a, const BwdPlan& p, cudaStream_t st) {
   auto kernel = norm::bwd_kernel<TX, TH, TW, VPT, NT>;
   static std::atomic<uint64_t> ready{0};
   if (const int rc = raise_smem(reinterpret_cast<const void*>(kernel), kBwdRing, ready)) return rc;
-  kernel<<<(unsigned)p.grid, dim3(p.s.nt, p.s.rows), p.smem, st>>>(a, p.depth);
-  return launched();
+  return launch(kernel, (unsigned)p.grid, dim3(p.s.nt, p.s.rows), p.smem, st, a, p.depth);
 }
 template <typename TX, typename TH, typename TW>
 int launch_bwd_w(const norm::BwdArgs& a, bool vec, const BwdPlan& p, cudaStream_t st) {
@@ -173,8 +177,7 @@ int launch_bwd_w(const norm::BwdArgs& a, bool vec, const BwdPlan& p, cudaStream_
 template <typename TX, typename TH>
 int launch_bwd(const norm::BwdArgs& a, bool vec, const BwdPlan& p, cudaStream_t st) {
   if (a.dim > norm::kRegDim) {
-    norm::bwd_long_kernel<TX, TH><<<(unsigned)p.grid, norm::kMaxThreads, 0, st>>>(a);
-    return launched();
+    return launch(norm::bwd_long_kernel<TX, TH>, (unsigned)p.grid, norm::kMaxThreads, 0, st, a);
   }
   if constexpr (sizeof(TX) == 2) {
     if (a.w && a.w_f32) return launch_bwd_w<TX, TH, float>(a, vec, p, st);
@@ -184,8 +187,7 @@ int launch_bwd(const norm::BwdArgs& a, bool vec, const BwdPlan& p, cudaStream_t 
 
 template <typename T>
 int launch_colsum(const float* part, int64_t parts, int64_t cols, void* out, cudaStream_t st) {
-  norm::colsum_kernel<T><<<(unsigned)((cols + 31) / 32), dim3(32, 32), 0, st>>>(part, parts, cols, static_cast<T*>(out));
-  return launched();
+  return launch(norm::colsum_kernel<T>, (unsigned)((cols + 31) / 32), dim3(32, 32), 0, st, part, parts, cols, static_cast<T*>(out));
 }
 int colsum(const float* part, int64_t parts, int64_t cols, void* out, int32_t dtype, cudaStream_t st) {
   if (dtype == QRB200_F32) return launch_colsum<float>(part, parts, cols, out, st);
@@ -228,9 +230,8 @@ struct Aligner {
   int run(cudaStream_t st) const {
     if (!count) return QRB200_OK;
     const dim3 grid((unsigned)std::min<int64_t>((most + 255) / 256, kSMs * 8), (unsigned)count);
-    if (es == 2) lin::align_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(jobs);
-    else lin::align_rows_kernel<uint8_t><<<grid, 256, 0, st>>>(jobs);
-    return launched();
+    return es == 2 ? launch(lin::align_rows_kernel<uint16_t>, grid, 256, 0, st, jobs)
+                   : launch(lin::align_rows_kernel<uint8_t>, grid, 256, 0, st, jobs);
   }
 };
 
@@ -255,24 +256,8 @@ int launch_tile_as(const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
   using C = lin::TileCfg<T, RINGS>;
   static std::atomic<uint64_t> ready{0};
   if (const int rc = raise_smem(reinterpret_cast<const void*>(kernel), C::SMEM, ready)) return rc;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)a.splits, (unsigned)((a.n + 127) / 128), (unsigned)((a.m + T - 1) / T));
-  cfg.blockDim = dim3(lin::kTileThreads);
-  cfg.dynamicSmemBytes = C::SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)a.splits;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps, a);
-  count_launches(1);
-  if (note(e) != cudaSuccess) {
-    cudaGetLastError();
-    return QRB200_ERR_CUDA;
-  }
-  return QRB200_OK;
+  const dim3 grid((unsigned)a.splits, (unsigned)((a.n + 127) / 128), (unsigned)((a.m + T - 1) / T));
+  return launch_cluster(kernel, grid, lin::kTileThreads, C::SMEM, st, (unsigned)a.splits, maps, a);
 }
 template <typename Out, int ES, int T, bool SLOPE>
 int launch_tile(const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
@@ -332,8 +317,7 @@ int launch_pair(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_
   }
   const int64_t tiles = (int64_t)a.tiles_i * a.tiles_j;
   const unsigned grid = 2 * (unsigned)std::min<int64_t>(tiles, kSMs / 2);
-  kernel<<<grid, lin::kPairThreads, C::SMEM, st>>>(maps, a);
-  return launched();
+  return launch(kernel, grid, lin::kPairThreads, C::SMEM, st, maps, a);
 }
 
 template <int TN>
@@ -359,10 +343,9 @@ int product_pair(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64
 bool few_tokens(int64_t m, int64_t n, int64_t k) { return m <= 2 || (m <= 4 && n * k <= 1 << 22); }
 template <typename Out, typename In, int M, bool VEC>
 int launch_token(const lin::TokenArgs& a, cudaStream_t st) {
-  if (a.n >= 8192) lin::token_kernel<Out, In, M, 2, 1, VEC><<<(a.n + 7) / 8, 128, 0, st>>>(a);
-  else if ((int64_t)a.k * sizeof(In) >= 4 * (int64_t)a.n) lin::token_kernel<Out, In, M, 1, 8, VEC><<<a.n, 256, 0, st>>>(a);
-  else lin::token_kernel<Out, In, M, 1, 1, VEC><<<(a.n + 3) / 4, 128, 0, st>>>(a);
-  return launched();
+  if (a.n >= 8192) return launch(lin::token_kernel<Out, In, M, 2, 1, VEC>, (a.n + 7) / 8, 128, 0, st, a);
+  if ((int64_t)a.k * sizeof(In) >= 4 * (int64_t)a.n) return launch(lin::token_kernel<Out, In, M, 1, 8, VEC>, a.n, 256, 0, st, a);
+  return launch(lin::token_kernel<Out, In, M, 1, 1, VEC>, (a.n + 3) / 4, 128, 0, st, a);
 }
 template <typename Out, typename In>
 int product_token(const lin::TokenArgs& a, cudaStream_t st) {
@@ -465,9 +448,8 @@ int launch_dz(const void* dy, int64_t lddy, const uint16_t* slope, void* dz, int
               int64_t n, int64_t parts, cudaStream_t st) {
   const bool vec = n % 8 == 0 && rows_on16(dy, lddy, 2) && (!slope || on16(slope)) && (!dz || on16(dz));
   const dim3 grid((unsigned)((n + 255) / 256), (unsigned)parts);
-  if (vec) lin::dz_kernel<T, true><<<grid, 256, 0, st>>>(static_cast<const T*>(dy), lddy, slope, static_cast<T*>(dz), lddz, part, m, n);
-  else lin::dz_kernel<T, false><<<grid, 256, 0, st>>>(static_cast<const T*>(dy), lddy, slope, static_cast<T*>(dz), lddz, part, m, n);
-  return launched();
+  return launch(vec ? lin::dz_kernel<T, true> : lin::dz_kernel<T, false>, grid, 256, 0, st, static_cast<const T*>(dy), lddy,
+                slope, static_cast<T*>(dz), lddz, part, m, n);
 }
 
 struct BackwardPlan {

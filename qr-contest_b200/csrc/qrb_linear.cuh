@@ -18,6 +18,7 @@
 #include <cuda_fp8.h>
 
 #include "qrb_f2.cuh"
+#include "qrb_pdl.cuh"
 #include "qrb_tc.cuh"
 #include "qrb_tmap.cuh"
 
@@ -313,6 +314,7 @@ template <typename Out, int ES, int T, bool SLOPE, int RINGS>
 __global__ void __launch_bounds__(kTileThreads, RINGS)
     tile_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a) {
   using C = TileCfg<T, RINGS>;
+  allow_next();
   extern __shared__ char smraw[];
   char* sm = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[C::STAGES], empty[C::STAGES], done;
@@ -354,6 +356,7 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
     tc::mbar_init(&done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tc::fence_async_smem();
+    after_previous();
     for (int t = 0; t < nk && t < C::STAGES; ++t) {
       load_q(t, t);
       load_p(t, t);
@@ -366,6 +369,7 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tslot;
+  after_previous();
 
   // the tile's rows that this CTA finishes, two per warp at a time
   const int per = T / S, j = j0 + 4 * lane, left = a.n - j;
@@ -574,6 +578,8 @@ struct TokenArgs {
 
 template <typename Out, typename In, int M, int R, int SPLIT, bool VEC>
 __global__ void __launch_bounds__(256) token_kernel(TokenArgs a) {
+  allow_next();
+  after_previous();
   __shared__ float s_part[SPLIT == 1 ? 1 : 8][M * R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = SPLIT == 1 ? 0 : warp;
@@ -683,6 +689,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     dz_kernel(const T* dy, int64_t lddy, const uint16_t* slope, T* dz, int64_t lddz, float* part,
               int64_t m, int64_t n) {
+  allow_next();
+  after_previous();
   __shared__ float s[8][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t j0 = (int64_t)blockIdx.x * 256;
@@ -744,6 +752,8 @@ struct AlignJobs {
 };
 template <typename T>
 __global__ void __launch_bounds__(256) align_rows_kernel(AlignJobs jobs) {
+  allow_next();
+  after_previous();
   constexpr int V = 16 / sizeof(T);
   const auto& o = jobs.job[blockIdx.y];
   const T* src = static_cast<const T*>(o.src);

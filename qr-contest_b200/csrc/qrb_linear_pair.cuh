@@ -135,6 +135,7 @@ template <typename Out, int ES, int TN, bool SLOPE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ PairArgs a) {
   using C = PairCfg<TN>;
+  allow_next();
   extern __shared__ __align__(1024) char sm[];
   char* staging = sm + C::STAGES * C::STAGE;
   float(*s_col)[2][32] = reinterpret_cast<float(*)[2][32]>(staging + C::STAGING);
@@ -170,6 +171,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_wait();
   tc::tc_fence_after();
   const uint32_t tmem = *tslot;
+  after_previous();
 
   // tile t of the order: groups of `group` tiles along i, all j of a group before the next one, so
   // that the pairs at work at one time share their rows of P and of Q in the L2 cache

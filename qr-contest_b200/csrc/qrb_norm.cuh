@@ -21,6 +21,7 @@
 
 #include "qrb_common.cuh"
 #include "qrb_f2.cuh"
+#include "qrb_pdl.cuh"
 
 namespace qrb {
 namespace norm {
@@ -280,6 +281,8 @@ struct Weight {
 // TH is the type that the norm reads: the stream's with a residual, else x's.
 template <typename TX, typename TH, bool RES, bool Q8, bool NORM, int VPT, int NT>
 __global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VPT)) fwd_kernel(FwdArgs a) {
+  allow_next();
+  after_previous();
   __shared__ float s_sum[32];
   __shared__ uint2 s_both[32];
   // rows past the end are computed again from the last row and not stored: no thread leaves early
@@ -375,6 +378,8 @@ __global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VP
 // where this thread has just written it).
 template <typename TX, typename TR, bool Q8, bool NORM>
 __global__ void __launch_bounds__(kMaxThreads) fwd_long_kernel(FwdArgs a) {
+  allow_next();
+  after_previous();
   __shared__ float s_sum[32];
   __shared__ uint32_t s_max[32];
   const int64_t row = blockIdx.x;
@@ -454,6 +459,8 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 template <typename TX, typename TH, typename TW, int VPT, int NT>
 __global__ void __launch_bounds__(NT == 32 ? 128 : NT == 256 ? 256 : 512, NT == 32 ? 8 : NT == 256 ? 4 : 1)
     bwd_kernel(BwdArgs a, int depth) {
+  allow_next();
+  after_previous();
   constexpr bool VEC = NT == 0;
   extern __shared__ __align__(16) char ring[];
   __shared__ float2 s_sum[2][32];
@@ -634,6 +641,8 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT == 256 ? 256 : 512, NT == 
 // Rows too long for registers; the partial weight gradients are added up in memory.
 template <typename TX, typename TR>
 __global__ void __launch_bounds__(kMaxThreads) bwd_long_kernel(BwdArgs a) {
+  allow_next();
+  after_previous();
   __shared__ float2 s_sum[2][32];
   const float* wf = a.w && a.w_f32 ? static_cast<const float*>(a.w) : nullptr;
   const TX* wx = a.w && !a.w_f32 ? static_cast<const TX*>(a.w) : nullptr;
@@ -667,6 +676,8 @@ __global__ void __launch_bounds__(kMaxThreads) bwd_long_kernel(BwdArgs a) {
 // threads that each add every 32nd part, then a tree.
 template <typename T>
 __global__ void __launch_bounds__(1024) colsum_kernel(const float* part, int64_t parts, int64_t cols, T* out) {
+  allow_next();
+  after_previous();
   __shared__ float s[32][33];
   const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
   float v = 0.f;
