@@ -14,10 +14,11 @@ namespace qrb {
 __device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Launches a kernel that way; cluster: blocks of a cluster along x (0: as the kernel says).
+// Launches a kernel that way (early) or when all before it is done; cluster: blocks of a cluster along
+// x (0: as the kernel says).
 template <typename... P, typename... A>
-inline cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                                     unsigned cluster, A&&... args) {
+inline cudaError_t launch_kernel(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                                 unsigned cluster, bool early, A&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -25,7 +26,7 @@ inline cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[0].val.programmaticStreamSerializationAllowed = early;
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = cluster;
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
