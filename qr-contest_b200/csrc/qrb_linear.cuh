@@ -294,7 +294,9 @@ __device__ __forceinline__ void put4(void* p, uint2 packed, bool vec, int left) 
 // start before anything else is set up, and the epilogue warps fetch bias and scales (and the
 // residual, as far as the L2 cache) while the sums are made: these calls are short, and each wait
 // for memory would show.  So would the time to fetch instructions that run once (with 16 rows
-// unrolled, finishing a tile took 16 us): loops stay loops, and there are no divisions.
+// unrolled, finishing a tile took 16 us): loops stay loops, and there are no divisions.  Bound by the
+// rate at which an SM fetches its operands, and when short by set-up, exchange and epilogue, about
+// 4 us: 16 x 8192 x 8192 in 8 bits 14.8 us (4.6 TB/s), 128 x 4096 x 4096 bf16 13.2 us.
 constexpr int kTileThreads = 352;
 constexpr int kTileQ = 128;
 
@@ -525,7 +527,8 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
 // memory, no set-up.  A warp reads 512 bytes of each of its R rows of W at a time (32 lanes x 16
 // bytes; single elements where rows start off 16 bytes), the same part of the M tokens from the L1
 // cache, and adds the products in float32; SPLIT warps share a feature's k where there are too few
-// features to fill the GPU.  One lane per (token, feature) finishes it.
+// features to fill the GPU.  One lane per (token, feature) finishes it.  Measured, bf16: 1 x 8192 x 8192
+// 23.7 us (5.7 TB/s), 1 x 4096 x 4096 8.8 us, 1 x 512 x 512 2.0 us (tiles: 10.5, 4.4 for the last two).
 template <typename T> struct Chunk;  // 16 bytes of an operand as float
 template <> struct Chunk<__nv_bfloat16> {
   static constexpr int N = 8;
@@ -684,7 +687,7 @@ __global__ void __launch_bounds__(256) token_kernel(TokenArgs a) {
 // ---- dz = dy act'(z), and the column sums of dz (the bias' gradient) ----
 // Bound by memory: dy and the slope are read once, dz is written once; 8 columns a thread, 256 a
 // block, a block takes every gridDim.y-th group of 8 rows.  The sums are of the float32 values,
-// before dz is rounded to the operands' type for the two products.
+// before dz is rounded to the operands' type for the two products.  8192 x 8192 bf16: 57 us for 402 MB.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     dz_kernel(const T* dy, int64_t lddy, const uint16_t* slope, T* dz, int64_t lddz, float* part,
