@@ -287,6 +287,7 @@ __global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VP
   after_previous();
   __shared__ float s_sum[32];
   __shared__ uint2 s_both[32];
+  __shared__ uint32_t s_max[32];
   // rows past the end are computed again from the last row and not stored: no thread leaves early
   const int64_t at = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const bool live = at < a.rows;
@@ -355,6 +356,19 @@ __global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VP
     }
   };
   if (Q8) {
+    if (NORM && __any_sync(0xffffffffu, !(absmax <= 3.402823466e38f))) {
+      // h w may have left float32's range where y does not: the same question of y itself (the whole
+      // row agrees on it)
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float v[8];
+        value(i, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+      }
+      absmax = row_absmax(top, s_max);
+    }
     const float s = scale_of(absmax);
     const float inv = 1.f / s;
 #pragma unroll

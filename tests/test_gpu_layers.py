@@ -114,6 +114,17 @@ def test_norm_special_rows():
     # the rows beside them are not touched, and a masked-out row of the lowest value is a row like others
     low = torch.full((2, 64), torch.finfo(BF).min, dtype=BF, device="cuda")
     assert not bool(q().rms_norm(low).any())  # its square overflows: r = 0
+    # in 8 bits too, where h w would overflow float32 but y = (h r) w does not; beside ordinary rows
+    for rows, dim, w in ((2, 64, 2.0), (700, 72, 2.0), (3, 4096, 3.0), (400, 2047, 2.0), (2, 20000, 2.0)):
+        low = rnd(rows, dim, dtype=BF, seed=12)
+        low[::2] = torch.finfo(BF).min
+        q8, s8 = q().rms_norm(low, torch.full((dim,), w, dtype=BF, device="cuda"), out_dtype=FP8)
+        assert not bool(q8[::2].float().any()) and bool((s8[::2] == 2.0 ** -126).all())
+        check_norm(low[1::2], torch.full((dim,), w, dtype=BF, device="cuda"), None, fp8=True)
+    big = torch.full((4, 256), 1e-3, device="cuda")
+    w = torch.full((256,), 3e38, device="cuda")
+    q8, s8 = q().rms_norm(big, w, eps=0.0, out_dtype=FP8)
+    assert bool((q8.float() == 448).all()) and bool(((s8 - 3e38 / 448).abs() <= 2e33).all())
     # an in-place stream
     from qrb200 import _lib
     a, r = rnd(4, 64, dtype=BF, seed=8), rnd(4, 64, dtype=BF, seed=9)
@@ -518,3 +529,78 @@ def test_both_ways_in():
     assert y.requires_grad and torch.autograd.grad(y.sum(), p)[0].shape == W.shape
     with pytest.raises(NotImplementedError):
         torch.autograd.grad(q().linear(x, p).square().sum(), p, create_graph=True)
+
+
+def test_offsets_past_32_bits():
+    """Rows whose offsets pass 2^31 elements (and 2^32 bytes)."""
+    rows, ld = 33000, 66048
+    wide = torch.empty(rows, ld, dtype=BF, device="cuda")  # 4.4 GB, of which the views below are filled
+    last = slice(rows - 40, rows)
+    for c in (0, 65000, 65001):
+        x = wide[:, c:c + 136]
+        x.copy_(rnd(rows, 136, dtype=BF, seed=1))
+        w, W = rnd(136, dtype=BF, seed=2), rnd(264, 136, dtype=BF, seed=3)
+        y, h = q().rms_norm(x, w, residual=x)
+        y1, h1 = q().rms_norm(x[last].clone(), w, residual=x[last].clone())
+        assert torch.equal(y[last], y1) and torch.equal(h[last], h1)
+        z = q().linear(x, W, activation="gelu", residual=wide[:, :264] if c else None)
+        if not c:
+            check_linear(x[last].clone(), W, act="gelu")
+            want = q().linear(x.contiguous(), W, activation="gelu")
+        else:
+            want = q().linear(x.contiguous(), W, activation="gelu", residual=wide[:, :264].contiguous())
+        assert torch.equal(z, want)
+        t = q().linear(x[rows - 1], W)
+        check_linear(x[rows - 1].clone(), W)
+        assert torch.equal(t, q().linear(x[rows - 1].clone(), W))
+        wide[:, :264].copy_(rnd(rows, 264, dtype=BF, seed=4))
+
+
+@pytest.mark.parametrize("m,n", [(1, 4096), (40, 520), (40, 519), (2100, 2056), (2100, 2049)])
+def test_linear_in_place_residual(m, n):
+    """y over its own residual, through the C ABI, in each kernel and with rows off 16 bytes."""
+    from qrb200 import _lib
+    x, w, r = rnd(m, 256, dtype=BF, seed=1), rnd(n, 256, dtype=BF, seed=2), rnd(m, n, dtype=BF, seed=3)
+    want = q().linear(x, w, activation="silu", residual=r)
+    rc = _lib.lib().qrb200_linear(x.data_ptr(), 256, w.data_ptr(), 256, 0, None, None, None, r.data_ptr(), n, r.data_ptr(), n, None,
+                                  m, n, 256, _lib.QRB200_BF16, _lib.QRB200_BF16, _lib.ACT_SILU, None, 0,
+                                  torch.cuda.current_stream().cuda_stream)
+    assert rc == _lib.QRB200_OK and torch.equal(r, want)
+
+
+@pytest.mark.parametrize("m", [1, 3, 40, 300])
+def test_linear_8bit_nan(m):
+    x8, xs = q().quantize_rows(rnd(m, 96, seed=1))
+    w8, ws = q().quantize_rows(rnd(72, 96, seed=2))
+    x8.view(torch.uint8)[m // 2, 5] = 0x7F  # e4m3's NaN
+    y = q().linear(x8, w8, x_scale=xs, weight_scale=ws)
+    rows = torch.isnan(y).all(-1)
+    assert bool(rows[m // 2]) and int(rows.sum()) == 1 and int(torch.isnan(y).any(-1).sum()) == 1
+
+
+def test_chain_is_ordered():
+    """Kernels that start before the ones ahead of them have ended still see what those wrote: a chain that is
+    long and short by turns, against the same chain with a wait after every call."""
+    W = [rnd(512, 512, dtype=BF, seed=i, gain=0.04) for i in range(3)]
+    x0 = rnd(700, 512, dtype=BF, seed=9)
+
+    def chain(wait):
+        x, h = x0, x0
+        for i in range(60):
+            rows = (700, 3, 1, 260)[i % 4]
+            y, h2 = q().rms_norm(x[:rows], residual=h[:rows])
+            wait()
+            y8, s = q().quantize_rows(y)
+            wait()
+            w8, t = q().quantize_rows(W[i % 3])
+            wait()
+            z = q().linear(y8, w8, x_scale=s, weight_scale=t, activation="silu", residual=h2)
+            wait()
+            u = q().linear(z, W[(i + 1) % 3], activation="gelu")
+            wait()
+            x = torch.cat((u, x[rows:]))
+            h = torch.cat((z, h[rows:]))
+        return x, h
+    a = chain(lambda: None)
+    b = chain(torch.cuda.synchronize)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
