@@ -316,7 +316,6 @@ template <typename Out, int ES, int T, bool SLOPE, int RINGS>
 __global__ void __launch_bounds__(kTileThreads, RINGS)
     tile_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a) {
   using C = TileCfg<T, RINGS>;
-  allow_next();
   extern __shared__ char smraw[];
   char* sm = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[C::STAGES], empty[C::STAGES], done;
@@ -436,6 +435,7 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
       }
     }
     bool ok = nk == 0 || tc::mbar_wait(&done, 0);
+    allow_next();
     if (!ok) atomicExch(&g_timeout, 1);
     ok = __all_sync(0xffffffffu, ok);
     tc::tc_fence_after();
@@ -581,7 +581,6 @@ struct TokenArgs {
 
 template <typename Out, typename In, int M, int R, int SPLIT, bool VEC>
 __global__ void __launch_bounds__(256) token_kernel(TokenArgs a) {
-  allow_next();
   after_previous();
   __shared__ float s_part[SPLIT == 1 ? 1 : 8][M * R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -608,7 +607,7 @@ __global__ void __launch_bounds__(256) token_kernel(TokenArgs a) {
   float acc[M][R] = {};
   constexpr int N = VEC ? Chunk<In>::N : 1;
   constexpr int STEP = 32 * N * SPLIT;
-  constexpr int U = VEC ? (R * M >= 8 ? 2 : 4) : 8;  // steps in flight
+  constexpr int U = VEC ? (R * M == 1 ? 8 : R * M >= 8 ? 2 : 4) : 8;  // steps in flight
   for (int k0 = 32 * N * part + N * lane; k0 < a.k; k0 += STEP * U) {
     if constexpr (VEC) {
       uint4 wv[U][R];
@@ -658,6 +657,7 @@ __global__ void __launch_bounds__(256) token_kernel(TokenArgs a) {
       }
     }
   }
+  allow_next();
   float sum = 0.f;  // of this lane's output
 #pragma unroll
   for (int t = 0; t < M; ++t)
@@ -692,7 +692,6 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     dz_kernel(const T* dy, int64_t lddy, const uint16_t* slope, T* dz, int64_t lddz, float* part,
               int64_t m, int64_t n) {
-  allow_next();
   after_previous();
   __shared__ float s[8][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -737,6 +736,7 @@ __global__ void __launch_bounds__(256)
       }
     }
   }
+  allow_next();
   if (!part) return;
 #pragma unroll
   for (int c = 0; c < 8; ++c) s[warp][VEC ? 8 * lane + c : 32 * c + lane] = sum[c];

@@ -138,7 +138,6 @@ template <typename Out, int ES, int TN, bool SLOPE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ PairArgs a) {
   using C = PairCfg<TN>;
-  allow_next();
   extern __shared__ __align__(1024) char sm[];
   char* staging = sm + C::STAGES * C::STAGE;
   float(*s_col)[2][32] = reinterpret_cast<float(*)[2][32]>(staging + C::STAGING);
@@ -292,6 +291,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           if (ok && !tc::mbar_wait(&acc_full[b], (turn >> 1) & 1)) ok = false;
           tc::tc_fence_after();
           waited = true;
+          if (t + pairs >= tiles) allow_next();  // this CTA's last sums
         }
         if (e.res && live && a.tma_res) {
           if (ok && !tc::mbar_wait(&res_bar[warp], res_phase)) ok = false;

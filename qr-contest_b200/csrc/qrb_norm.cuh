@@ -283,7 +283,6 @@ struct Weight {
 // TH is the type that the norm reads: the stream's with a residual, else x's.
 template <typename TX, typename TH, bool RES, bool Q8, bool NORM, int VPT, int NT>
 __global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VPT)) fwd_kernel(FwdArgs a) {
-  allow_next();
   after_previous();
   __shared__ float s_sum[32];
   __shared__ uint2 s_both[32];
@@ -318,6 +317,7 @@ __global__ void __launch_bounds__(max_threads(VPT), kMaxThreads / max_threads(VP
   }
   float r = 1.f;
   if (NORM) w.load(mine, a.w, a.w_f32);
+  allow_next();
   float absmax = 0.f;
   if (NORM || Q8) {
     // max |y| = r max |h w|, so the scale takes no reduction of its own after r is known
@@ -477,7 +477,6 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 template <typename TX, typename TH, typename TW, int VPT, int NT>
 __global__ void __launch_bounds__(NT == 32 ? 128 : NT == 256 ? 256 : 512, NT == 32 ? 8 : NT == 256 ? 4 : 1)
     bwd_kernel(BwdArgs a, int depth) {
-  allow_next();
   after_previous();
   constexpr bool VEC = NT == 0;
   extern __shared__ __align__(16) char ring[];
@@ -626,6 +625,7 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT == 256 ? 256 : 512, NT == 
     }
     if (VEC && depth == 2) stage ^= 1;
   }
+  allow_next();
   if (!a.part) return;
   float sum[VPT][8];
 #pragma unroll

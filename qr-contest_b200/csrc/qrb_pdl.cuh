@@ -4,8 +4,11 @@
 // microsecond or more for the next to be launched and set up.  Launched with programmatic stream
 // serialization, a kernel may start once every block of the one before has called allow_next() (or has
 // ended); it sets itself up and then waits in after_previous() until everything before it in the
-// stream has completed and is visible.  So every kernel here calls allow_next() first, and no thread
-// touches global memory before after_previous().  Without the launch attribute both do nothing.
+// stream has completed and is visible.  So no thread touches global memory before after_previous(), and
+// a kernel calls allow_next() when its loads are done: blocks that wait take places, and with the call
+// at the start, blocks of the next kernels but one settled unevenly between this one's (one token
+// 4096 x 4096 in 8 bits: 8.2 us, with the call after the loads 6.2).  Without the launch attribute both do
+// nothing.
 #pragma once
 #include <cuda_runtime.h>
 
