@@ -360,13 +360,14 @@ int product_token(const lin::TokenArgs& a, cudaStream_t st) {
 }
 
 // Which kernel and tile: the least of their times by a model of them, in microseconds, that fits
-// what a sweep over 18 sizes measured (64 x 4096 x 4096 to 2048^3, each at 5 to 7 choices) and picks
-// the fastest or one within 4% of it on all of them.  Every kernel moves its operands at the rate
+// what a sweep over 30 sizes measured (16 x 4096 x 4096 to 2048^3 and 8192 x 256 x 1024, each at 3 to 7
+// choices) and picks the fastest or one within 7% of it on all of them, the fastest on 26.  Every kernel moves its operands at the rate
 // at which an SM can fetch them, so a CTA's time is its blocks of 128 bytes of k times a cost a block.
 //   pair kernel, 256 x 256: 8 + 0.33 a block and wave over 74 pairs; 256 x 128: 7.3 + 0.31
 //   (2048^3: 18.6, measured 19.2; 512 x 4096 x 4096 in 256 x 128: 27.1, measured 27.3)
 //   tile kernel, 128 x T: 7.3 + T / 128 + 0.21 to 0.28 a block with one CTA an SM, 0.30 to 0.44 with
-//   two, and 0.6 to 3.5 for a cluster's exchange (128 x 4096 x 4096 over clusters of 4: 14.0, measured 13.9)
+//   two, and 0.6 to 1.6 for a cluster's exchange (128 x 4096 x 4096 over clusters of 4: 14.0, measured 12.9);
+//   clusters of 8 that fill more than 64 SMs do not all find 8 free ones side by side: 6
 struct Choice { bool pair; int tile, splits; };
 Choice choose(int64_t m, int64_t n, int64_t k, int es, bool p_row) {
   const int64_t nkb = (k * es + 127) / 128, tj = (n + 127) / 128;
@@ -379,7 +380,7 @@ Choice choose(int64_t m, int64_t n, int64_t k, int es, bool p_row) {
     }
   };
   const struct { int tile; double alone, shared; } kinds[] = {{16, 0.21, 0.30}, {32, 0.21, 0.32}, {64, 0.22, 0.36}, {128, 0.28, 0.44}};
-  const struct { int splits; double exchange; } clusters[] = {{1, 0.0}, {2, 0.6}, {4, 1.2}, {8, 3.5}};
+  const struct { int splits; double exchange; } clusters[] = {{1, 0.0}, {2, 0.6}, {4, 1.2}, {8, 1.6}};
   for (const auto& kind : kinds) {
     const int T = kind.tile;
     // no tile that a narrower one would hold, none that m takes more than two of (128: any number);
@@ -390,7 +391,8 @@ Choice choose(int64_t m, int64_t n, int64_t k, int es, bool p_row) {
       if (cl.splits > 1 && nkb / cl.splits < 2) break;
       const int64_t ctas = tiles * cl.splits, part = (nkb + cl.splits - 1) / cl.splits, waves = (ctas + 2 * kSMs - 1) / (2 * kSMs);
       const double body = ctas <= kSMs ? part * kind.alone : waves * part * kind.shared * (waves > 1 ? 1.25 : 1.0);
-      offer({false, T, cl.splits}, 7.3 + T / 128.0 + cl.exchange + body);
+      const double exchange = cl.splits == 8 && ctas > 64 ? 6.0 : cl.exchange;
+      offer({false, T, cl.splits}, 7.3 + T / 128.0 + exchange + body);
     }
   }
   if (m > 128 && k > 0)
