@@ -296,7 +296,7 @@ __device__ __forceinline__ void put4(void* p, uint2 packed, bool vec, int left) 
 // for memory would show.  So would the time to fetch instructions that run once (with 16 rows
 // unrolled, finishing a tile took 16 us): loops stay loops, and there are no divisions.  Bound by the
 // rate at which an SM fetches its operands, and when short by set-up, exchange and epilogue, about
-// 4 us: 16 x 8192 x 8192 in 8 bits 14.8 us (4.6 TB/s), 128 x 4096 x 4096 bf16 13.2 us.
+// 4 us: 16 x 8192 x 8192 in 8 bits 14.5 us (4.6 TB/s), 128 x 4096 x 4096 bf16 12.9 us.
 constexpr int kTileThreads = 352;
 constexpr int kTileQ = 128;
 
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
 // bytes; single elements where rows start off 16 bytes), the same part of the M tokens from the L1
 // cache, and adds the products in float32; SPLIT warps share a feature's k where there are too few
 // features to fill the GPU.  One lane per (token, feature) finishes it.  Measured, bf16: 1 x 8192 x 8192
-// 23.7 us (5.7 TB/s), 1 x 4096 x 4096 8.8 us, 1 x 512 x 512 2.0 us (tiles: 10.5, 4.4 for the last two).
+// 23.7 us (5.7 TB/s), 1 x 4096 x 4096 8.1 us, 1 x 512 x 512 2.0 us (tiles: 10.5, 4.4 for the last two).
 template <typename T> struct Chunk;  // 16 bytes of an operand as float
 template <> struct Chunk<__nv_bfloat16> {
   static constexpr int N = 8;

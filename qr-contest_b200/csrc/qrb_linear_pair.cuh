@@ -16,7 +16,7 @@
 // a row at a time); a residual comes in the same way before the sums are needed.  No multicast loads.
 // Bound by power in long runs (4096 x 16384 x 4096 bf16: 356 us in short runs, 400 to 413 sustained, 1.3 to
 // 1.4 PFLOP/s; with bias and gelu 430) and by the operands' way into shared memory in 8 bits
-// (8192 x 8192 x 4096: 196 us, 2.8 PFLOP/s).  The tensor pipe is 77 % active.
+// (8192 x 8192 x 4096: 196 us, 2.8 PFLOP/s).  The tensor pipe is 80 % active.
 //
 // Every wait is bounded.  A role whose wait runs out raises g_timeout and stops; the epilogue then
 // writes NaN for the tiles it still owes, and the loads in flight get time to land before the exit.

@@ -17,6 +17,14 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(scope="module", autouse=True)
+def _give_memory_back():
+    """Leaves no cached blocks behind: with none, what the next module allocates comes from the device again."""
+    yield
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+
 BF, F16, F32, FP8 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
 U = {BF: 2.0 ** -8, F16: 2.0 ** -11, F32: 2.0 ** -24}
 SUB = {BF: 2.0 ** -133, F16: 2.0 ** -25, F32: 2.0 ** -149}

@@ -9,8 +9,17 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _give_memory_back():
+    """Leaves no cached blocks behind: with none, what the next module allocates comes from the device again."""
+    yield
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("width,hidden,tokens", [(512, 2048, 300), (64, 200, 17)])
