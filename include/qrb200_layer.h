@@ -4,7 +4,8 @@
  *
  * All pointers are device pointers; rows of a matrix are `ld` elements apart (any ld that keeps
  * rows apart on outputs; inputs may overlap or repeat, ld = 0 included, except matrix-product
- * operands) and contiguous inside; bases and strides need no alignment.  Everything is
+ * operands) and contiguous inside; bases and strides need no alignment but their elements'.  A
+ * workspace may start at any byte: the queried sizes allow for that.  Everything is
  * enqueued on `stream`; nothing is synchronised.  Empty sizes are a successful no-op.
  *
  * Status codes, element types and the conventions of qrb200.h; nothing here depends on PyTorch or

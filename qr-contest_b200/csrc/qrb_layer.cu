@@ -47,7 +47,12 @@ int raise_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready) {
   return QRB200_OK;
 }
 
-// Device memory for one call when the caller gives none; freed in stream order.
+// A workspace may start anywhere: its first byte on 16 is where it is used from, so the sizes that
+// the queries report hold 15 bytes more than the buffers in it (TMA and 16-byte stores need the
+// alignment, and what is planned for aligned buffers would not fit the copies of others).
+size_t workspace_size(size_t need) { return need ? need + 15 : 0; }
+
+// Device memory for one call: the caller's, or our own when there is none, freed in stream order.
 struct Scratch {
   void* p = nullptr;
   cudaStream_t st;
@@ -56,8 +61,9 @@ struct Scratch {
   int get(void* given, size_t given_bytes, size_t need) {
     if (!need) return QRB200_OK;
     if (given) {
-      if (given_bytes < need) return QRB200_ERR_WORKSPACE;
-      p = given;
+      const size_t skip = -reinterpret_cast<uintptr_t>(given) & 15;
+      if (given_bytes < need || given_bytes - need < skip) return QRB200_ERR_WORKSPACE;
+      p = static_cast<char*>(given) + skip;
       return QRB200_OK;
     }
     if (note(cudaMallocAsync(&p, need, st)) != cudaSuccess) return QRB200_ERR_CUDA;
@@ -527,10 +533,11 @@ int qrb200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t dim, int32_t 
                                              size_t* bytes) {
   if (!bytes || !float_type(dtype) || !(stream_dtype == dtype || stream_dtype == QRB200_F32) || rows < 0 || dim < 0 || rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30))
     return QRB200_ERR_INVALID_ARG;
-  *bytes = 0;
+  size_t need = 0;
   if (rows && dim)  // aligned or not
     for (const bool vec : {false, true})
-      *bytes = std::max(*bytes, (size_t)bwd_plan(rows, (int)dim, esize(dtype), esize(stream_dtype), vec).parts * dim * sizeof(float));
+      need = std::max(need, (size_t)bwd_plan(rows, (int)dim, esize(dtype), esize(stream_dtype), vec).parts * dim * sizeof(float));
+  *bytes = workspace_size(need);
   return QRB200_OK;
 }
 
@@ -555,7 +562,7 @@ int qrb200_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_
   const int es = esize(dtype), rs = esize(stream_dtype);
   const bool vec = dim % 8 == 0 && rows_on16(dy, lddy, es) && rows_on16(h, ldh, rs) &&
                    (!dh || rows_on16(dh, lddh, rs)) && (!dx || on16(dx)) && (!dresidual || on16(dresidual)) &&
-                   (!weight || on16(weight)) && on16(workspace);
+                   (!weight || on16(weight));
   const BwdPlan plan = bwd_plan(rows, (int)dim, es, rs, vec);
   Scratch ws(st);
   int rc = ws.get(workspace, workspace_bytes, dweight ? (size_t)plan.parts * dim * sizeof(float) : 0);
@@ -580,8 +587,8 @@ int qrb200_linear_workspace_bytes(const void* x, int64_t ldx, const void* w, int
       (dtype == QRB200_E4M3 && w_transposed))
     return QRB200_ERR_INVALID_ARG;
   const int es = esize(dtype);
-  *bytes = m && n && k ? aligned_copy_bytes(Operand{x, ldx, false}, m, k, es) +
-                             aligned_copy_bytes(Operand{w, ldw, w_transposed != 0}, n, k, es)
+  *bytes = m && n && k ? workspace_size(aligned_copy_bytes(Operand{x, ldx, false}, m, k, es) +
+                                        aligned_copy_bytes(Operand{w, ldw, w_transposed != 0}, n, k, es))
                        : 0;
   return QRB200_OK;
 }
@@ -625,9 +632,9 @@ int qrb200_linear_backward_workspace_bytes(const void* dy, int64_t lddy, int32_t
                                            int32_t want_dw, int32_t want_dbias, int64_t m, int64_t n, int64_t k,
                                            size_t* bytes) {
   if (!bytes || !sizes_ok(m, n, k) || !sizes_ok(k, m, n)) return QRB200_ERR_INVALID_ARG;
-  *bytes = m && n ? backward_plan(dy, lddy, has_slope != 0, Operand{x, ldx, false}, Operand{w, ldw, w_transposed != 0},
-                                  want_dx && k, want_dw && k, want_dbias, m, n, k)
-                        .total
+  *bytes = m && n ? workspace_size(backward_plan(dy, lddy, has_slope != 0, Operand{x, ldx, false}, Operand{w, ldw, w_transposed != 0},
+                                                 want_dx && k, want_dw && k, want_dbias, m, n, k)
+                                       .total)
                   : 0;
   return QRB200_OK;
 }

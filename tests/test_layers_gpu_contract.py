@@ -1,0 +1,87 @@
+"""GPU: what the layer operators promise about workspaces, streams, waits and the ends of their ranges.
+
+Bounds are derived beside each test; u is the unit roundoff of a type (2^-8 bf16, 2^-11 f16, 2^-24 f32)."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, F16, F32, FP8 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _give_memory_back():
+    """No bounded wait ran out in here; leaves no cached blocks behind."""
+    yield
+    from qrb200 import _lib
+    assert not _lib.layer_timed_out()
+    torch.cuda.empty_cache()
+
+
+def q():
+    import qrb200
+    return qrb200
+
+
+def rnd(*shape, dtype=F32, seed=0, gain=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * gain).to(dtype)
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+# ---------------------------------------------------------------------- workspaces
+
+class Workspace:
+    """`size` bytes that start `off` bytes past a 256-byte boundary, in front of and behind bytes of 0xA5."""
+
+    def __init__(self, size, off):
+        self.all = torch.full((size + 1024,), 0xA5, dtype=torch.uint8, device="cuda")
+        assert self.all.data_ptr() % 256 == 0
+        self.first, self.size, self.ptr = 256 + off, size, self.all.data_ptr() + 256 + off
+
+    def untouched(self):
+        return bool((self.all[:self.first] == 0xA5).all()) and bool((self.all[self.first + self.size:] == 0xA5).all())
+
+
+@pytest.mark.parametrize("off", [0, 1, 2, 4, 8, 15])
+def test_workspace_starts_anywhere(off):
+    """Same bits as with a workspace of torch's, and nothing written outside it."""
+    from qrb200 import _lib
+    L, n = _lib.lib(), ctypes.c_size_t()
+    ok = _lib.QRB200_OK
+    # a product whose operands are both copied
+    x, w = rnd(40, 37, dtype=BF, seed=1), rnd(50, 37, dtype=BF, seed=2)
+    want = q().linear(x, w)
+    y = torch.empty_like(want)
+    assert L.qrb200_linear_workspace_bytes(x.data_ptr(), 37, w.data_ptr(), 37, 0, 40, 50, 37, 1, ctypes.byref(n)) == ok
+    ws = Workspace(n.value, off)
+    assert L.qrb200_linear(x.data_ptr(), 37, w.data_ptr(), 37, 0, None, None, None, None, 0, y.data_ptr(), 50, None, 40, 50, 37, 1, 1, 0,
+                           ws.ptr, ws.size, stream()) == ok
+    assert torch.equal(y, want) and ws.untouched()
+    # its gradients, with dz, partial sums and copies in the workspace
+    dy = rnd(40, 50, dtype=BF, seed=3)
+    slope = torch.ops.qrb200.linear(x, w, None, None, _lib.ACT_SILU, None, None, None, True)[1]
+    want = torch.ops.qrb200.linear_backward(dy, slope, x, w, True, True, True)
+    got = [torch.empty_like(t) for t in want]
+    assert L.qrb200_linear_backward_workspace_bytes(dy.data_ptr(), 50, 1, x.data_ptr(), 37, w.data_ptr(), 37, 0, 1, 1, 1, 40, 50, 37,
+                                                    ctypes.byref(n)) == ok
+    ws = Workspace(n.value, off)
+    assert L.qrb200_linear_backward(dy.data_ptr(), 50, slope.data_ptr(), x.data_ptr(), 37, w.data_ptr(), 37, 0, *(t.data_ptr() for t in got),
+                                    40, 50, 37, 1, ws.ptr, ws.size, stream()) == ok
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and ws.untouched()
+    # the norm's gradients, by vectors and by single elements
+    for dim in (64, 65):
+        h, dy, w = rnd(300, dim, seed=4), rnd(300, dim, seed=5), rnd(dim, seed=6)
+        want = torch.ops.qrb200.rms_norm_backward(dy, h, None, w, 1e-6, True, False, True)
+        dx, dw = torch.empty_like(h), torch.empty_like(w)
+        assert L.qrb200_rms_norm_backward_workspace_bytes(300, dim, 0, 0, ctypes.byref(n)) == ok
+        ws = Workspace(n.value, off)
+        assert L.qrb200_rms_norm_backward(dy.data_ptr(), dim, h.data_ptr(), dim, None, 0, w.data_ptr(), 0, dx.data_ptr(), None,
+                                          dw.data_ptr(), 300, dim, 1e-6, 0, 0, ws.ptr, ws.size, stream()) == ok
+        assert torch.equal(dx, want[0]) and torch.equal(dw, want[2]) and ws.untouched()
