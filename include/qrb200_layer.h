@@ -76,8 +76,9 @@ int qrb200_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_
  *            residual may be y itself (in place)
  *   slope    [m][n] contiguous, or NULL: act'(z) for qrb200_linear_backward as
  *            round(2^15 (act' + 1/4)), 65535 for NaN; not for E4M3
- * m and n up to 8388480 (128 * 65535).  Sums are float32; y is rounded once.  `workspace` (NULL: allocated stream-ordered) holds aligned
- * copies of operands whose rows do not all start on 16 bytes; none is needed otherwise. */
+ * m and n up to 8388480 (128 * 65535), k up to 2^31 - 65537.  Sums are float32; y is rounded once.
+ * `workspace` (NULL: allocated stream-ordered) holds aligned copies of operands whose rows do not
+ * all start on 16 bytes; none is needed otherwise. */
 int qrb200_linear_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw,
                                   int32_t w_transposed, int64_t m, int64_t n, int64_t k,
                                   int32_t dtype, size_t* bytes);

@@ -442,10 +442,12 @@ int product(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_t k,
 }
 
 constexpr int64_t kMostRows = 128 * 65535;  // of x, and of the weight
+// Kernels walk along k with int indices that run past it: tiles by less than a block of 128, token_kernel
+// by less than a turn of all its warps, 32768 elements of 8 bits.
+constexpr int64_t kMostColumns = ((int64_t)1 << 31) - 65537;
 bool sizes_ok(int64_t m, int64_t n, int64_t k) {
-  constexpr int64_t top = (int64_t)1 << 31;
   // a grid's y and z have 16 bits, and an index into one operand's rows 31
-  return m >= 0 && n >= 0 && k >= 0 && m <= kMostRows && n <= kMostRows && k < top - 256;
+  return m >= 0 && n >= 0 && k >= 0 && m <= kMostRows && n <= kMostRows && k <= kMostColumns;
 }
 
 // Blocks of dz_kernel along m, each of which leaves one part of the bias' sum: 8 blocks an SM.

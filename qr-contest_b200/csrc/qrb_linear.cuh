@@ -608,6 +608,7 @@ __global__ void __launch_bounds__(256) token_kernel(TokenArgs a) {
   constexpr int N = VEC ? Chunk<In>::N : 1;
   constexpr int STEP = 32 * N * SPLIT;
   constexpr int U = VEC ? (R * M == 1 ? 8 : R * M >= 8 ? 2 : 4) : 8;  // steps in flight
+  static_assert(STEP * U <= 32768, "k0 passes k by less than the margin below 2^31 that callers keep");
   for (int k0 = 32 * N * part + N * lane; k0 < a.k; k0 += STEP * U) {
     if constexpr (VEC) {
       uint4 wv[U][R];

@@ -44,3 +44,17 @@ def test_workspace_off_16_bytes_has_to_be_larger(start):
     for size in (0, 31, 32, 32 + skip - 1):
         assert L.qrb200_rms_norm_backward(16, 8, 16, 8, None, 8, 16, 0, 16, None, 16, 2, 8, 1e-6, 0, 0, start, size,
                                           None) == _lib.QRB200_ERR_WORKSPACE
+
+
+# ---------------------------------------------------------------------- sizes
+
+def test_sums_too_long_for_int_indices_are_refused():
+    """Kernels step past k by up to 32768 elements: their int index must not pass 2^31 on the way."""
+    L, n, most = _lib.lib(), ctypes.c_size_t(), 2 ** 31 - 65537
+    size = lambda k, t: L.qrb200_linear_workspace_bytes(16, k, 16, k, 0, 1, 1, k, t, ctypes.byref(n))  # noqa: E731
+    for t in (_lib.QRB200_BF16, _lib.QRB200_E4M3):
+        assert size(most, t) == _lib.QRB200_OK
+        for k in (most + 1, 2 ** 31 - 32768, 2 ** 31 - 257, 2 ** 31):
+            assert size(k, t) == _lib.QRB200_ERR_INVALID_ARG
+            assert L.qrb200_linear(16, k, 16, k, 0, None, None, None, None, 0, 16, 1, None, 1, 1, k, t, _lib.QRB200_BF16, 0, None, 0,
+                                   None) == _lib.QRB200_ERR_INVALID_ARG
