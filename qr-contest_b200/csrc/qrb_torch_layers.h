@@ -1,5 +1,7 @@
 // qrb200 -- the layer operators as C++ functions on tensors (libqrb200_torch_ops.so), with their
-// gradients: what torch.ops.qrb200.* and the Python entry points call.
+// gradients, for callers that have made sure that nothing listens for operators (no dispatch mode, no
+// tensor subclass, no transform): with nothing to differentiate they do not go through the dispatcher.
+// All others call torch.ops.qrb200.*.
 #pragma once
 #include <ATen/ATen.h>
 

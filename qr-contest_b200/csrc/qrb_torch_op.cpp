@@ -18,6 +18,7 @@
 // TypeError before anything is allocated.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -353,6 +354,27 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward(const at::Tensor&
 }
 
 // ---- gradients ----
+// The operators by way of the dispatcher.  What runs below autograd is called like this and not as a
+// function, so that whatever is listening there (a dispatch mode, a fake tensor, a trace) sees the operator.
+auto& rms_norm_op() {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("qrb200::rms_norm", "").typed<decltype(rms_norm)>();
+  return op;
+}
+auto& rms_norm_backward_op() {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("qrb200::rms_norm_backward", "").typed<decltype(rms_norm_backward)>();
+  return op;
+}
+auto& linear_op() {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("qrb200::linear", "").typed<decltype(linear)>();
+  return op;
+}
+auto& linear_backward_op() {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("qrb200::linear_backward", "").typed<decltype(linear_backward)>();
+  return op;
+}
+
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -372,7 +394,7 @@ struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
                                const OptTensor& residual, double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
     ctx->set_materialize_grads(false);
-    auto [y, scale, h] = rms_norm(x, weight, residual, eps, c10::nullopt);
+    auto [y, scale, h] = rms_norm_op().call(x, weight, residual, eps, c10::nullopt);
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["residual"] = residual.has_value();
     ctx->saved_data["type"] = x.scalar_type();
@@ -393,28 +415,26 @@ struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
       if (!dh.defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
       dy = at::zeros(h.sizes(), h.options().dtype(ctx->saved_data["type"].toScalarType()));
     }
-    auto [dx, dres, dw] = rms_norm_backward(dy, h, given(dh), given(weight), ctx->saved_data["eps"].toDouble(), want_x, want_r, want_w);
+    auto [dx, dres, dw] =
+        rms_norm_backward_op().call(dy, h, given(dh), given(weight), ctx->saved_data["eps"].toDouble(), want_x, want_r, want_w);
     return {want_x ? dx : at::Tensor(), dw, dres, at::Tensor()};
   }
 };
 
-}  // namespace
-
-// Below autograd with nothing to differentiate; otherwise with a node that can.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> qrb200::rms_norm(const at::Tensor& x, const OptTensor& weight,
-                                                                const OptTensor& residual, double eps,
-                                                                c10::optional<at::ScalarType> out_dtype) {
+// Below autograd with nothing to differentiate; otherwise with a node that can.  LISTENED: something may
+// see operators below autograd.
+template <bool LISTENED>
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_grad(const at::Tensor& x, const OptTensor& weight, const OptTensor& residual,
+                                                             double eps, c10::optional<at::ScalarType> out_dtype) {
   const at::Tensor w = weight.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
   if (!wants_grad({&x, &w, &r})) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return ::rms_norm(x, weight, residual, eps, out_dtype);
+    return LISTENED ? rms_norm_op().call(x, weight, residual, eps, out_dtype) : rms_norm(x, weight, residual, eps, out_dtype);
   }
   TORCH_CHECK_VALUE(!out_dtype || *out_dtype == x.scalar_type(), "qrb200: the 8-bit norm has no gradient (use torch.no_grad())");
   variable_list out = RmsNormGrad::apply(x, weight, residual, eps);
   return {out[0], at::Tensor(), out.size() > 1 ? out[1] : at::Tensor()};
 }
-
-namespace {
 
 struct LinearGrad : torch::autograd::Function<LinearGrad> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
@@ -424,8 +444,8 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
     const bool sums = x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad());
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["residual"] = residual.has_value();
-    auto [y, slope] = linear(x, weight, bias, residual, activation, c10::nullopt, c10::nullopt, out_dtype,
-                             sums && activation != QRB200_ACT_NONE);
+    auto [y, slope] = linear_op().call(x, weight, bias, residual, activation, c10::nullopt, c10::nullopt, out_dtype,
+                                       sums && activation != QRB200_ACT_NONE);
     if (sums) ctx->save_for_backward({x, weight, slope});
     return {y};
   }
@@ -440,27 +460,43 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
     const bool want_r = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(edge++);
     if (want_x || want_w || want_b) {
       const auto saved = ctx->get_saved_variables();
-      std::tie(out[0], out[1], out[2]) = linear_backward(dy, given(saved[2]), saved[0], saved[1], want_x, want_w, want_b);
+      std::tie(out[0], out[1], out[2]) =
+          linear_backward_op().call(dy, given(saved[2]), saved[0], saved[1], want_x, want_w, want_b);
     }
     if (want_r) out[3] = dy;
     return out;
   }
 };
 
-}  // namespace
-
-std::tuple<at::Tensor, at::Tensor> qrb200::linear(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
-                                                  const OptTensor& residual, int64_t activation, const OptTensor& x_scale,
-                                                  const OptTensor& weight_scale, c10::optional<at::ScalarType> out_dtype,
-                                                  bool want_slope) {
+template <bool LISTENED>
+std::tuple<at::Tensor, at::Tensor> linear_grad(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
+                                               const OptTensor& residual, int64_t activation, const OptTensor& x_scale,
+                                               const OptTensor& weight_scale, c10::optional<at::ScalarType> out_dtype,
+                                               bool want_slope) {
   const at::Tensor b = bias.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
   if (!wants_grad({&x, &weight, &b, &r})) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return ::linear(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
+    return LISTENED ? linear_op().call(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope)
+                    : linear(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
   }
   TORCH_CHECK_VALUE(x.scalar_type() != at::kFloat8_e4m3fn, "qrb200: the 8-bit product has no gradient (use torch.no_grad())");
   TORCH_CHECK_VALUE(!x_scale && !weight_scale, "qrb200: scales belong to 8-bit operands");
   return {LinearGrad::apply(x, weight, bias, residual, activation, out_dtype)[0], at::Tensor()};
+}
+
+}  // namespace
+
+// The short way: its callers have made sure that nothing listens.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> qrb200::rms_norm(const at::Tensor& x, const OptTensor& weight,
+                                                                const OptTensor& residual, double eps,
+                                                                c10::optional<at::ScalarType> out_dtype) {
+  return rms_norm_grad<false>(x, weight, residual, eps, out_dtype);
+}
+std::tuple<at::Tensor, at::Tensor> qrb200::linear(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
+                                                  const OptTensor& residual, int64_t activation, const OptTensor& x_scale,
+                                                  const OptTensor& weight_scale, c10::optional<at::ScalarType> out_dtype,
+                                                  bool want_slope) {
+  return linear_grad<false>(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
 }
 
 TORCH_LIBRARY(qrb200, m) {
@@ -494,8 +530,8 @@ TORCH_LIBRARY_IMPL(qrb200, Meta, m) {
 }
 
 TORCH_LIBRARY_IMPL(qrb200, Autograd, m) {
-  m.impl("rms_norm", qrb200::rms_norm);
-  m.impl("linear", qrb200::linear);
+  m.impl("rms_norm", rms_norm_grad<true>);
+  m.impl("linear", linear_grad<true>);
 }
 
 // Host tensors (and mixes of host and device tensors, which reach this key too) are refused by the

@@ -12,6 +12,10 @@ FP8 = torch.float8_e4m3fn
 BF = torch.bfloat16
 
 
+def meta(*shape, dtype=BF):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
 def size_of(fn, *args):
     n = ctypes.c_size_t()
     assert getattr(_lib.lib(), fn)(*args, ctypes.byref(n)) == _lib.QRB200_OK
@@ -58,3 +62,86 @@ def test_sums_too_long_for_int_indices_are_refused():
             assert size(k, t) == _lib.QRB200_ERR_INVALID_ARG
             assert L.qrb200_linear(16, k, 16, k, 0, None, None, None, None, 0, 16, 1, None, 1, 1, k, t, _lib.QRB200_BF16, 0, None, 0,
                                    None) == _lib.QRB200_ERR_INVALID_ARG
+
+
+# ---------------------------------------------------------------------- what listens below autograd
+
+class Seen(torch.utils._python_dispatch.TorchDispatchMode):
+    """Records the layer operators that reach a dispatch mode."""
+
+    def __init__(self):
+        super().__init__()
+        self.ops = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        if func.namespace == "qrb200":
+            self.ops.append(func._opname)
+        return func(*args, **(kwargs or {}))
+
+
+def test_dispatch_modes_see_the_operators():
+    with Seen() as seen:
+        qrb200.rms_norm(meta(2, 8))
+        qrb200.rms_norm(meta(2, 8), residual=meta(2, 8), out_dtype=FP8)
+        qrb200.linear(meta(2, 8), meta(4, 8), activation="gelu")
+        qrb200.linear(meta(2, 8, dtype=FP8), meta(4, 8, dtype=FP8), x_scale=meta(2, dtype=torch.float32))
+    assert seen.ops == ["rms_norm", "rms_norm", "linear", "linear"]
+
+
+def test_dispatch_modes_see_the_gradients():
+    x, w = meta(2, 8).requires_grad_(), meta(4, 8).requires_grad_()
+    with Seen() as seen:
+        y, h = qrb200.rms_norm(x, residual=meta(2, 8))
+        dx, dw = torch.autograd.grad(qrb200.linear(y, w, activation="silu").sum() + h.sum(), (x, w))
+    assert seen.ops == ["rms_norm", "linear", "linear_backward", "rms_norm_backward"]
+    assert dx.shape == x.shape and dw.shape == w.shape
+
+
+def test_fake_tensors_of_a_gpu():
+    """Shapes without the GPU: nothing is allocated there."""
+    from torch._subclasses import FakeTensorMode
+    with FakeTensorMode():
+        x, w = (torch.empty(*s, dtype=BF, device="cuda") for s in ((2, 3, 8), (4, 8)))
+        y, h = qrb200.rms_norm(x, residual=x.float())
+        z = qrb200.linear(y, w, activation="gelu")
+        q8, s, h8 = qrb200.rms_norm(x, residual=x, out_dtype=FP8)
+    assert z.shape == (2, 3, 4) and z.dtype == BF and z.device.type == "cuda" and h.dtype == torch.float32
+    assert q8.shape == (2, 3, 8) and q8.dtype == FP8 and s.shape == (2, 3) and h8.dtype == BF
+
+
+def called(graph):
+    return [n.target._opname for n in graph.nodes if getattr(n.target, "namespace", "") == "qrb200"]
+
+
+def test_a_trace_holds_the_operators():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def forward(x, w):
+        return qrb200.linear(qrb200.rms_norm(x), w, activation="silu")
+
+    def gradients(x, w):
+        return torch.autograd.grad(forward(x, w).sum(), (x, w))
+    assert called(make_fx(forward)(meta(2, 8), meta(4, 8)).graph) == ["rms_norm", "linear"]
+    assert called(make_fx(gradients)(meta(2, 8).requires_grad_(), meta(4, 8).requires_grad_()).graph) == [
+        "rms_norm", "linear", "linear_backward", "rms_norm_backward"]
+
+
+def test_exported_and_compiled_programs_hold_the_operators():
+    class Block(torch.nn.Module):
+        def forward(self, x, w):
+            return qrb200.linear(qrb200.rms_norm(x), w, activation="silu")
+    qrb200.rms_norm(meta(2, 8))
+    assert called(torch.export.export(Block(), (meta(2, 8), meta(4, 8))).graph) == ["rms_norm", "linear"]
+    graphs = []
+
+    def keep(gm, inputs):
+        graphs.append(called(gm.graph))
+        return gm.forward
+    from torch._dynamo.backends.common import aot_autograd
+    torch._dynamo.reset()
+    step = torch.compile(Block(), backend=aot_autograd(fw_compiler=keep), fullgraph=True, dynamic=True)
+    for rows in (2, 5):
+        x, w = meta(rows, 8).requires_grad_(), meta(4, 8).requires_grad_()
+        dx, dw = torch.autograd.grad(step(x, w).sum(), (x, w))
+        assert dx.shape == x.shape and dw.shape == w.shape
+    assert graphs[:2] == [["rms_norm", "linear"], ["linear_backward", "rms_norm_backward"]]

@@ -85,3 +85,28 @@ def test_workspace_starts_anywhere(off):
         assert L.qrb200_rms_norm_backward(dy.data_ptr(), dim, h.data_ptr(), dim, None, 0, w.data_ptr(), 0, dx.data_ptr(), None,
                                           dw.data_ptr(), 300, dim, 1e-6, 0, 0, ws.ptr, ws.size, stream()) == ok
         assert torch.equal(dx, want[0]) and torch.equal(dw, want[2]) and ws.untouched()
+
+
+# ---------------------------------------------------------------------- what listens below autograd
+
+def test_a_trace_answers_for_its_own_inputs():
+    """A traced or compiled step gives on other inputs what the operators give there, to the bit."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def forward(x, w):
+        return q().linear(q().rms_norm(x), w, activation="silu")
+
+    def step(x, w):
+        return torch.autograd.grad(forward(x, w).sum(), (x, w))
+    first = rnd(33, 64, dtype=BF, seed=1), rnd(40, 64, dtype=BF, seed=2)
+    other = rnd(33, 64, dtype=BF, seed=3), rnd(40, 64, dtype=BF, seed=4)
+    assert torch.equal(make_fx(forward)(*first)(*other), forward(*other))
+    first, other = ([t.requires_grad_() for t in ts] for ts in (first, other))
+    want = step(*other)
+    assert all(torch.equal(a, b) for a, b in zip(make_fx(step)(*first)(*(t.detach() for t in other)), want))
+    torch._dynamo.reset()
+    compiled = torch.compile(forward, backend="aot_eager", fullgraph=True)
+    for x, w in (first, other):
+        y = compiled(x, w)
+        assert torch.equal(y, forward(x, w))
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y.sum(), (x, w)), step(x, w)))
