@@ -438,20 +438,23 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_grad(const at::Tensor& x
 
 struct LinearGrad : torch::autograd::Function<LinearGrad> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
-                               const OptTensor& residual, int64_t activation, c10::optional<at::ScalarType> out_dtype) {
+                               const OptTensor& residual, int64_t activation, c10::optional<at::ScalarType> out_dtype,
+                               bool want_slope) {
     at::AutoDispatchBelowADInplaceOrView below;
     ctx->set_materialize_grads(false);
     const bool sums = x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad());
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["residual"] = residual.has_value();
     auto [y, slope] = linear_op().call(x, weight, bias, residual, activation, c10::nullopt, c10::nullopt, out_dtype,
-                                       sums && activation != QRB200_ACT_NONE);
-    if (sums) ctx->save_for_backward({x, weight, slope});
-    return {y};
+                                       want_slope || (sums && activation != QRB200_ACT_NONE));
+    if (sums) ctx->save_for_backward({x, weight, activation == QRB200_ACT_NONE ? at::Tensor() : slope});
+    if (!want_slope) return {y};
+    ctx->mark_non_differentiable({slope});
+    return {y, slope};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_once();
-    variable_list out(6);
+    variable_list out(7);
     const at::Tensor& dy = grads[0];
     if (!dy.defined()) return out;
     size_t edge = 0;
@@ -481,7 +484,8 @@ std::tuple<at::Tensor, at::Tensor> linear_grad(const at::Tensor& x, const at::Te
   }
   TORCH_CHECK_VALUE(x.scalar_type() != at::kFloat8_e4m3fn, "qrb200: the 8-bit product has no gradient (use torch.no_grad())");
   TORCH_CHECK_VALUE(!x_scale && !weight_scale, "qrb200: scales belong to 8-bit operands");
-  return {LinearGrad::apply(x, weight, bias, residual, activation, out_dtype)[0], at::Tensor()};
+  variable_list out = LinearGrad::apply(x, weight, bias, residual, activation, out_dtype, want_slope);
+  return {out[0], out.size() > 1 ? out[1] : at::Tensor()};
 }
 
 }  // namespace

@@ -145,3 +145,16 @@ def test_exported_and_compiled_programs_hold_the_operators():
         dx, dw = torch.autograd.grad(step(x, w).sum(), (x, w))
         assert dx.shape == x.shape and dw.shape == w.shape
     assert graphs[:2] == [["rms_norm", "linear"], ["linear_backward", "rms_norm_backward"]]
+
+
+def test_the_slope_comes_with_gradients():
+    """linear's want_slope is for linear_backward: without the slope that takes the activation for the identity."""
+    qrb200.api.load_torch_ops()
+    x, w = meta(2, 8).requires_grad_(), meta(4, 8)
+    y, slope = torch.ops.qrb200.linear(x, w, None, None, _lib.ACT_SILU, None, None, None, True)
+    assert y.requires_grad and slope is not None and slope.shape == (2, 4) and slope.dtype == torch.int16 and not slope.requires_grad
+    # asked for, it is there without an activation as well, as it is without gradients
+    for grad in (False, True):
+        x = meta(2, 8).requires_grad_(grad)
+        assert torch.ops.qrb200.linear(x, w, None, None, _lib.ACT_NONE, None, None, None, True)[1] is not None
+        assert torch.ops.qrb200.linear(x, w, None, None, _lib.ACT_SILU, None, None, None, False)[1] is None

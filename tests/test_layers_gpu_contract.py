@@ -110,3 +110,18 @@ def test_a_trace_answers_for_its_own_inputs():
         y = compiled(x, w)
         assert torch.equal(y, forward(x, w))
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y.sum(), (x, w)), step(x, w)))
+
+
+def test_the_slope_comes_with_gradients():
+    """The operator's slope is the same with and without something to differentiate, and so are the gradients made
+    from it: a traced step may be run on tensors that require gradients."""
+    from qrb200 import _lib
+    x, w, dy = rnd(33, 64, dtype=BF, seed=1), rnd(40, 64, dtype=BF, seed=2), rnd(33, 40, dtype=BF, seed=3)
+    op = torch.ops.qrb200.linear
+    for act in (_lib.ACT_NONE, _lib.ACT_SILU):
+        y, slope = op(x, w, None, None, act, None, None, None, True)
+        xg = x.clone().requires_grad_()
+        yg, slope_g = op(xg, w, None, None, act, None, None, None, True)
+        assert torch.equal(y, yg) and torch.equal(slope, slope_g)
+        dx, = torch.autograd.grad(yg, xg, dy)
+        assert torch.equal(dx, torch.ops.qrb200.linear_backward(dy, slope_g, x, w, True, False, False)[0])
