@@ -21,6 +21,7 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -385,6 +386,12 @@ bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// A tangent would be lost without a word below here: it hangs on a tensor that need not require a gradient.
+void check_no_tangent(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(),
+                                "qrb200: the layer operators have no forward-mode derivative");
+}
 void check_once() {
   TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), "qrb200: the layer operators are differentiable once (no create_graph)");
 }
@@ -427,6 +434,7 @@ template <bool LISTENED>
 std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_grad(const at::Tensor& x, const OptTensor& weight, const OptTensor& residual,
                                                              double eps, c10::optional<at::ScalarType> out_dtype) {
   const at::Tensor w = weight.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
+  check_no_tangent({&x, &w, &r});
   if (!wants_grad({&x, &w, &r})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return LISTENED ? rms_norm_op().call(x, weight, residual, eps, out_dtype) : rms_norm(x, weight, residual, eps, out_dtype);
@@ -477,6 +485,8 @@ std::tuple<at::Tensor, at::Tensor> linear_grad(const at::Tensor& x, const at::Te
                                                const OptTensor& weight_scale, c10::optional<at::ScalarType> out_dtype,
                                                bool want_slope) {
   const at::Tensor b = bias.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
+  const at::Tensor xs = x_scale.value_or(at::Tensor()), ws = weight_scale.value_or(at::Tensor());
+  check_no_tangent({&x, &weight, &b, &r, &xs, &ws});
   if (!wants_grad({&x, &weight, &b, &r})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return LISTENED ? linear_op().call(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope)
@@ -536,6 +546,10 @@ TORCH_LIBRARY_IMPL(qrb200, Meta, m) {
 TORCH_LIBRARY_IMPL(qrb200, Autograd, m) {
   m.impl("rms_norm", rms_norm_grad<true>);
   m.impl("linear", linear_grad<true>);
+  // no derivative of either mode: refused where one is asked for
+  m.impl("quantize_rows", torch::autograd::autogradNotImplementedFallback());
+  m.impl("rms_norm_backward", torch::autograd::autogradNotImplementedFallback());
+  m.impl("linear_backward", torch::autograd::autogradNotImplementedFallback());
 }
 
 // Host tensors (and mixes of host and device tensors, which reach this key too) are refused by the

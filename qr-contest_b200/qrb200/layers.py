@@ -11,7 +11,8 @@ All take CUDA tensors, run on the current stream without synchronising, and rais
 ``ValueError`` on arguments they do not take.  Leading dimensions are free; rows may be slices or
 expanded views (one row stride: read in place, anything else is copied first).  ``rms_norm`` and
 ``linear`` are differentiable once in every floating input where all types are 16 bits or more (the
-operators' own autograd formulas, in C++); the same inputs give the same bits.
+operators' own autograd formulas, in C++), in reverse mode: a second derivative, a forward-mode one or one of an
+8-bit output is refused, not dropped.  The same inputs give the same bits.
 """
 from __future__ import annotations
 

@@ -158,3 +158,58 @@ def test_the_slope_comes_with_gradients():
         x = meta(2, 8).requires_grad_(grad)
         assert torch.ops.qrb200.linear(x, w, None, None, _lib.ACT_NONE, None, None, None, True)[1] is not None
         assert torch.ops.qrb200.linear(x, w, None, None, _lib.ACT_SILU, None, None, None, False)[1] is None
+
+
+# ---------------------------------------------------------------------- derivatives there are not
+
+def tangents(call, *shapes, dual):
+    """call() on tensors of these shapes, the one at `dual` with a tangent."""
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level():
+        ts = [meta(*s) if isinstance(s, tuple) else s for s in shapes]
+        ts[dual] = fw.make_dual(ts[dual], torch.empty_like(ts[dual]))
+        return call(*ts)
+
+
+F32_4 = meta(4, dtype=torch.float32)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: tangents(lambda x: qrb200.rms_norm(x), (2, 8), dual=0),
+    lambda: tangents(lambda x: qrb200.rms_norm(x, out_dtype=FP8), (2, 8), dual=0),
+    lambda: tangents(lambda x, w: qrb200.rms_norm(x, w), (2, 8), (8,), dual=1),
+    lambda: tangents(lambda x, r: qrb200.rms_norm(x, residual=r), (2, 8), (2, 8), dual=1),
+    lambda: tangents(lambda x, w: qrb200.linear(x, w), (2, 8), (4, 8), dual=0),
+    lambda: tangents(lambda x, w: qrb200.linear(x, w, activation="gelu"), (2, 8), (4, 8), dual=1),
+    lambda: tangents(lambda x, w, b: qrb200.linear(x, w, b), (2, 8), (4, 8), (4,), dual=2),
+    lambda: tangents(lambda x, w, r: qrb200.linear(x, w, residual=r), (2, 8), (4, 8), (2, 4), dual=2),
+    lambda: tangents(lambda x, w, s: qrb200.linear(x, w, weight_scale=s), meta(2, 8, dtype=FP8), meta(4, 8, dtype=FP8), F32_4, dual=2),
+    lambda: tangents(lambda x: qrb200.quantize_rows(x), (2, 8), dual=0),
+    lambda: tangents(lambda x, w: qrb200.linear(x.requires_grad_(), w), (2, 8), (4, 8), dual=1),
+    lambda: torch.func.jvp(lambda x: qrb200.linear(x, meta(4, 8)), (meta(2, 8),), (meta(2, 8),)),
+    lambda: torch.func.jvp(lambda x: qrb200.rms_norm(x), (meta(2, 8),), (meta(2, 8),)),
+])
+def test_forward_mode_is_refused(call):
+    with pytest.raises(NotImplementedError):
+        call()
+
+
+@pytest.mark.parametrize("call", [lambda x: qrb200.rms_norm(x), lambda x: qrb200.linear(x, meta(8, 8), activation="silu")])
+def test_forward_over_reverse_is_refused(call):
+    """A tangent of the gradient that comes in is not dropped on the way back either."""
+    import torch.autograd.forward_ad as fw
+    x = meta(2, 8).requires_grad_()
+    y = call(x)
+    with fw.dual_level(), pytest.raises(NotImplementedError):
+        torch.autograd.grad(y, x, fw.make_dual(torch.empty_like(y), torch.empty_like(y)))
+
+
+def test_gradients_of_8_bits_are_refused():
+    w = meta(4, 8).requires_grad_()
+    w8, scale = qrb200.quantize_rows(w)
+    with pytest.raises(RuntimeError, match="not implemented"):
+        scale.sum().backward()
+    # quantizing what requires a gradient is fine where none is asked for
+    with torch.no_grad():
+        w8, scale = qrb200.quantize_rows(w)
+    assert not scale.requires_grad and qrb200.linear(meta(2, 8, dtype=FP8), w8, weight_scale=scale).shape == (2, 4)

@@ -125,3 +125,16 @@ def test_the_slope_comes_with_gradients():
         assert torch.equal(y, yg) and torch.equal(slope, slope_g)
         dx, = torch.autograd.grad(yg, xg, dy)
         assert torch.equal(dx, torch.ops.qrb200.linear_backward(dy, slope_g, x, w, True, False, False)[0])
+
+
+def test_forward_mode_is_refused():
+    """On the short way from Python too."""
+    import torch.autograd.forward_ad as fw
+    x, w = rnd(5, 64, dtype=BF, seed=1), rnd(40, 64, dtype=BF, seed=2)
+    with fw.dual_level():
+        d = fw.make_dual(x, x)
+        for call in (lambda: q().rms_norm(d), lambda: q().linear(d, w), lambda: q().rms_norm(x, residual=d, out_dtype=FP8),
+                     lambda: q().quantize_rows(d)):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(q().linear(x, w), q().linear(x.clone(), w))
