@@ -46,6 +46,13 @@ class _Ops:
         cls.loaded = True
 
 
+def _load():
+    _Ops.load()
+
+
+_load._dynamo_marked_constant = True  # run, not traced, where the first call is in a compiled program
+
+
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
              eps: float = 1e-6, out_dtype: torch.dtype | None = None):
     """``h = x + residual``; ``y = h * (mean(h**2, -1) + eps)**-0.5 * weight``.
@@ -57,7 +64,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
     ``scale`` is float32, one a row, ``max(max|y| / 448, 2**-126)``, and ``y * scale[..., None]`` the value.
     """
     if not _Ops.loaded:
-        _Ops.load()
+        _load()
     if not torch.compiler.is_compiling():
         got = _Ops.fast_rms_norm(x, weight, residual, eps, out_dtype)
         if got is not NotImplemented:
@@ -73,7 +80,7 @@ def quantize_rows(x: torch.Tensor):
     :func:`rms_norm`'s rule: returns ``(q, scale)``.  For a weight ``(n, k)`` that is one scale per
     output feature."""
     if not _Ops.loaded:
-        _Ops.load()
+        _load()
     return _Ops.quantize_rows(x)
 
 
@@ -90,7 +97,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     ``weight_scale`` (one, or one an output feature).  Sums are float32; the result is rounded once.
     """
     if not _Ops.loaded:
-        _Ops.load()
+        _load()
     try:
         act = _ACTIVATIONS[activation]
     except (KeyError, TypeError):

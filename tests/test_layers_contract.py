@@ -1,6 +1,9 @@
 """CPU: what the layer operators promise about workspaces, sizes, dispatch and derivatives; nothing here
 reaches a GPU (calls of the C ABI return before any CUDA call)."""
 import ctypes
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -158,6 +161,18 @@ def test_the_slope_comes_with_gradients():
         x = meta(2, 8).requires_grad_(grad)
         assert torch.ops.qrb200.linear(x, w, None, None, _lib.ACT_NONE, None, None, None, True)[1] is not None
         assert torch.ops.qrb200.linear(x, w, None, None, _lib.ACT_SILU, None, None, None, False)[1] is None
+
+
+def test_the_first_call_may_be_a_compiled_one():
+    """The libraries are loaded while a whole-program graph is traced; in a process of its own, where nothing has been."""
+    code = """if True:
+        import torch, qrb200
+        x, w = (torch.empty(*s, dtype=torch.bfloat16, device="meta") for s in ((2, 8), (4, 8)))
+        step = torch.compile(lambda x, w: qrb200.quantize_rows(qrb200.linear(qrb200.rms_norm(x), w))[1], backend="aot_eager", fullgraph=True)
+        assert step(x, w).shape == (2,)
+        """
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(qrb200.__file__).resolve().parents[1], capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 # ---------------------------------------------------------------------- derivatives there are not
