@@ -53,6 +53,20 @@ def _load():
 _load._dynamo_marked_constant = True  # run, not traced, where the first call is in a compiled program
 
 
+def _check(what, optional=(), eps=0.0, out_dtype=None):
+    """Kinds of arguments that the registry would refuse with a RuntimeError."""
+    for name, t in what:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"qrb200: {name} must be a tensor, got {type(t).__name__}")
+    for name, t in optional:
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise TypeError(f"qrb200: {name} must be a tensor or None, got {type(t).__name__}")
+    if not isinstance(eps, (float, int)) and not hasattr(eps, "__float__"):
+        raise TypeError(f"qrb200: eps must be a number, got {type(eps).__name__}")
+    if out_dtype is not None and not isinstance(out_dtype, torch.dtype):
+        raise TypeError(f"qrb200: out_dtype must be a torch.dtype or None, got {type(out_dtype).__name__}")
+
+
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
              eps: float = 1e-6, out_dtype: torch.dtype | None = None):
     """``h = x + residual``; ``y = h * (mean(h**2, -1) + eps)**-0.5 * weight``.
@@ -69,6 +83,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
         got = _Ops.fast_rms_norm(x, weight, residual, eps, out_dtype)
         if got is not NotImplemented:
             return got
+    _check((("x", x),), (("weight", weight), ("residual", residual)), eps, out_dtype)
     y, scale, h = _Ops.rms_norm(x, weight, residual, eps, out_dtype)
     if scale is None:
         return y if h is None else (y, h)
@@ -81,6 +96,7 @@ def quantize_rows(x: torch.Tensor):
     output feature."""
     if not _Ops.loaded:
         _load()
+    _check((("x", x),))
     return _Ops.quantize_rows(x)
 
 
@@ -106,4 +122,6 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         got = _Ops.fast_linear(x, weight, bias, residual, act, x_scale, weight_scale, out_dtype)
         if got is not NotImplemented:
             return got
+    _check((("x", x), ("weight", weight)), (("bias", bias), ("residual", residual), ("x_scale", x_scale),
+                                            ("weight_scale", weight_scale)), out_dtype=out_dtype)
     return _Ops.linear(x, weight, bias, residual, act, x_scale, weight_scale, out_dtype, False)[0]

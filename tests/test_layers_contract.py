@@ -228,3 +228,28 @@ def test_gradients_of_8_bits_are_refused():
     with torch.no_grad():
         w8, scale = qrb200.quantize_rows(w)
     assert not scale.requires_grad and qrb200.linear(meta(2, 8, dtype=FP8), w8, weight_scale=scale).shape == (2, 4)
+
+
+# ---------------------------------------------------------------------- arguments of the wrong kind
+
+@pytest.mark.parametrize("call", [
+    lambda: qrb200.rms_norm([1.0, 2.0]),
+    lambda: qrb200.rms_norm(None),
+    lambda: qrb200.rms_norm(meta(2, 8), weight=1.0),
+    lambda: qrb200.rms_norm(meta(2, 8), residual=[0.0]),
+    lambda: qrb200.rms_norm(meta(2, 8), eps="1e-6"),
+    lambda: qrb200.rms_norm(meta(2, 8), eps=None),
+    lambda: qrb200.rms_norm(meta(2, 8), out_dtype="bf16"),
+    lambda: qrb200.quantize_rows([1.0, 2.0]),
+    lambda: qrb200.quantize_rows(None),
+    lambda: qrb200.linear(meta(2, 8), None),
+    lambda: qrb200.linear(None, meta(4, 8)),
+    lambda: qrb200.linear(meta(2, 8), meta(4, 8), 1.0),
+    lambda: qrb200.linear(meta(2, 8), meta(4, 8), residual=0),
+    lambda: qrb200.linear(meta(2, 8), meta(4, 8), out_dtype="bf16"),
+    lambda: qrb200.linear(meta(2, 8, dtype=FP8), meta(4, 8, dtype=FP8), x_scale=0.5),
+])
+def test_arguments_of_another_kind(call):
+    """TypeError, as the documentation says, and not the operator registry's RuntimeError."""
+    with pytest.raises(TypeError):
+        call()
