@@ -103,7 +103,8 @@ int qrb200_linear_backward(const void* dy, int64_t lddy, const uint16_t* slope, 
                            int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* *timed_out = 1 if a bounded in-kernel wait of a layer operator has run out on the current device
- * since the last call (never expected; the outputs it concerned are NaN).  Synchronises. */
+ * since the last call (never expected; the outputs it concerned are NaN).  Waits for all work of the
+ * device, on any stream; not while one of its streams is being captured. */
 int qrb200_layer_status(int32_t* timed_out);
 
 #ifdef __cplusplus

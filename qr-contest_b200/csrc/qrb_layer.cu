@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 #include <utility>
 
 namespace qrb {
@@ -696,9 +697,16 @@ int qrb200_linear_backward(const void* dy, int64_t lddy, const uint16_t* slope, 
 
 int qrb200_layer_status(int32_t* timed_out) {
   if (!timed_out) return QRB200_ERR_INVALID_ARG;
-  int v = 0, zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, lin::g_timeout, sizeof(v));
-  if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(lin::g_timeout, &zero, sizeof(zero));
+  static std::mutex one;  // calls share g_taken
+  const std::lock_guard<std::mutex> lock(one);
+  int v = 0;
+  // all streams: a copy on the default one does not wait for those made without its blocking
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) {
+    lin::take_timeout<<<1, 1>>>();
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, lin::g_taken, sizeof(v));
   *timed_out = v;
   return note(e) == cudaSuccess ? QRB200_OK : QRB200_ERR_CUDA;
 }

@@ -29,6 +29,9 @@ enum Activation : int { ACT_NONE = 0, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SIL
 
 // Raised by a kernel whose bounded wait ran out; its tile is then filled with NaN.
 __device__ int g_timeout;
+// Takes it for the host in one step: what another stream raises meanwhile stays for the next time.
+__device__ int g_taken;
+__global__ void take_timeout() { g_taken = atomicExch(&g_timeout, 0); }
 
 struct Epilogue {
   const float* row_scale;  // p (null: 1)

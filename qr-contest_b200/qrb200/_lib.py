@@ -227,7 +227,7 @@ def set_closure_dual_n(n_max: int) -> None:
 
 def layer_timed_out() -> bool:
     """Whether a bounded wait of a layer operator has run out on the current device since the last
-    call (its outputs are NaN then).  Synchronises."""
+    call (its outputs are NaN then).  Waits for all work of the device, on any stream."""
     v = ctypes.c_int32(0)
     rc = lib().qrb200_layer_status(ctypes.byref(v))
     if rc != QRB200_OK:

@@ -138,3 +138,17 @@ def test_forward_mode_is_refused():
             with pytest.raises(NotImplementedError):
                 call()
         assert torch.equal(q().linear(x, w), q().linear(x.clone(), w))
+
+
+# ---------------------------------------------------------------------- waits
+
+def test_status_waits_for_every_stream():
+    """Torch's side streams do not block the default one, and what still runs there has not reported yet."""
+    from qrb200 import _lib
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    _lib.layer_timed_out()  # whatever a first call takes longer for
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # cycles: 0.1 s
+        done.record()
+    assert not _lib.layer_timed_out()
+    assert done.query()
