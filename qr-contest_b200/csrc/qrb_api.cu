@@ -323,7 +323,7 @@ static cudaError_t set_common_attrs() {
 // allocation-free scratch address, the host-path staging buffers) are keyed on it as well as
 // on the device index: after cudaDeviceReset the primary context is created again, module
 // globals may move, and streams and allocations of the old context are gone.
-static cudaError_t current_ctx(int* dev_out, unsigned long long* id_out) {
+cudaError_t current_ctx(int* dev_out, unsigned long long* id_out) {
   using GetCur = CUresult (*)(CUcontext*);
   using GetId = CUresult (*)(CUcontext, unsigned long long*);
   static GetCur get_cur = nullptr;

@@ -37,14 +37,17 @@ int launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_
   return launch_as(kernel, grid, block, smem, st, 0, true, std::forward<A>(args)...);
 }
 
-// Lets a kernel use `bytes` of dynamic shared memory, once per device (`ready`: the devices done).
-int raise_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready) {
+// Lets a kernel use `bytes` of dynamic shared memory, once per context (`ready`: each device's context
+// that it is done for).
+using Ready = std::atomic<unsigned long long>[128];
+int raise_smem(const void* kernel, int bytes, Ready& ready) {
   int dev = 0;
-  if (note(cudaGetDevice(&dev)) != cudaSuccess) return QRB200_ERR_CUDA;
-  if (ready.load(std::memory_order_relaxed) >> (dev & 63) & 1) return QRB200_OK;
+  unsigned long long ctx = 0;
+  if (note(current_ctx(&dev, &ctx)) != cudaSuccess) return QRB200_ERR_CUDA;
+  if (ready[dev].load(std::memory_order_relaxed) == ctx) return QRB200_OK;
   if (note(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) != cudaSuccess)
     return QRB200_ERR_CUDA;
-  if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  ready[dev].store(ctx, std::memory_order_relaxed);
   return QRB200_OK;
 }
 
@@ -168,7 +171,7 @@ BwdPlan bwd_plan(int64_t rows, int dim, int es, int hs, bool vec) {
 template <typename TX, typename TH, typename TW, int VPT, int NT>
 int launch_bwd_as(const norm::BwdArgs& a, const BwdPlan& p, cudaStream_t st) {
   auto kernel = norm::bwd_kernel<TX, TH, TW, VPT, NT>;
-  static std::atomic<uint64_t> ready{0};
+  static Ready ready;
   if (const int rc = raise_smem(reinterpret_cast<const void*>(kernel), kBwdRing, ready)) return rc;
   return launch(kernel, (unsigned)p.grid, dim3(p.s.nt, p.s.rows), p.smem, st, a, p.depth);
 }
@@ -264,7 +267,7 @@ template <typename Out, int ES, int T, bool SLOPE, int RINGS>
 int launch_tile_as(const lin::Maps& maps, const lin::Args& a, cudaStream_t st) {
   auto kernel = lin::tile_kernel<Out, ES, T, SLOPE, RINGS>;
   using C = lin::TileCfg<T, RINGS>;
-  static std::atomic<uint64_t> ready{0};
+  static Ready ready;
   if (const int rc = raise_smem(reinterpret_cast<const void*>(kernel), C::SMEM, ready)) return rc;
   const dim3 grid((unsigned)a.splits, (unsigned)((a.n + 127) / 128), (unsigned)((a.m + T - 1) / T));
   return launch_as(kernel, grid, lin::kTileThreads, C::SMEM, st, (unsigned)a.splits, true, maps, a);
@@ -303,7 +306,7 @@ int launch_pair(const Operand& P, const Operand& Q, int64_t m, int64_t n, int64_
                 const lin::Epilogue& e, cudaStream_t st) {
   auto kernel = lin::pair_kernel<Out, ES, TN, SLOPE>;
   using C = lin::PairCfg<TN>;
-  static std::atomic<uint64_t> ready{0};
+  static Ready ready;
   if (const int rc = raise_smem(reinterpret_cast<const void*>(kernel), C::SMEM, ready)) return rc;
   lin::PairMaps maps{};
   lin::PairArgs a{};

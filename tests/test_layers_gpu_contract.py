@@ -152,3 +152,56 @@ def test_status_waits_for_every_stream():
         done.record()
     assert not _lib.layer_timed_out()
     assert done.query()
+
+
+# ---------------------------------------------------------------------- contexts
+
+IN_TWO_CONTEXTS = """if True:
+    # each kernel that asks for more than 48 KB of shared memory, before and after the context is made again
+    import ctypes, numpy, torch
+    from qrb200 import _lib
+    L, rt = _lib.lib(), ctypes.CDLL("libcudart.so.12")
+    rng = numpy.random.default_rng(1)
+
+    def check(rc):
+        assert rc == 0, (rc, L.qrb200_last_cuda_error())
+
+    def bf16(*shape):
+        return (rng.standard_normal(shape, numpy.float32).view(numpy.uint32) >> 16).astype(numpy.uint16)
+
+    class Array:
+        def __init__(self, host):
+            self.host, self.p = host, ctypes.c_void_p()
+            check(rt.cudaMalloc(ctypes.byref(self.p), ctypes.c_size_t(host.nbytes)))
+            check(rt.cudaMemcpy(self.p, host.ctypes.data_as(ctypes.c_void_p), ctypes.c_size_t(host.nbytes), 1))
+
+        def back(self):
+            check(rt.cudaDeviceSynchronize())
+            out = numpy.empty_like(self.host)
+            check(rt.cudaMemcpy(out.ctypes.data_as(ctypes.c_void_p), self.p, ctypes.c_size_t(out.nbytes), 2))
+            return out
+    m, n, k = 300, 256, 256
+    hosts = [bf16(m, k), bf16(n, k), bf16(k), bf16(5000, k), bf16(4096, k)]
+
+    def run():
+        x, w, gain, many, wide = map(Array, hosts)
+        y, u, dx, dw = (Array(numpy.zeros(s, numpy.uint16)) for s in ((m, n), (5000, 4096), (m, k), (k,)))
+        check(L.qrb200_linear(x.p, k, w.p, k, 0, None, None, None, None, 0, y.p, n, None, m, n, k, 1, 1, 0, None, 0, None))
+        check(L.qrb200_linear(many.p, k, wide.p, k, 0, None, None, None, None, 0, u.p, 4096, None, 5000, 4096, k, 1, 1, 0, None, 0, None))
+        check(L.qrb200_rms_norm_backward(x.p, k, x.p, k, None, 0, gain.p, 1, dx.p, None, dw.p, m, k, 1e-6, 1, 1, None, 0, None))
+        return [t.back() for t in (y, u, dx, dw)]
+    first = run()
+    check(rt.cudaDeviceReset())
+    second = run()
+    assert all(numpy.array_equal(a, b) and a.any() for a, b in zip(first, second))
+    """
+
+
+def test_a_context_that_is_made_again():
+    """In a process of its own: what the library remembers of a context goes with it."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    done = subprocess.run([sys.executable, "-c", IN_TWO_CONTEXTS], cwd=Path(q().__file__).resolve().parents[1], capture_output=True,
+                          text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
