@@ -27,6 +27,13 @@ namespace lin {
 
 enum Activation : int { ACT_NONE = 0, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU, ACT_COUNT };
 
+// Bounded wait; false when it ran out.  The limit is that of the factorization's tiles; a library of its own,
+// for a test, is built with waits that run out at once.
+#ifndef QRB_LAYER_WAIT_LIMIT
+#define QRB_LAYER_WAIT_LIMIT tc::kSpinLimit
+#endif
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t phase) { return tc::mbar_wait_n(bar, phase, QRB_LAYER_WAIT_LIMIT); }
+
 // Raised by a kernel whose bounded wait ran out; its tile is then filled with NaN.
 __device__ int g_timeout;
 // Takes it for the host in one step: what another stream raises meanwhile stays for the next time.
@@ -385,7 +392,7 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
       int s = 0;
       uint32_t phase = 0;  // of the wait for the slot's last use
       for (int t = C::STAGES; t < nk && ok; ++t) {
-        ok = tc::mbar_wait(&empty[s], phase);
+        ok = wait(&empty[s], phase);
         if (ok) {
           if (warp == 8) load_q(t, s);
           else load_p(t, s);
@@ -405,7 +412,7 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
       int s = 0;
       uint32_t phase = 0;
       for (int t = 0; t < nk; ++t) {
-        ok = tc::mbar_wait(&full[s], phase);
+        ok = wait(&full[s], phase);
         if (!ok) break;
         tc::tc_fence_after();
         uint64_t dq = q0 + (uint64_t)(s * (C::STAGE >> 4)), dp = p0 + (uint64_t)(s * (C::STAGE >> 4));
@@ -437,9 +444,9 @@ __global__ void __launch_bounds__(kTileThreads, RINGS)
           asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const Out*>(e.res) + (int64_t)i * e.ldr + c));
       }
     }
-    bool ok = nk == 0 || tc::mbar_wait(&done, 0);
+    bool ok = nk == 0 || wait(&done, 0);
     allow_next();
-    if (!ok) atomicExch(&g_timeout, 1);
+    if (!ok) give_up();  // loads in flight land where the sums' places are
     ok = __all_sync(0xffffffffu, ok);
     tc::tc_fence_after();
     // float32 sums to shared memory as acc[i][j]: a warp's 32 lanes are 32 adjacent j

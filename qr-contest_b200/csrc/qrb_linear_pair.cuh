@@ -198,7 +198,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         place(t, ti, tj);
         const int r0 = is_p ? ti * kPairM + 128 * (int)rank : tj * TN + TN / 2 * (int)rank;
         for (int kb = 0, k0 = 0; kb < nk; ++kb, k0 += BKE) {
-          if (!first && !tc::mbar_wait(&empty[s], phase)) { ok = false; break; }
+          if (!first && !lin::wait(&empty[s], phase)) { ok = false; break; }
           if (is_p && rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
           const uint32_t to = base + s * C::STAGE, bar = full0 + 8 * s;
           if (by_rows) {
@@ -224,10 +224,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       uint32_t phase = 0;
       for (int t = pair; t < tiles && ok; t += pairs, ++turn) {
         const int b = turn & 1;
-        if (turn >= 2 && !tc::mbar_wait(&acc_empty[b], ((turn >> 1) - 1) & 1)) { ok = false; break; }
+        if (turn >= 2 && !lin::wait(&acc_empty[b], ((turn >> 1) - 1) & 1)) { ok = false; break; }
         tc::tc_fence_after();
         for (int kb = 0; kb < nk; ++kb) {
-          if (!tc::mbar_wait(&full[s], phase)) { ok = false; break; }
+          if (!lin::wait(&full[s], phase)) { ok = false; break; }
           tc::tc_fence_after();
           uint64_t dp = p0 + (uint64_t)(s * (C::STAGE >> 4)), dq = q0 + (uint64_t)(s * (C::STAGE >> 4));
 #pragma unroll
@@ -270,7 +270,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
         tc::fence_async_smem();  // this warp's own accesses to the block, before a load overwrites it
         __syncwarp();
-        if (e.res && live) {
+        const bool fetch = e.res && live && ok;
+        if (fetch) {
           if (a.tma_res) {
             if (lane == 0) {
               mbar_expect_tx(&res_bar[warp], 4096);
@@ -288,13 +289,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           cscale[h] = ES == 1 && e.col_scale && j < a.n ? e.col_scale[j] : 1.f;
         }
         if (!waited) {
-          if (ok && !tc::mbar_wait(&acc_full[b], (turn >> 1) & 1)) ok = false;
+          if (ok && !lin::wait(&acc_full[b], (turn >> 1) & 1)) ok = false;
           tc::tc_fence_after();
           waited = true;
           if (t + pairs >= tiles) allow_next();  // this CTA's last sums
         }
-        if (e.res && live && a.tma_res) {
-          if (ok && !tc::mbar_wait(&res_bar[warp], res_phase)) ok = false;
+        if (fetch && a.tma_res) {  // also where the sums have not come: it lands in the block
+          if (!lin::wait(&res_bar[warp], res_phase)) {
+            ok = false;
+            give_up();
+          }
           res_phase ^= 1;
         }
         ok = __all_sync(0xffffffffu, ok);

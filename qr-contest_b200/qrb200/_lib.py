@@ -13,6 +13,8 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libqrb200.so"
 # the same library built with -DQRB_BOUNDS_CHECK (pivot-map indices checked, INFO_BOUNDS)
 CHECKED_LIB_PATH = Path(__file__).resolve().parent / "libqrb200_checked.so"
+# the same library with layer operators whose bounded waits run out at once (-DQRB_LAYER_WAIT_LIMIT=0)
+NOWAIT_LIB_PATH = Path(__file__).resolve().parent / "libqrb200_nowait.so"
 
 QRB200_OK = 0
 QRB200_ERR_INVALID_ARG = 1

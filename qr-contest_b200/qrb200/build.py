@@ -21,6 +21,7 @@ INCLUDE = ROOT.parent / "include"
 LIB = PKG / "libqrb200.so"
 TESTKIT = PKG / "libqrb200_testkit.so"   # single-stage entry points for the GPU unit tests
 CHECKED = PKG / "libqrb200_checked.so"   # the library with the pivot-map bounds checks
+NOWAIT = PKG / "libqrb200_nowait.so"     # the layer operators with bounded waits that run out at once
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
@@ -45,7 +46,7 @@ OBJ = ROOT / "build"                   # objects and their dependency files (git
 
 
 def _object(src: Path, defs) -> Path:
-    return OBJ / (src.stem + "".join(d.replace("-D", "-") for d in defs) + ".o")
+    return OBJ / (src.stem + "".join(d.replace("-D", "-").replace("=", "-") for d in defs) + ".o")
 
 
 def _inputs(obj: Path):
@@ -113,7 +114,8 @@ def _compile_py(verbose: bool) -> None:
 _CHECK = ["-DQRB_BOUNDS_CHECK"]
 _LINKS = ((LIB, [("qrb_api.cu", []), ("qrb_layer.cu", [])]),
           (CHECKED, [("qrb_api.cu", _CHECK), ("qrb_layer.cu", [])]),
-          (TESTKIT, [("qrb_testkit.cu", ["-DQRB_PANEL_TIMERS"])]))
+          (TESTKIT, [("qrb_testkit.cu", ["-DQRB_PANEL_TIMERS"])]),
+          (NOWAIT, [("qrb_api.cu", []), ("qrb_layer.cu", ["-DQRB_LAYER_WAIT_LIMIT=0"])]))
 
 
 def build(force: bool = False, verbose: bool = False, extra=()) -> Path:

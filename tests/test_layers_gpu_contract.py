@@ -205,3 +205,36 @@ def test_a_context_that_is_made_again():
     done = subprocess.run([sys.executable, "-c", IN_TWO_CONTEXTS], cwd=Path(q().__file__).resolve().parents[1], capture_output=True,
                           text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+# ---------------------------------------------------------------------- waits that run out
+
+@pytest.fixture(scope="module")
+def nowait():
+    """The library whose bounded waits run out at once: no kernel of it waits for anything, none fails otherwise."""
+    from qrb200 import _lib
+    h = ctypes.CDLL(str(_lib.NOWAIT_LIB_PATH))
+    for name, (res, args) in _lib.SIGNATURES.items():
+        fn = getattr(h, name)
+        fn.restype, fn.argtypes = res, args
+    return h
+
+
+# one CTA a tile; a cluster of several; the persistent pairs, with and without rows that TMA can address
+@pytest.mark.parametrize("m,n,k", [(40, 20000, 64), (16, 256, 4096), (2048, 2048, 256), (2048, 2049, 256), (300, 520, 4096)])
+@pytest.mark.parametrize("residual,slope", [(False, False), (True, False), (True, True)])
+def test_waits_that_run_out_are_reported(nowait, m, n, k, residual, slope):
+    """The call returns, the flag is up and every output is NaN; the flag comes down, and the context works on."""
+    from qrb200 import _lib
+    x, w = rnd(m, k, dtype=BF, seed=1), rnd(n, k, dtype=BF, seed=2)
+    r, y = rnd(m, n, dtype=BF, seed=3), torch.zeros(m, n, dtype=BF, device="cuda")
+    s = torch.zeros(m, n, dtype=torch.int16, device="cuda")
+    timed_out = ctypes.c_int32(-1)
+    assert nowait.qrb200_layer_status(ctypes.byref(timed_out)) == _lib.QRB200_OK and timed_out.value == 0
+    assert nowait.qrb200_linear(x.data_ptr(), k, w.data_ptr(), k, 0, None, None, None, r.data_ptr() if residual else None, n, y.data_ptr(), n,
+                                s.data_ptr() if slope else None, m, n, k, 1, 1, _lib.ACT_GELU, None, 0, stream()) == _lib.QRB200_OK
+    assert nowait.qrb200_layer_status(ctypes.byref(timed_out)) == _lib.QRB200_OK and timed_out.value == 1
+    assert bool(torch.isnan(y).all())
+    assert not slope or bool((s == -1).all())  # 65535: NaN
+    assert nowait.qrb200_layer_status(ctypes.byref(timed_out)) == _lib.QRB200_OK and timed_out.value == 0
+    assert bool(torch.isfinite(q().linear(x, w, residual=r)).all()) and not _lib.layer_timed_out()
