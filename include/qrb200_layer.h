@@ -6,7 +6,8 @@
  * rows apart on outputs; inputs may overlap or repeat, ld = 0 included, except matrix-product
  * operands) and contiguous inside; bases and strides need no alignment but their elements'.  A
  * workspace may start at any byte: the queried sizes allow for that.  Everything is
- * enqueued on `stream`; nothing is synchronised.  Empty sizes are a successful no-op.
+ * enqueued on `stream`; nothing is synchronised.  Empty sizes are a successful no-op
+ * (but rows of no elements have their scale written).
  *
  * Status codes, element types and the conventions of qrb200.h; nothing here depends on PyTorch or
  * on the CUDA headers. */

@@ -134,6 +134,14 @@ int launch_norm(const norm::FwdArgs& a, bool q8, bool stream_f32, bool vec, cuda
   return q8 ? launch_fwd<TX, TX, true, true, true>(a, vec, st) : launch_fwd<TX, TX, true, false, true>(a, vec, st);
 }
 
+// Rows of no elements have a scale all the same.
+int scales_of_empty_rows(float* scale, int64_t rows, void* stream) {
+  if (!rows || !scale) return QRB200_OK;
+  if (rows >= ((int64_t)1 << 31)) return QRB200_ERR_INVALID_ARG;
+  const norm::FwdArgs a{nullptr, 0, nullptr, 0, nullptr, 0, nullptr, scale, nullptr, rows, 0, 0.f};
+  return launch_fwd<float, float, false, true, false>(a, true, static_cast<cudaStream_t>(stream));
+}
+
 // Shape, rows of look-ahead and grid of the backward kernel; parts = rows of partial weight gradients
 // it writes, one a block.  A block walks over its rows, so the grid is what the GPU holds at once: 128
 // registers a thread (64 for rows of single elements up to 4096, which have no look-ahead and need
@@ -506,7 +514,7 @@ int qrb200_rms_norm(const void* x, int64_t ldx, const void* weight, int32_t weig
     return QRB200_ERR_INVALID_ARG;
   if (weight && !(weight_dtype == dtype || weight_dtype == QRB200_F32)) return QRB200_ERR_INVALID_ARG;
   if (residual && !(stream_dtype == dtype || stream_dtype == QRB200_F32)) return QRB200_ERR_INVALID_ARG;
-  if (rows == 0 || dim == 0) return QRB200_OK;
+  if (rows == 0 || dim == 0) return q8 ? scales_of_empty_rows(scale, rows, stream) : QRB200_OK;
   if (!x || !y || (q8 && !scale) || (residual && !h)) return QRB200_ERR_INVALID_ARG;
   if (rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30) || ldx < 0 || (residual && ldr < 0))
     return QRB200_ERR_INVALID_ARG;
@@ -524,7 +532,7 @@ int qrb200_rms_norm(const void* x, int64_t ldx, const void* weight, int32_t weig
 int qrb200_quantize_rows(const void* x, int64_t ldx, void* q, float* scale, int64_t rows, int64_t dim, int32_t dtype,
                          void* stream) {
   if (!float_type(dtype) || rows < 0 || dim < 0) return QRB200_ERR_INVALID_ARG;
-  if (rows == 0 || dim == 0) return QRB200_OK;
+  if (rows == 0 || dim == 0) return scales_of_empty_rows(scale, rows, stream);
   if (!x || !q || !scale || rows >= ((int64_t)1 << 31) || dim >= ((int64_t)1 << 30) || ldx < 0)
     return QRB200_ERR_INVALID_ARG;
   norm::FwdArgs a{x, ldx, nullptr, 0, nullptr, 0, q, scale, nullptr, rows, (int)dim, 0.f};

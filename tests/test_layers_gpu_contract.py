@@ -238,3 +238,21 @@ def test_waits_that_run_out_are_reported(nowait, m, n, k, residual, slope):
     assert not slope or bool((s == -1).all())  # 65535: NaN
     assert nowait.qrb200_layer_status(ctypes.byref(timed_out)) == _lib.QRB200_OK and timed_out.value == 0
     assert bool(torch.isfinite(q().linear(x, w, residual=r)).all()) and not _lib.layer_timed_out()
+
+
+# ---------------------------------------------------------------------- the ends of the ranges
+
+def test_scales_of_empty_rows():
+    """The largest of no elements is 0, so the scale is the smallest one, 2^-126, and not what was there."""
+    import ctypes
+    from qrb200 import _lib
+    L = _lib.lib()
+    for rows in (1, 5, 1000):
+        for call in (lambda s: L.qrb200_quantize_rows(None, 0, None, s, rows, 0, _lib.QRB200_BF16, stream()),
+                     lambda s: L.qrb200_rms_norm(None, 0, None, 0, None, 0, 0, None, s, None, rows, 0, 1e-6, _lib.QRB200_F32, _lib.QRB200_E4M3,
+                                                 stream())):
+            scale = torch.full((rows + 1,), 7.0, device="cuda")
+            assert call(ctypes.c_void_p(scale.data_ptr())) == _lib.QRB200_OK
+            assert bool((scale[:rows] == 2.0 ** -126).all()) and float(scale[rows]) == 7.0
+    y, s = q().quantize_rows(torch.empty(3, 4, 0, dtype=BF, device="cuda"))
+    assert y.shape == (3, 4, 0) and s.shape == (3, 4) and bool((s == 2.0 ** -126).all())
