@@ -256,3 +256,22 @@ def test_scales_of_empty_rows():
             assert bool((scale[:rows] == 2.0 ** -126).all()) and float(scale[rows]) == 7.0
     y, s = q().quantize_rows(torch.empty(3, 4, 0, dtype=BF, device="cuda"))
     assert y.shape == (3, 4, 0) and s.shape == (3, 4) and bool((s == 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize("gain", [1e-16, 1e15])
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("rows,dim", [(300, 64), (5, 4096), (300, 65), (2, 3001), (3, 20000)])
+def test_norm_gradient_of_tiny_and_huge_rows(rows, dim, dtype, gain):
+    """eps = 0 and rows of about 1e-16 or 1e15: the cube of the root's inverse leaves float32, the gradient does not.
+    Sums of float32 against their magnitudes: 2^-17 as for ordinary rows (squares and their sums are normal numbers)."""
+    x = rnd(rows, dim, dtype=dtype, seed=1, gain=gain).requires_grad_()
+    w, dy = (rnd(dim, dtype=dtype, seed=2) + 1).requires_grad_(), rnd(rows, dim, dtype=dtype, seed=3)
+    dx, dw = torch.autograd.grad(q().rms_norm(x, w, eps=0.0), (x, w), dy)
+    h, g = x.detach().double(), dy.double() * w.detach().double()
+    r = h.square().mean(-1, keepdim=True).rsqrt()
+    want = r * g - r ** 3 * (g * h).mean(-1, keepdim=True) * h
+    size = (r * g).abs() + r ** 3 * (g * h).abs().mean(-1, keepdim=True) * h.abs()
+    u = {F32: 2.0 ** -24, BF: 2.0 ** -8}[dtype]
+    assert bool(((dx.double() - want).abs() <= u * (1 + 2 ** -10) * want.abs() + 2.0 ** -17 * size).all())
+    terms = dy.double() * h * r
+    assert bool(((dw.double() - terms.sum(0)).abs() <= u * (1 + 2 ** -10) * terms.sum(0).abs() + 2.0 ** -16 * terms.abs().sum(0)).all())
