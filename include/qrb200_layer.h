@@ -76,7 +76,7 @@ int qrb200_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_
  *   bias     [n], residual [m][n], y [m][n]: `out_dtype` (= `dtype`; BF16 or F16 for E4M3);
  *            residual may be y itself (in place)
  *   slope    [m][n] contiguous, or NULL: act'(z) for qrb200_linear_backward as
- *            round(2^15 (act' + 1/4)), 65535 for NaN; not for E4M3
+ *            round(2^15 (t + 3/8)) with act' = t |t|, 65535 for NaN; not for E4M3
  * m and n up to 8388480 (128 * 65535), k up to 2^31 - 65537.  Sums are float32; y is rounded once.
  * `workspace` (NULL: allocated stream-ordered) holds aligned copies of operands whose rows do not
  * all start on 16 bytes; none is needed otherwise. */

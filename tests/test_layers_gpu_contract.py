@@ -275,3 +275,32 @@ def test_norm_gradient_of_tiny_and_huge_rows(rows, dim, dtype, gain):
     assert bool(((dx.double() - want).abs() <= u * (1 + 2 ** -10) * want.abs() + 2.0 ** -17 * size).all())
     terms = dy.double() * h * r
     assert bool(((dw.double() - terms.sum(0)).abs() <= u * (1 + 2 ** -10) * terms.sum(0).abs() + 2.0 ** -16 * terms.abs().sum(0)).all())
+
+
+# ---------------------------------------------------------------------- gradients in an activation's tail
+
+@pytest.mark.parametrize("m", [40, 512, 6000])
+@pytest.mark.parametrize("act,bias", [("gelu", -3.0), ("gelu", -4.0), ("gelu", -5.0), ("gelu_tanh", -4.0), ("silu", -10.0), ("silu", -14.0)])
+def test_gradients_in_a_tail(act, bias, m):
+    """Features whose z all lie where act' is small still learn.  act' is held as its root in steps of 2^-15, so it is
+    off by 2 |act'|^(1/2) 2^-16 + 2^-32, and by 2^-9 of itself through the formula's approximations out there; dz is
+    rounded to bf16 (u = 2^-8) for dw and dx, not for db; sums are added as in any product."""
+    n, k, u = 16, 64, 2.0 ** -8
+    x, w = rnd(m, k, dtype=BF, seed=1).requires_grad_(), rnd(n, k, dtype=BF, seed=2, gain=0.02).requires_grad_()
+    b = torch.full((n,), bias, dtype=BF, device="cuda").requires_grad_()
+    dy = rnd(m, n, dtype=BF, seed=3).abs()
+    dx, dw, db = torch.autograd.grad(q().linear(x, w, b, activation=act), (x, w, b), dy)
+    x64, w64, z = x.detach().double(), w.detach().double(), None
+    z = (x64 @ w64.T + bias).requires_grad_()
+    f = {"gelu": lambda t: t * torch.special.ndtr(t), "gelu_tanh": lambda t: t * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (t + 0.044715 * t ** 3)),
+         "silu": lambda t: t * torch.sigmoid(t)}[act]
+    slope, = torch.autograd.grad(f(z).sum(), z)
+    dz = dy.double() * slope
+    ddz = dy.double() * (2.0 ** -15 * slope.abs().sqrt() + 2.0 ** -32 + 2.0 ** -9 * slope.abs())
+    rdz = ddz + u * (1 + 2 ** -10) * dz.abs()
+    for got, want, err, mag, steps in ((dw, dz.T @ x64, rdz.T @ x64.abs(), dz.abs().T @ x64.abs(), m), (dx, dz @ w64, rdz @ w64.abs(), dz.abs() @ w64.abs(), n),
+                                       (db, dz.sum(0), ddz.sum(0), dz.abs().sum(0), m)):
+        tol = u * (1 + 2 ** -10) * want.abs() + err * (1 + u) + (steps / 16 + 16) * 2.0 ** -23 * (mag + err)
+        assert bool(((got.double() - want).abs() <= tol).all())
+    # all terms of db have one sign, so its bound is one on its relative error
+    assert bool((db.double() / dz.sum(0) - 1).abs().max() < 2.0 ** -5)
