@@ -1,7 +1,6 @@
 // qrb200 -- the layer operators as C++ functions on tensors (libqrb200_torch_ops.so), with their
 // gradients, for callers that have made sure that nothing listens for operators (no dispatch mode, no
-// tensor subclass, no transform): with nothing to differentiate they do not go through the dispatcher.
-// All others call torch.ops.qrb200.*.
+// tensor subclass, no transform).  All others call torch.ops.qrb200.*.
 #pragma once
 #include <ATen/ATen.h>
 

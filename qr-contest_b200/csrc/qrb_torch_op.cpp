@@ -20,6 +20,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -355,42 +357,73 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward(const at::Tensor&
 }
 
 // ---- gradients ----
-// The operators by way of the dispatcher.  What runs below autograd is called like this and not as a
-// function, so that whatever is listening there (a dispatch mode, a fake tensor, a trace) sees the operator.
-auto& rms_norm_op() {
-  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("qrb200::rms_norm", "").typed<decltype(rms_norm)>();
-  return op;
+// The operators as they run below autograd: by way of the dispatcher where anything may be listening
+// there (a dispatch mode, a fake tensor, a trace, another device), so that it sees the operator; as plain
+// functions where nothing can: CUDA tensors of no other kind, no mode, no transform.  The dispatcher takes
+// about 1 us a call: 4 of the 77 us of a small training step, which is bound by the host.
+bool is_plain(const at::Tensor& t) {
+  constexpr c10::DispatchKeySet plain = c10::DispatchKeySet(c10::DispatchKey::CUDA) | c10::DispatchKeySet(c10::DispatchKey::AutogradCUDA) |
+                                        c10::DispatchKeySet(c10::DispatchKey::ADInplaceOrView) |
+                                        c10::DispatchKeySet(c10::DispatchKey::AutocastCUDA);
+  return !t.defined() || (t.key_set() - plain).empty();
 }
-auto& rms_norm_backward_op() {
+bool is_plain(const OptTensor& t) { return !t || is_plain(*t); }
+template <typename... T>
+bool nothing_listens(const T&... ts) {
+  return (is_plain(ts) && ...) && !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+         (c10::impl::tls_local_dispatch_key_set().included_ - c10::default_included_set).empty();
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_below(const at::Tensor& x, const OptTensor& weight, const OptTensor& residual,
+                                                              double eps, c10::optional<at::ScalarType> out_dtype) {
+  if (nothing_listens(x, weight, residual)) return rms_norm(x, weight, residual, eps, out_dtype);
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("qrb200::rms_norm", "").typed<decltype(rms_norm)>();
+  return op.call(x, weight, residual, eps, out_dtype);
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_backward_below(const at::Tensor& dy, const at::Tensor& h, const OptTensor& dh,
+                                                                       const OptTensor& weight, double eps, bool want_dx,
+                                                                       bool want_dresidual, bool want_dweight) {
+  if (nothing_listens(dy, h, dh, weight)) return rms_norm_backward(dy, h, dh, weight, eps, want_dx, want_dresidual, want_dweight);
   static const auto op =
       c10::Dispatcher::singleton().findSchemaOrThrow("qrb200::rms_norm_backward", "").typed<decltype(rms_norm_backward)>();
-  return op;
+  return op.call(dy, h, dh, weight, eps, want_dx, want_dresidual, want_dweight);
 }
-auto& linear_op() {
+std::tuple<at::Tensor, at::Tensor> linear_below(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
+                                                const OptTensor& residual, int64_t activation, const OptTensor& x_scale,
+                                                const OptTensor& weight_scale, c10::optional<at::ScalarType> out_dtype,
+                                                bool want_slope) {
+  if (nothing_listens(x, weight, bias, residual, x_scale, weight_scale))
+    return linear(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("qrb200::linear", "").typed<decltype(linear)>();
-  return op;
+  return op.call(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
 }
-auto& linear_backward_op() {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward_below(const at::Tensor& dy, const OptTensor& slope, const at::Tensor& x,
+                                                                     const at::Tensor& weight, bool want_dx, bool want_dweight,
+                                                                     bool want_dbias) {
+  if (nothing_listens(dy, slope, x, weight)) return linear_backward(dy, slope, x, weight, want_dx, want_dweight, want_dbias);
   static const auto op =
       c10::Dispatcher::singleton().findSchemaOrThrow("qrb200::linear_backward", "").typed<decltype(linear_backward)>();
-  return op;
+  return op.call(dy, slope, x, weight, want_dx, want_dweight, want_dbias);
 }
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 OptTensor given(const at::Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
-bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const at::Tensor* t : ts)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
+bool requires_grad(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
+bool requires_grad(const OptTensor& t) { return t && requires_grad(*t); }
+template <typename... T>
+bool wants_grad(const T&... ts) {
+  return at::GradMode::is_enabled() && (requires_grad(ts) || ...);
 }
 // A tangent would be lost without a word below here: it hangs on a tensor that need not require a gradient.
-void check_no_tangent(std::initializer_list<const at::Tensor*> ts) {
-  for (const at::Tensor* t : ts)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(),
-                                "qrb200: the layer operators have no forward-mode derivative");
+bool has_tangent(const at::Tensor& t) {
+  return t.defined() && t.unsafeGetTensorImpl()->autograd_meta() && t._fw_grad(/*level=*/0).defined();
+}
+bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
+template <typename... T>
+void check_no_tangent(const T&... ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(ts) || ...), "qrb200: the layer operators have no forward-mode derivative");
 }
 void check_once() {
   TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), "qrb200: the layer operators are differentiable once (no create_graph)");
@@ -401,7 +434,7 @@ struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
                                const OptTensor& residual, double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
     ctx->set_materialize_grads(false);
-    auto [y, scale, h] = rms_norm_op().call(x, weight, residual, eps, c10::nullopt);
+    auto [y, scale, h] = rms_norm_below(x, weight, residual, eps, c10::nullopt);
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["residual"] = residual.has_value();
     ctx->saved_data["type"] = x.scalar_type();
@@ -413,6 +446,7 @@ struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &h = saved[0], &weight = saved[1];
     at::Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : at::Tensor();
+    check_no_tangent(dy, dh);
     // inputs that were given, in order, have an edge each
     size_t edge = 0;
     const bool want_x = ctx->needs_input_grad(edge++);
@@ -423,21 +457,20 @@ struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
       dy = at::zeros(h.sizes(), h.options().dtype(ctx->saved_data["type"].toScalarType()));
     }
     auto [dx, dres, dw] =
-        rms_norm_backward_op().call(dy, h, given(dh), given(weight), ctx->saved_data["eps"].toDouble(), want_x, want_r, want_w);
+        rms_norm_backward_below(dy, h, given(dh), given(weight), ctx->saved_data["eps"].toDouble(), want_x, want_r, want_w);
     return {want_x ? dx : at::Tensor(), dw, dres, at::Tensor()};
   }
 };
 
-// Below autograd with nothing to differentiate; otherwise with a node that can.  LISTENED: something may
-// see operators below autograd.
-template <bool LISTENED>
+// Below autograd with nothing to differentiate; otherwise with a node that can.  PLAIN: the caller knows
+// that nothing listens.
+template <bool PLAIN>
 std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_grad(const at::Tensor& x, const OptTensor& weight, const OptTensor& residual,
                                                              double eps, c10::optional<at::ScalarType> out_dtype) {
-  const at::Tensor w = weight.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
-  check_no_tangent({&x, &w, &r});
-  if (!wants_grad({&x, &w, &r})) {
+  check_no_tangent(x, weight, residual);
+  if (!wants_grad(x, weight, residual)) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return LISTENED ? rms_norm_op().call(x, weight, residual, eps, out_dtype) : rms_norm(x, weight, residual, eps, out_dtype);
+    return PLAIN ? rms_norm(x, weight, residual, eps, out_dtype) : rms_norm_below(x, weight, residual, eps, out_dtype);
   }
   TORCH_CHECK_VALUE(!out_dtype || *out_dtype == x.scalar_type(), "qrb200: the 8-bit norm has no gradient (use torch.no_grad())");
   variable_list out = RmsNormGrad::apply(x, weight, residual, eps);
@@ -453,8 +486,8 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
     const bool sums = x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad());
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["residual"] = residual.has_value();
-    auto [y, slope] = linear_op().call(x, weight, bias, residual, activation, c10::nullopt, c10::nullopt, out_dtype,
-                                       want_slope || (sums && activation != QRB200_ACT_NONE));
+    auto [y, slope] = linear_below(x, weight, bias, residual, activation, c10::nullopt, c10::nullopt, out_dtype,
+                                   want_slope || (sums && activation != QRB200_ACT_NONE));
     if (sums) ctx->save_for_backward({x, weight, activation == QRB200_ACT_NONE ? at::Tensor() : slope});
     if (!want_slope) return {y};
     ctx->mark_non_differentiable({slope});
@@ -464,6 +497,7 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
     check_once();
     variable_list out(7);
     const at::Tensor& dy = grads[0];
+    check_no_tangent(dy);
     if (!dy.defined()) return out;
     size_t edge = 0;
     const bool want_x = ctx->needs_input_grad(edge++), want_w = ctx->needs_input_grad(edge++);
@@ -472,25 +506,23 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
     if (want_x || want_w || want_b) {
       const auto saved = ctx->get_saved_variables();
       std::tie(out[0], out[1], out[2]) =
-          linear_backward_op().call(dy, given(saved[2]), saved[0], saved[1], want_x, want_w, want_b);
+          linear_backward_below(dy, given(saved[2]), saved[0], saved[1], want_x, want_w, want_b);
     }
     if (want_r) out[3] = dy;
     return out;
   }
 };
 
-template <bool LISTENED>
+template <bool PLAIN>
 std::tuple<at::Tensor, at::Tensor> linear_grad(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
                                                const OptTensor& residual, int64_t activation, const OptTensor& x_scale,
                                                const OptTensor& weight_scale, c10::optional<at::ScalarType> out_dtype,
                                                bool want_slope) {
-  const at::Tensor b = bias.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
-  const at::Tensor xs = x_scale.value_or(at::Tensor()), ws = weight_scale.value_or(at::Tensor());
-  check_no_tangent({&x, &weight, &b, &r, &xs, &ws});
-  if (!wants_grad({&x, &weight, &b, &r})) {
+  check_no_tangent(x, weight, bias, residual, x_scale, weight_scale);
+  if (!wants_grad(x, weight, bias, residual)) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return LISTENED ? linear_op().call(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope)
-                    : linear(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
+    return PLAIN ? linear(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope)
+                 : linear_below(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
   }
   TORCH_CHECK_VALUE(x.scalar_type() != at::kFloat8_e4m3fn, "qrb200: the 8-bit product has no gradient (use torch.no_grad())");
   TORCH_CHECK_VALUE(!x_scale && !weight_scale, "qrb200: scales belong to 8-bit operands");
@@ -500,17 +532,17 @@ std::tuple<at::Tensor, at::Tensor> linear_grad(const at::Tensor& x, const at::Te
 
 }  // namespace
 
-// The short way: its callers have made sure that nothing listens.
+// The short way from Python.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> qrb200::rms_norm(const at::Tensor& x, const OptTensor& weight,
                                                                 const OptTensor& residual, double eps,
                                                                 c10::optional<at::ScalarType> out_dtype) {
-  return rms_norm_grad<false>(x, weight, residual, eps, out_dtype);
+  return rms_norm_grad<true>(x, weight, residual, eps, out_dtype);
 }
 std::tuple<at::Tensor, at::Tensor> qrb200::linear(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
                                                   const OptTensor& residual, int64_t activation, const OptTensor& x_scale,
                                                   const OptTensor& weight_scale, c10::optional<at::ScalarType> out_dtype,
                                                   bool want_slope) {
-  return linear_grad<false>(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
+  return linear_grad<true>(x, weight, bias, residual, activation, x_scale, weight_scale, out_dtype, want_slope);
 }
 
 TORCH_LIBRARY(qrb200, m) {
@@ -544,8 +576,8 @@ TORCH_LIBRARY_IMPL(qrb200, Meta, m) {
 }
 
 TORCH_LIBRARY_IMPL(qrb200, Autograd, m) {
-  m.impl("rms_norm", rms_norm_grad<true>);
-  m.impl("linear", linear_grad<true>);
+  m.impl("rms_norm", rms_norm_grad<false>);
+  m.impl("linear", linear_grad<false>);
   // no derivative of either mode: refused where one is asked for
   m.impl("quantize_rows", torch::autograd::autogradNotImplementedFallback());
   m.impl("rms_norm_backward", torch::autograd::autogradNotImplementedFallback());
