@@ -304,3 +304,44 @@ def test_gradients_in_a_tail(act, bias, m):
         assert bool(((got.double() - want).abs() <= tol).all())
     # all terms of db have one sign, so its bound is one on its relative error
     assert bool((db.double() / dz.sum(0) - 1).abs().max() < 2.0 ** -5)
+
+
+# ---------------------------------------------------------------------- strides
+
+def bits(t):
+    return t.view(torch.uint8) if t.dtype == FP8 else t
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("rows,dim", [(40, 96), (300, 96), (40, 2048), (400, 2048), (7, 16392)])
+def test_norm_of_strided_rows(rows, dim, fp8, dtype):
+    """Rows that all start on 16 bytes give the bits of their contiguous copies, whatever lies between them; so do, among
+    themselves, rows that do not, which are read one element at a time.  The stream is the same everywhere.  Between the
+    two the sums are added in another order: each y is within u + 2^-18 of the exact one (u = 2^-8, 2^-24), so two of them
+    are within twice that, and in 8 bits within twice 2^-4 of a value or 2^-10 of the scale."""
+    wide = rnd(rows, dim + 72, dtype=dtype, seed=1)
+    w, res = rnd(dim, dtype=dtype, seed=2) + 1, rnd(rows, dim, dtype=dtype, seed=3)
+    call = lambda x: q().rms_norm(x, w, residual=res, out_dtype=FP8 if fp8 else None)  # noqa: E731
+    on, off = [0, 16, 64], [1, 3, 17]  # elements
+    for starts in (on, off):
+        for c in starts:
+            x = wide[:, c:c + dim]
+            assert (x.data_ptr() % 16 == 0) == (starts is on) and not x.is_contiguous()
+            got = call(x)
+            if starts is on:
+                same = call(x.contiguous())
+            else:  # the same rows at another odd distance
+                other = torch.empty(rows, dim + 41, dtype=dtype, device="cuda")[:, 5:5 + dim]
+                same = call(other.copy_(x))
+            assert all(torch.equal(bits(a), bits(b)) for a, b in zip(got, same))
+            plain = call(x.contiguous())
+            assert torch.equal(got[-1], plain[-1])  # the stream
+            if fp8:
+                assert bool(((got[1] - plain[1]).abs() <= 2.0 ** -17 * plain[1]).all())
+                a, b, s = got[0].double() * got[1].double()[:, None], plain[0].double() * plain[1].double()[:, None], plain[1].double()[:, None]
+                tol = 2 * (torch.maximum(2.0 ** -4 * torch.maximum(a.abs(), b.abs()) * (1 + 2.0 ** -4), 2.0 ** -10 * s * (1 + 2.0 ** -12)))
+            else:
+                a, b = got[0].double(), plain[0].double()
+                tol = 2 * ({BF: 2.0 ** -8, F32: 2.0 ** -24}[dtype] + 2.0 ** -18) * (1 + 2.0 ** -7) * b.abs() + 2.0 ** -133
+            assert bool(((a - b).abs() <= tol).all())
