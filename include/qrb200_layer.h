@@ -72,7 +72,7 @@ int qrb200_rms_norm_backward(const void* dy, int64_t lddy, const void* h, int64_
  *   y = act(x_scale_i w_scale_j sum_k x_ik w_jk + bias_j) + residual_ij
  *   x        [m][k], w [n][k], `dtype` BF16, F16 or E4M3; w_transposed != 0: w is stored [k][n]
  *            (not for E4M3)
- *   x_scale  [m], w_scale [n], float32, or NULL for ones
+ *   x_scale  [m], w_scale [n], float32, or NULL for ones; for E4M3 only
  *   bias     [n], residual [m][n], y [m][n]: `out_dtype` (= `dtype`; BF16 or F16 for E4M3);
  *            residual may be y itself (in place)
  *   slope    [m][n] contiguous, or NULL: act'(z) for qrb200_linear_backward as

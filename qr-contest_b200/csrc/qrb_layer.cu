@@ -614,7 +614,7 @@ int qrb200_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_
   const bool q8 = dtype == QRB200_E4M3;
   if (!(dtype == QRB200_BF16 || dtype == QRB200_F16 || q8) || !sizes_ok(m, n, k)) return QRB200_ERR_INVALID_ARG;
   if (q8 ? !(out_dtype == QRB200_BF16 || out_dtype == QRB200_F16) : out_dtype != dtype) return QRB200_ERR_INVALID_ARG;
-  if (activation < 0 || activation >= lin::ACT_COUNT || (q8 && (w_transposed || slope))) return QRB200_ERR_INVALID_ARG;
+  if (activation < 0 || activation >= lin::ACT_COUNT || (q8 ? w_transposed || slope : x_scale || w_scale)) return QRB200_ERR_INVALID_ARG;
   if (m == 0 || n == 0) return QRB200_OK;
   if (!y || (k > 0 && (!x || !w))) return QRB200_ERR_INVALID_ARG;
   if (ldy < n || (residual && ldr < 0) || (k > 0 && (ldx < k || ldw < (w_transposed ? n : k))))

@@ -41,8 +41,8 @@ __device__ int g_taken;
 __global__ void take_timeout() { g_taken = atomicExch(&g_timeout, 0); }
 
 struct Epilogue {
-  const float* row_scale;  // p (null: 1)
-  const float* col_scale;  // q (null: 1)
+  const float* row_scale;  // p (null: 1); 8-bit operands only
+  const float* col_scale;  // q (null: 1); likewise
   const void* bias;        // b, in the output's type, or null
   const void* res;         // R, in the output's type, or null
   int64_t ldr;

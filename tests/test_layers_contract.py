@@ -253,3 +253,16 @@ def test_arguments_of_another_kind(call):
     """TypeError, as the documentation says, and not the operator registry's RuntimeError."""
     with pytest.raises(TypeError):
         call()
+
+
+# ---------------------------------------------------------------------- scales
+
+@pytest.mark.parametrize("m", [1, 2, 40, 3000])
+def test_scales_of_16_bit_operands_are_refused(m):
+    """From C as from Python: one kernel multiplied by them and the others did not."""
+    L, bad = _lib.lib(), _lib.QRB200_ERR_INVALID_ARG
+    for t in (_lib.QRB200_BF16, _lib.QRB200_F16):
+        for xs, ws in ((16, None), (None, 16), (16, 16)):
+            assert L.qrb200_linear(16, 8, 16, 8, 0, xs, ws, None, None, 0, 16, 4, None, m, 4, 8, t, t, 0, None, 0, None) == bad
+    with pytest.raises(ValueError):
+        qrb200.linear(meta(m, 8), meta(4, 8), weight_scale=F32_4)
