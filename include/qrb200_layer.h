@@ -31,7 +31,8 @@ extern "C" {
  *   weight   [dim], `dtype` or F32, or NULL for ones
  *   residual [rows][dim], `stream_dtype` (= `dtype`, or F32), or NULL
  *   y        [rows][dim] contiguous; out_dtype = `dtype`, or E4M3: then scale[rows] is written too,
- *            scale = max(max |y| / 448, 2^-126) of the row, y = e4m3(y / scale)
+ *            scale = max(max |y| / 448, 2^-126) of the row, y = e4m3(y / scale), in float32 as
+ *            y (1 / scale): beside the middle between two codes either may be taken
  *   h        [rows][dim] contiguous, `stream_dtype`; may be `residual` itself (in place, ldr = dim);
  *            not written (may be NULL) without a residual
  * A NaN in a row makes its y (and scale) NaN. */

@@ -4,7 +4,9 @@
 //                           what is kept, so a backward pass or a later layer that reads h sees
 //                           the numbers y was made from
 //   r = (mean_j h_j^2 + eps)^-1/2,   y_j = h_j r w_j
-//   8 bits: s = max(max_j |y_j| / 448, 2^-126),  q_j = e4m3(y_j / s)
+//   8 bits: s = max(max_j |y_j| / 448, 2^-126),  q_j = e4m3(y_j / s), computed as r max |h w| / 448 and
+//           y_j (1 / s): one reduction less and no division an element, for a rounding of float32 that
+//           an e4m3 code shows only beside the middle between two of them
 // and, with g = dy w and c = r^3 / D sum_j g_j h_j,
 //   dx = dresidual = dh + r g - c h,      dw_j = sum_rows dy_j h_j r.
 // All sums, r, s and c are float32; every output is rounded once, when it is stored.

@@ -4,7 +4,8 @@
 // torch.ops, 1.5 us went into finding the operator by its schema.  These two functions take their
 // arguments straight from Python instead.  They answer only for plain CUDA tensors with nothing else
 // listening (no tensor subclass, no dispatch or function mode, no functorch transform); for anything
-// else they return NotImplemented, and the caller takes torch.ops, which every such feature knows.
+// else (under torch.inference_mode(), which excludes autograd's keys, too) they return NotImplemented, and
+// the caller takes torch.ops, which every such feature knows.
 #include <Python.h>
 
 #include <ATen/PythonTorchFunctionTLS.h>
