@@ -229,7 +229,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_backward(const at::Tenso
   const Rows rg = as_rows(dy), rh = as_rows(h), rd = dh ? as_rows(*dh) : Rows{{}, 0, 0, 0};
   at::Tensor dx, dres, dw;
   if (want_dx || (want_dresidual && ht == xt)) dx = fresh(dy.sizes(), dy, xt);
-  if (want_dresidual) dres = ht == xt ? dx : fresh(dy.sizes(), dy, ht);
+  if (want_dresidual && ht != xt) dres = fresh(dy.sizes(), dy, ht);  // dx is it otherwise: no two outputs share memory
   if (want_dweight) dw = fresh(w.sizes(), dy, w.scalar_type());
   if (dy.is_meta()) return {dx, dres, dw};
   size_t bytes = 0;
@@ -237,7 +237,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_backward(const at::Tenso
   at::Tensor ws;
   if (bytes) ws = fresh({(int64_t)bytes}, dy, at::kByte);
   check_rc(qrb200_rms_norm_backward(rg.t.data_ptr(), rg.ld, rh.t.data_ptr(), rh.ld, ptr(rd.t), rd.ld, ptr(w),
-                                    w.defined() ? layer_code(w.scalar_type()) : 0, ptr(dx), ht == xt ? nullptr : ptr(dres),
+                                    w.defined() ? layer_code(w.scalar_type()) : 0, ptr(dx), ptr(dres),
                                     ptr(dw), rg.rows, rg.d, (float)eps, layer_code(xt), layer_code(ht), ptr(ws), bytes,
                                     cur_stream(dy)),
            "qrb200_rms_norm_backward");
@@ -458,6 +458,7 @@ struct RmsNormGrad : torch::autograd::Function<RmsNormGrad> {
     }
     auto [dx, dres, dw] =
         rms_norm_backward_below(dy, h, given(dh), given(weight), ctx->saved_data["eps"].toDouble(), want_x, want_r, want_w);
+    if (want_r && !dres.defined()) dres = dx;
     return {want_x ? dx : at::Tensor(), dw, dres, at::Tensor()};
   }
 };

@@ -175,6 +175,24 @@ def test_the_first_call_may_be_a_compiled_one():
     assert done.returncode == 0, done.stderr[-2000:]
 
 
+def test_outputs_share_no_memory():
+    """The residual's gradient is dx itself where the types are the same: the operator returns it once, because what
+    compiles a program may write over one output while it still needs the other."""
+    qrb200.api.load_torch_ops()
+    op = torch.ops.qrb200.rms_norm_backward
+    for want_dx in (False, True):
+        dx, dres, dw = op(meta(2, 8), meta(2, 8), None, meta(8), 1e-6, want_dx, True, True)
+        assert dx.shape == (2, 8) and dres is None and dw.shape == (8,)
+        dx, dres, _ = op(meta(2, 8), meta(2, 8, dtype=torch.float32), None, meta(8), 1e-6, want_dx, True, True)
+        assert (dx is not None) == want_dx and dres.dtype == torch.float32
+    x, r = meta(2, 8).requires_grad_(), meta(2, 8).requires_grad_()
+    y, h = qrb200.rms_norm(x, residual=r)
+    dx, dr = torch.autograd.grad(y.sum() + h.sum(), (x, r))
+    assert dx.shape == dr.shape == (2, 8)
+    y, h = qrb200.rms_norm(meta(2, 8), residual=r)
+    assert torch.autograd.grad(y.sum(), r)[0].shape == (2, 8)
+
+
 # ---------------------------------------------------------------------- derivatives there are not
 
 def tangents(call, *shapes, dual):

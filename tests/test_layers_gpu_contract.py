@@ -345,3 +345,34 @@ def test_norm_of_strided_rows(rows, dim, fp8, dtype):
                 a, b = got[0].double(), plain[0].double()
                 tol = 2 * ({BF: 2.0 ** -8, F32: 2.0 ** -24}[dtype] + 2.0 ** -18) * (1 + 2.0 ** -7) * b.abs() + 2.0 ** -133
             assert bool(((a - b).abs() <= tol).all())
+
+
+# ---------------------------------------------------------------------- the operators' registration
+
+@pytest.mark.parametrize("kept", [BF, F32])
+def test_operators_keep_their_schemas(kept):
+    """Torch's own checks of an operator: no output shares memory with an input or another output, the meta kernel agrees
+    with the CUDA one, and a compiled step gives what the operator gives."""
+    from qrb200 import _lib
+    q().api.load_torch_ops()
+    ops, grad = torch.ops.qrb200, lambda *ts: [t.clone().requires_grad_() for t in ts]  # noqa: E731
+    x, g, r, w, b = (rnd(5, 64, dtype=BF, seed=1), rnd(64, dtype=BF, seed=2), rnd(5, 64, dtype=kept, seed=3), rnd(40, 64, dtype=BF, seed=4),
+                     rnd(40, dtype=BF, seed=5))
+    dy, dh, dz = rnd(5, 64, dtype=BF, seed=6), rnd(5, 64, dtype=kept, seed=7), rnd(5, 40, dtype=BF, seed=8)
+    slope = ops.linear(x, w, b, None, _lib.ACT_SILU, None, None, None, True)[1]
+    for op, args in ((ops.rms_norm, (x, g, r, 1e-6, None)), (ops.rms_norm, (*grad(x, g, r), 1e-6, None)), (ops.rms_norm, (x, None, None, 1e-6, FP8)),
+                     (ops.rms_norm_backward, (dy, r, dh, g, 1e-6, True, True, True)),
+                     (ops.rms_norm_backward, (dy, r, None, None, 1e-6, False, True, False)),
+                     (ops.quantize_rows, (r,)),
+                     (ops.linear, (x, w, b, None, _lib.ACT_GELU, None, None, None, True)),
+                     (ops.linear, (*grad(x, w, b), None, _lib.ACT_GELU, None, None, None, False)),
+                     (ops.linear_backward, (dz, slope, x, w, True, True, True)), (ops.linear_backward, (dz, None, x, w, False, True, False))):
+        torch.library.opcheck(op.default, args)
+    # the same numbers by way of autograd, with the residual's gradient where it is dx and where it is not
+    xg, rg = grad(x, r)
+    y, h = q().rms_norm(xg, g, residual=rg)
+    dx, dr = torch.autograd.grad((y, h), (xg, rg), (dy, dh))
+    want = ops.rms_norm_backward(dy, h.detach(), dh, g, 1e-6, True, True, False)
+    assert torch.equal(dx, want[0]) and torch.equal(dr, want[0] if kept == BF else want[1])
+    dr, = torch.autograd.grad(q().rms_norm(x, g, residual=rg), rg, (dy, dh))
+    assert torch.equal(dr, want[0] if kept == BF else want[1])
